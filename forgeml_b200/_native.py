@@ -77,11 +77,28 @@ class neb_fusion(ctypes.Structure):
     ]
 
 
+class neb_kv4_pool(ctypes.Structure):
+    """One layer's 4-bit key/value pool (include/forgeml_b200.h)."""
+
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p),
+        ("v_codes", ctypes.c_void_p),
+        ("k_params", ctypes.c_void_p),
+        ("v_params", ctypes.c_void_p),
+        ("slots", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("max_seq", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
 _F = ctypes.c_float
 _S4 = ctypes.POINTER(ctypes.c_int64)
+_KV4 = ctypes.POINTER(neb_kv4_pool)
 
 _SIGNATURES = {
     "fml_gemm_workspace_size": (
@@ -119,6 +136,11 @@ _SIGNATURES = {
     ),
     "neb_attention": (_I, [_P, _S4, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _F, _I, _P]),
     "neb_kv_append": (_I, [_P, _S4, _P, _S4, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _P]),
+    "neb_kv4_codes_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64]),
+    "neb_kv4_params_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64, _I]),
+    "neb_kv4_append": (_I, [_P, _S4, _P, _S4, _KV4, _P, _P, _I64, _I64, _P]),
+    "neb_kv4_read": (_I, [_KV4, _P, _P, _I64, _P, _P, _I64, _P]),
+    "neb_kv4_attention": (_I, [_P, _S4, _KV4, _P, _P, _P, _I64, _I64, _I64, _F, _P]),
     "neb_embed": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _P]),
     "neb_argmax": (_I, [_P, _I64, _I64, _I64, _P, _I, _P]),
     "neb_add": (_I, [_P, _P, _P, _I64, _I, _P]),

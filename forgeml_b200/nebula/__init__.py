@@ -1,6 +1,6 @@
 """Nebula tensor-/pipeline-parallel decoding on sm_100a kernels (drop-in for `nebula`)."""
 
-from forgeml_b200.nebula.cache import CacheError, KVCache
+from forgeml_b200.nebula.cache import CacheError, KV4Pool, KVCache
 from forgeml_b200.nebula.model import DecoderConfig, TinyDecoder
 from forgeml_b200.nebula.parallel import ParallelContext
 from forgeml_b200.nebula.engine import Engine, EngineFailed
@@ -15,6 +15,7 @@ __all__ = [
     "DecoderConfig",
     "Engine",
     "EngineFailed",
+    "KV4Pool",
     "KVCache",
     "ParallelContext",
     "ShardedDecoder",

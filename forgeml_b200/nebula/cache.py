@@ -23,13 +23,20 @@ message texts.  The storage is designed for the decode kernels instead:
 ``append`` keeps the reference's contract (write [B, heads, T, hd] at
 ``start_pos``, return the stacked prefixes [B, heads, end, hd] as a copy) for
 callers of the reference API; the decoder itself never uses it.
+
+``kv_bits=4`` holds each layer's rows in a ``KV4Pool`` (``kv4_pool``) instead
+of ``k_pool`` / ``v_pool``; ``append`` then returns the prefixes as the numbers
+the quantised rows stand for.
 """
 
 from __future__ import annotations
 
+import ctypes
 import heapq
 
 import torch
+
+from forgeml_b200 import _native
 
 
 class CacheError(RuntimeError):
@@ -72,9 +79,55 @@ class _Ticket:
             self.set_all(end)
 
 
+class KV4Pool:
+    """Keys and values of one layer in 4 bits: ``slots`` requests of up to
+    ``max_seq_len`` positions, ``heads`` key/value heads of ``head_dim``
+    numbers (at most 256) of ``dtype``.
+
+    Per group of 32 channels a row keeps the minimum and a step in ``dtype``
+    and a 4-bit code per channel: 4.5 to 5 bits a number for 16-bit types at
+    the usual head sizes (2 bytes of codes and 4 bytes of parameters per 4 and
+    32 channels), against 16.  The format is stated in
+    include/forgeml_b200.h; ``ops.kv4_append`` writes rows, ``ops.kv4_read``
+    gives them back as numbers and ``ops.kv4_attention`` attends over them in
+    place.  Rows never written hold whatever the memory held."""
+
+    def __init__(self, *, slots: int, heads: int, max_seq_len: int, head_dim: int, device: torch.device,
+                 dtype: torch.dtype):
+        sizes = {"slots": slots, "heads": heads, "max_seq_len": max_seq_len, "head_dim": head_dim}
+        bad = next((k for k, v in sizes.items() if not _plain_int(v) or v <= 0), None)
+        if bad is not None:
+            raise CacheError(f"{bad} must be a positive integer")
+        if head_dim > 256:
+            raise CacheError("the 4-bit cache supports head_dim <= 256")
+        if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise CacheError(f"dtype {dtype} is not supported by the 4-bit cache")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise CacheError("the 4-bit cache is written and read by the sm_100a kernels and needs a CUDA device")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.slots, self.heads, self.max_seq_len, self.head_dim = slots, heads, max_seq_len, head_dim
+        self.device, self.dtype = device, dtype
+        groups, rows = -(-head_dim // 32), -(-max_seq_len // 16) * 16
+        codes, params = (slots, heads, rows, 16 * groups), (slots, heads, rows, groups, 2)
+        self.k_codes = torch.empty(codes, device=device, dtype=torch.uint8)
+        self.v_codes = torch.empty(codes, device=device, dtype=torch.uint8)
+        self.k_params = torch.empty(params, device=device, dtype=dtype)
+        self.v_params = torch.empty(params, device=device, dtype=dtype)
+        self._struct = _native.neb_kv4_pool(
+            self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_params.data_ptr(), self.v_params.data_ptr(),
+            slots, heads, max_seq_len, head_dim, _native.dtype_code(dtype))
+        self.handle = ctypes.byref(self._struct)
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k_codes, self.v_codes, self.k_params, self.v_params))
+
+
 class KVCache:
     def __init__(self, *, layer_ids: tuple[int, ...], num_heads: int, head_dim: int, max_seq_len: int,
-                 max_requests: int, device: torch.device, dtype: torch.dtype):
+                 max_requests: int, device: torch.device, dtype: torch.dtype, kv_bits: int | None = None):
         sizes = {"num_heads": num_heads, "head_dim": head_dim, "max_seq_len": max_seq_len,
                  "max_requests": max_requests}
         bad = next((k for k, v in sizes.items() if not _plain_int(v) or v <= 0), None)
@@ -87,13 +140,19 @@ class KVCache:
             raise CacheError("device must be a torch.device")
         if not isinstance(dtype, torch.dtype):
             raise CacheError("dtype must be a torch.dtype")
+        if kv_bits is not None and (not _plain_int(kv_bits) or kv_bits != 4):
+            raise CacheError("kv_bits must be None (the cache's dtype) or 4")
         self.layer_ids = ids
         self.num_heads, self.head_dim = num_heads, head_dim
         self.max_seq_len, self.max_requests = max_seq_len, max_requests
         self.device, self.dtype = device, dtype
+        self.kv_bits = kv_bits
+        wide = ids if kv_bits is None else ()
         pool_shape = (max_requests, num_heads, max_seq_len, head_dim)
-        self.k_pool = {lid: torch.empty(pool_shape, device=device, dtype=dtype) for lid in ids}
-        self.v_pool = {lid: torch.empty(pool_shape, device=device, dtype=dtype) for lid in ids}
+        self.k_pool = {lid: torch.empty(pool_shape, device=device, dtype=dtype) for lid in wide}
+        self.v_pool = {lid: torch.empty(pool_shape, device=device, dtype=dtype) for lid in wide}
+        self.kv4_pool = {lid: KV4Pool(slots=max_requests, heads=num_heads, max_seq_len=max_seq_len, head_dim=head_dim,
+                                      device=device, dtype=dtype) for lid in ids if kv_bits == 4}
         self._tickets: dict[int, _Ticket] = {}
         self._free_slots = list(range(max_requests))  # min-heap: the lowest free slot goes first
         # the last request-id tuple check_ids accepted: a decode loop passes
@@ -207,6 +266,16 @@ class KVCache:
         and return the stacked prefixes [B, heads, start_pos+T, hd] (a copy)."""
         tickets = self._check_append(layer_id, request_ids, key, value, start_pos)
         end = start_pos + key.shape[2]
+        if self.kv_bits == 4:
+            from forgeml_b200.nebula import ops
+
+            pool = self.kv4_pool[layer_id]
+            slot_t = torch.tensor([tk.slot for tk in tickets], dtype=torch.int32, device=pool.device)
+            ops.kv4_append(key.transpose(1, 2), value.transpose(1, 2), pool, slot_t,
+                           torch.full_like(slot_t, start_pos))
+            for tk in tickets:
+                tk.set_layer(self.layer_ids, layer_id, end)
+            return ops.kv4_read(pool, slot_t, end)
         kp, vp = self.k_pool[layer_id], self.v_pool[layer_id]
         if self.device.type == "cuda":
             from forgeml_b200.nebula import ops
@@ -225,7 +294,7 @@ class KVCache:
         return kp.index_select(0, index)[:, :, :end], vp.index_select(0, index)[:, :, :end]
 
     def _check_append(self, layer_id, request_ids, key, value, start_pos) -> list[_Ticket]:
-        if layer_id not in self.k_pool:
+        if layer_id not in self.layer_ids:
             raise CacheError(f"layer {layer_id} not owned by this cache")
         tickets = self._tickets_of(request_ids)
         if not isinstance(key, torch.Tensor) or not isinstance(value, torch.Tensor):

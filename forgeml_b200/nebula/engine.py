@@ -295,11 +295,14 @@ class Engine:
     the decoder; the default is the native ``ShardedDecoder`` (with ``init``).
     Protocol tests on CPU (Gloo) inject a CPU decoder here; the product path
     has no CPU decoder.
+
+    ``kv_bits=4`` holds the KV cache in 4 bits (``cache.KV4Pool``) instead of
+    ``dtype``; every rank of a job passes the same value.
     """
 
     def __init__(self, config: DecoderConfig = _DEFAULT_CONFIG, *, context: ParallelContext | None = None,
                  dtype: torch.dtype = torch.float32, max_requests: int = 32, decoder_factory=None,
-                 init: str = "reference"):
+                 init: str = "reference", kv_bits: int | None = None):
         self._owns_context = context is None
         if context is None:
             context = ParallelContext.from_env(device="cuda" if torch.cuda.is_available() else "cpu")
@@ -309,19 +312,25 @@ class Engine:
             raise ValueError(f"unsupported dtype {dtype}")
         if context.device.type != "cuda" and dtype != torch.float32:
             raise ValueError("low-precision dtype requires CUDA")
+        if kv_bits is not None and (not _plain_int(kv_bits) or kv_bits != 4):
+            raise ValueError("kv_bits must be None (the cache in dtype) or 4")
+        if kv_bits is not None and context.device.type != "cuda":
+            raise ValueError("a quantised cache requires CUDA")
         self.config, self.context, self.max_requests = config, context, max_requests
         nccl = dist.is_available() and dist.is_initialized() and dist.get_backend() == "nccl"
         self._multi = context.world_size > 1 and dist.is_available() and dist.is_initialized()
         wire_device = context.device if nccl else torch.device("cpu")
         self._wire = _CommandWire(max_requests, config.max_seq_len, wire_device)
         if self._multi:
-            self._handshake(dtype)
+            self._handshake(dtype, kv_bits)
         if decoder_factory is None:
             from forgeml_b200.nebula.runtime import ShardedDecoder
 
-            self.decoder = ShardedDecoder(config, context, dtype=dtype, max_requests=max_requests, init=init)
+            self.decoder = ShardedDecoder(config, context, dtype=dtype, max_requests=max_requests, init=init,
+                                          kv_bits=kv_bits)
         else:
-            self.decoder = decoder_factory(config, context, dtype=dtype, max_requests=max_requests)
+            more = {} if kv_bits is None else {"kv_bits": kv_bits}
+            self.decoder = decoder_factory(config, context, dtype=dtype, max_requests=max_requests, **more)
         self._health = _StepHealth(context.device)
         self._healthy = True
         self._closed = False
@@ -334,10 +343,12 @@ class Engine:
         self.pipelined_prefill = context.pp_size > 1
         self._next_generated_id = _GENERATE_ID_BASE
 
-    def _handshake(self, dtype: torch.dtype) -> None:
-        """Every rank must hold the same configuration, dtype and capacity
-        (SHA-256 of their repr, first 8 bytes as a little-endian int64)."""
-        digest = hashlib.sha256(repr((asdict(self.config), str(dtype), self.max_requests)).encode()).digest()
+    def _handshake(self, dtype: torch.dtype, kv_bits: int | None) -> None:
+        """Every rank must hold the same configuration, dtype, capacity and
+        cache format (SHA-256 of their repr, first 8 bytes as a little-endian
+        int64; a cache in dtype adds nothing to the repr)."""
+        held = (asdict(self.config), str(dtype), self.max_requests) + (() if kv_bits is None else (kv_bits,))
+        digest = hashlib.sha256(repr(held).encode()).digest()
         mine = int.from_bytes(digest[:8], "little", signed=True)
         word = torch.tensor([mine], dtype=torch.int64, device=self._wire.device)
         self._wire.broadcast(word)

@@ -2,10 +2,13 @@
 
 All take device tensors, launch on the current stream of their device and
 raise on a nonzero status; none allocates except where an output is created.
+The kv4_* wrappers (cache in 4 bits, ``cache.KV4Pool``) also check their
+arguments (ValueError) and select the pool's device.
 """
 
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -40,6 +43,115 @@ def attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, slot_
         slot_of.data_ptr(), start_pos.data_ptr(), out.data_ptr(), b, t, h, d, k_pool.shape[2], k_pool.shape[0],
         1.0 / math.sqrt(d), _native.dtype_code(q.dtype), _stream(q),
     )
+    return out
+
+
+def _on_device(device: torch.device):
+    return torch.cuda.device(device) if torch.cuda.current_device() != device.index else contextlib.nullcontext()
+
+
+def _kv4_tables(pool, slot_of: torch.Tensor, start_pos: torch.Tensor | None, batch: int | None = None) -> int:
+    """Check a batch's slot and position tables; returns the batch size."""
+    for name, t in (("slot_of", slot_of), ("start_pos", start_pos)):
+        if t is None and name == "start_pos":
+            continue
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous 1-D int32 tensor")
+        if t.device != pool.device:
+            raise ValueError(f"{name} must be on the pool's device")
+        if batch is None:
+            batch = t.shape[0]
+        if t.shape[0] != batch:
+            raise ValueError(f"{name} must hold one entry per request")
+    if batch == 0:
+        raise ValueError("the batch must not be empty")
+    return batch
+
+
+def _kv4_rows(pool, name: str, x: torch.Tensor) -> torch.Tensor:
+    if not isinstance(x, torch.Tensor) or x.dim() != 4:
+        raise ValueError(f"{name} must be a tensor [B, T, heads, head_dim]")
+    if x.device != pool.device or x.dtype != pool.dtype:
+        raise ValueError(f"{name} must match the pool's device and dtype")
+    if x.shape[1] == 0 or x.shape[3] != pool.head_dim:
+        raise ValueError(f"bad {name} shape {tuple(x.shape)}")
+    if x.stride(3) != 1 and pool.head_dim > 1:
+        raise ValueError(f"{name} needs unit stride in the head dimension")
+    return x
+
+
+def _kv4_strides(x: torch.Tensor):
+    return _native.strides4((x.stride(0), x.stride(1), x.stride(2), 1))
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, pool, slot_of: torch.Tensor, start_pos: torch.Tensor) -> None:
+    """Quantise k and v [B,T,H,D] (views with unit innermost stride) into rows
+    start_pos[b] .. start_pos[b]+T-1 of slot slot_of[b] of a ``KV4Pool``.
+
+    The requests of a batch hold distinct slots: where a later request's rows
+    overlap an earlier one's in the same slot, the earlier one's are kept and
+    the device error word's bit 4 is raised, as for a slot or position outside
+    the pool, whose rows are not written."""
+    b = _kv4_tables(pool, slot_of, start_pos)
+    for name, x in (("k", k), ("v", v)):
+        _kv4_rows(pool, name, x)
+        if x.shape[0] != b or x.shape[1] != k.shape[1] or x.shape[2] != pool.heads:
+            raise ValueError(f"bad {name} shape {tuple(x.shape)}")
+    t = k.shape[1]
+    if t > pool.max_seq_len:
+        raise ValueError("more rows than the pool's max_seq_len")
+    with _on_device(pool.device):
+        _native.call("neb_kv4_append", k.data_ptr(), _kv4_strides(k), v.data_ptr(), _kv4_strides(v), pool.handle,
+                     slot_of.data_ptr(), start_pos.data_ptr(), b, t, _stream(k))
+
+
+def kv4_read(pool, slot_of: torch.Tensor, count: int, *, start_pos: torch.Tensor | None = None,
+             out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The numbers that rows start_pos[b] .. start_pos[b]+count-1 (from row 0
+    without ``start_pos``) of slot slot_of[b] stand for, rounded to the pool's
+    dtype: keys and values [B,H,count,D].  Rows of a slot or position outside
+    the pool come back as zeros and raise the device error word's bit 4."""
+    b = _kv4_tables(pool, slot_of, start_pos)
+    if not isinstance(count, int) or isinstance(count, bool) or not 0 < count <= pool.max_seq_len:
+        raise ValueError("count must be an integer in 1..max_seq_len")
+    shape = (b, pool.heads, count, pool.head_dim)
+    if out is None:
+        out = tuple(torch.empty(shape, dtype=pool.dtype, device=pool.device) for _ in range(2))
+    ko, vo = out
+    for x in (ko, vo):
+        if not isinstance(x, torch.Tensor) or tuple(x.shape) != shape or x.dtype != pool.dtype \
+                or x.device != pool.device or not x.is_contiguous():
+            raise ValueError(f"out must be two contiguous {shape} tensors of the pool's dtype and device")
+    with _on_device(pool.device):
+        _native.call("neb_kv4_read", pool.handle, slot_of.data_ptr(),
+                     start_pos.data_ptr() if start_pos is not None else None, count, ko.data_ptr(), vo.data_ptr(), b,
+                     _stream(ko))
+    return ko, vo
+
+
+def kv4_attention(q: torch.Tensor, pool, slot_of: torch.Tensor, start_pos: torch.Tensor,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """Masked attention of q [B,T,QH,D] over the quantised prefix: query t of
+    request b sits at position start_pos[b]+t and attends rows 0 up to its own.
+    QH is a multiple of the pool's heads; query head h reads head
+    h // (QH // heads).  Returns [B,T,QH*D]; scores, softmax and sums in fp32.
+    A slot or position outside the pool gives zeros and raises the device
+    error word's bit 4."""
+    b = _kv4_tables(pool, slot_of, start_pos)
+    _kv4_rows(pool, "q", q)
+    _, t, qh, d = q.shape
+    if q.shape[0] != b or qh == 0 or qh % pool.heads:
+        raise ValueError(f"bad q shape {tuple(q.shape)}")
+    if t > pool.max_seq_len:
+        raise ValueError("more rows than the pool's max_seq_len")
+    if out is None:
+        out = torch.empty((b, t, qh * d), dtype=q.dtype, device=q.device)
+    elif tuple(out.shape) != (b, t, qh * d) or out.dtype != q.dtype or out.device != q.device \
+            or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {(b, t, qh * d)} tensor of q's dtype and device")
+    with _on_device(pool.device):
+        _native.call("neb_kv4_attention", q.data_ptr(), _kv4_strides(q), pool.handle, slot_of.data_ptr(),
+                     start_pos.data_ptr(), out.data_ptr(), b, t, qh, 1.0 / math.sqrt(d), _stream(q))
     return out
 
 

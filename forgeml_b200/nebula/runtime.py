@@ -138,10 +138,16 @@ class ShardedDecoder(nn.Module):
     init="normal": every weight matrix ~ N(0, init_std) drawn on the device
     from per-tensor seeded generators (each rank draws the full tensor and
     keeps its shard, so shards agree); LayerNorm gamma=1, beta=0.
+
+    kv_bits=4: the cache holds its rows in 4 bits (cache.KV4Pool).  A layer's
+    K/V columns then leave the QKV product with the queries and are quantised
+    by neb_kv4_append before neb_kv4_attention reads them (the GEMM epilogue
+    writes rows of the model dtype only).
     """
 
     def __init__(self, config: DecoderConfig, context: ParallelContext, *, dtype: torch.dtype = torch.float32,
-                 max_requests: int = 32, init: str = "reference", init_std: float = 0.02):
+                 max_requests: int = 32, init: str = "reference", init_std: float = 0.02,
+                 kv_bits: int | None = None):
         super().__init__()
         tp, pp = context.tp_size, context.pp_size
         if config.num_heads % tp:
@@ -214,7 +220,8 @@ class ShardedDecoder(nn.Module):
         if self.is_last:
             self.head_gemm = _linear(self.head, self.workspace)
         self.cache = KVCache(layer_ids=self.owned_layer_ids, num_heads=self.num_heads_local, head_dim=self.head_dim,
-                             max_seq_len=config.max_seq_len, max_requests=max_requests, device=dev, dtype=dtype)
+                             max_seq_len=config.max_seq_len, max_requests=max_requests, device=dev, dtype=dtype,
+                             kv_bits=kv_bits)
         self._hl_hd = hl_hd
         self._graphs: dict[int, dict] = {}
         self._deferred: list[torch.Tensor] = []  # logits awaiting flush_deferred()
@@ -280,20 +287,26 @@ class ShardedDecoder(nn.Module):
         h = self.config.hidden_size
         hl, hd, hl_hd = self.num_heads_local, self.head_dim, self._hl_hd
         dev = x.device
-        kp, vp = self.cache.k_pool[lid], self.cache.v_pool[lid]
         ln_mode = self.decode_ln
+        kv4 = self.cache.kv_bits == 4
+        if kv4:  # q, k and v columns leave the product; kv4_append quantises the rows
+            kv, width = None, 3 * hl_hd
+        else:
+            kp, vp = self.cache.k_pool[lid], self.cache.v_pool[lid]
+            kv, width = (kp, vp, slots, starts, hl_hd, t), hl_hd
+        out = torch.empty((bt, width), dtype=self.dtype, device=dev)
         if ln_mode == "fold":
             lin, wsum, wbias = L.qkv_ln
-            q = lin.fused(x, torch.empty((bt, hl_hd), dtype=self.dtype, device=dev), ln_fold=(wsum, wbias, 1e-5),
-                          kv=(kp, vp, slots, starts, hl_hd, t))
+            q = lin.fused(x, out, ln_fold=(wsum, wbias, 1e-5), kv=kv)
         elif ln_mode == "prologue":
-            q = L.qkv.fused(x, torch.empty((bt, hl_hd), dtype=self.dtype, device=dev), ln=(L.ln1_w, L.ln1_b, 1e-5),
-                            kv=(kp, vp, slots, starts, hl_hd, t))
+            q = L.qkv.fused(x, out, ln=(L.ln1_w, L.ln1_b, 1e-5), kv=kv)
         else:
             h1 = _ln(x, L.ln1_w, L.ln1_b, torch.empty_like(x), bt)
-            q = L.qkv.fused(h1, torch.empty((bt, hl_hd), dtype=self.dtype, device=dev),
-                            kv=(kp, vp, slots, starts, hl_hd, t))
-        attn = ops.attention(q.view(b, t, hl, hd), kp, vp, slots, starts).view(bt, hl_hd)
+            q = L.qkv.fused(h1, out, kv=kv)
+        if kv4:
+            attn = self._kv4_attend(q, lid, b, t, slots, starts)
+        else:
+            attn = ops.attention(q.view(b, t, hl, hd), kp, vp, slots, starts).view(bt, hl_hd)
         tp = self.context.tp_size
         if tp == 1:  # residual add in the plain epilogue
             x = L.o(attn, torch.empty((bt, h), dtype=self.dtype, device=dev), residual=x)
@@ -319,6 +332,16 @@ class ShardedDecoder(nn.Module):
                                 ar_ctx=ar.handle)
         return self._tp_sum_add(L.down(mid, torch.empty((bt, h), dtype=self.dtype, device=dev)), x, ar)
 
+    def _kv4_attend(self, qkv: torch.Tensor, lid: int, b: int, t: int, slots: torch.Tensor,
+                    starts: torch.Tensor) -> torch.Tensor:
+        """Quantise the K/V columns of qkv [b*t, 3*h_local*hd] into the layer's
+        4-bit pool and attend over it: [b*t, h_local*hd]."""
+        pool = self.cache.kv4_pool[lid]
+        q, k, v = qkv.view(b, t, 3, self.num_heads_local, self.head_dim).unbind(2)
+        with record_function("nebula::kv_append"):
+            ops.kv4_append(k, v, pool, slots, starts)
+        return ops.kv4_attention(q, pool, slots, starts).view(b * t, self._hl_hd)
+
     def _layer(self, L: _Layer, lid: int, x: torch.Tensor, b: int, t: int, slots: torch.Tensor,
                starts: torch.Tensor, ar) -> torch.Tensor:
         ctx = self.context
@@ -331,12 +354,15 @@ class ShardedDecoder(nn.Module):
         dev = x.device
         h1 = _ln(x, L.ln1_w, L.ln1_b, torch.empty_like(x), bt)
         qkv = L.qkv(h1, torch.empty((bt, 3 * hl_hd), dtype=self.dtype, device=dev))
-        q = qkv[:, :hl_hd].view(b, t, hl, hd)
-        k = qkv[:, hl_hd:2 * hl_hd].view(b, t, hl, hd)
-        v = qkv[:, 2 * hl_hd:].view(b, t, hl, hd)
-        with record_function("nebula::kv_append"):
-            ops.kv_append(k, v, self.cache.k_pool[lid], self.cache.v_pool[lid], slots, starts)
-        attn = ops.attention(q, self.cache.k_pool[lid], self.cache.v_pool[lid], slots, starts).view(bt, hl_hd)
+        if self.cache.kv_bits == 4:
+            attn = self._kv4_attend(qkv, lid, b, t, slots, starts)
+        else:
+            q = qkv[:, :hl_hd].view(b, t, hl, hd)
+            k = qkv[:, hl_hd:2 * hl_hd].view(b, t, hl, hd)
+            v = qkv[:, 2 * hl_hd:].view(b, t, hl, hd)
+            with record_function("nebula::kv_append"):
+                ops.kv_append(k, v, self.cache.k_pool[lid], self.cache.v_pool[lid], slots, starts)
+            attn = ops.attention(q, self.cache.k_pool[lid], self.cache.v_pool[lid], slots, starts).view(bt, hl_hd)
         if ctx.tp_size == 1:
             x = L.o(attn, torch.empty((bt, h), dtype=self.dtype, device=dev), residual=x)
         else:

@@ -230,6 +230,59 @@ FML_API int neb_kv_append(const void* k, const int64_t k_strides[4],
                   int64_t max_seq, int dtype, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * 4-bit key/value cache (no counterpart in the reference, whose cache holds
+ * the model dtype, src/nebula/cache.py:62-89).  A row is one position of one
+ * key/value head.  Its head_dim numbers form groups of 32 channels (the last
+ * may be shorter); a group keeps its minimum z, the step
+ * s = dtype((max - z) / 15) and for each number x the code
+ * c = rint((x - z) / s) in 0..15 (ties to even; 0 where s is 0), and stands
+ * for z + c * s.  A group that holds an infinity or a NaN reads back as NaN.
+ *
+ * One layer's pool: codes [slots, heads, rows, 16 G] bytes and params
+ * [slots, heads, rows, G, 2] (s, z) in dtype, for keys and for values, with
+ * G = ceil(head_dim / 32) and rows = max_seq rounded up to 16; each tensor
+ * 16-byte aligned, neb_kv4_codes_bytes / neb_kv4_params_bytes long.  The
+ * order of the codes within a row is the kernels' own.
+ *
+ * Request b of a batch holds slot slot_of[b] (int32, device) and its rows
+ * begin at start_pos[b] (int32, device).  A slot or position outside the pool
+ * raises bit 4 of fml_device_status(); nothing is written for it (append) and
+ * its outputs are zeros (read, attention).  head_dim <= 256.
+ * ------------------------------------------------------------------------- */
+typedef struct neb_kv4_pool {
+  void* k_codes;
+  void* v_codes;
+  void* k_params;
+  void* v_params;
+  int64_t slots, heads, max_seq, head_dim;
+  int32_t dtype;
+} neb_kv4_pool;
+
+FML_API size_t neb_kv4_codes_bytes(int64_t slots, int64_t heads, int64_t max_seq, int64_t head_dim);
+FML_API size_t neb_kv4_params_bytes(int64_t slots, int64_t heads, int64_t max_seq, int64_t head_dim, int dtype);
+/* Quantise k and v [B,T,H,D] (dtype of the pool, element strides, innermost 1)
+ * into rows start_pos[b] .. start_pos[b]+T-1.  The requests of a batch hold
+ * distinct slots; where a later one's rows overlap an earlier one's in the
+ * same slot, the earlier one's are kept and bit 4 is raised. */
+FML_API int neb_kv4_append(const void* k, const int64_t k_strides[4],
+                   const void* v, const int64_t v_strides[4],
+                   const neb_kv4_pool* pool, const int32_t* slot_of, const int32_t* start_pos,
+                   int64_t batch, int64_t t, void* stream);
+/* k_out / v_out [B,H,count,D] (contiguous, dtype of the pool) = what rows
+ * start_pos[b] .. start_pos[b]+count-1 stand for, rounded to dtype within its finite range;
+ * start_pos NULL reads from 0. */
+FML_API int neb_kv4_read(const neb_kv4_pool* pool, const int32_t* slot_of, const int32_t* start_pos,
+                 int64_t count, void* k_out, void* v_out, int64_t batch, void* stream);
+/* Attention over the pool: query t of request b sits at start_pos[b] + t and
+ * attends rows 0 .. start_pos[b]+t.  q is [B,T,q_heads,D] (dtype of the pool,
+ * element strides, innermost 1), q_heads a multiple of the pool's heads: query
+ * head h reads head h / (q_heads / heads).  out is [B,T,q_heads*D] contiguous.
+ * Scores, softmax and the sums over the rows in fp32. */
+FML_API int neb_kv4_attention(const void* q, const int64_t q_strides[4], const neb_kv4_pool* pool,
+                      const int32_t* slot_of, const int32_t* start_pos, void* out,
+                      int64_t batch, int64_t t, int64_t q_heads, float scale, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Token + learned position embedding:
  *   x[b,t,:] = r( tok_emb[tokens[b,t],:] + pos_emb[start_pos[b]+t,:] )
  * Replaces src/nebula/runtime.py:166-169.  tokens int64 [B,T] contiguous,

@@ -1,0 +1,42 @@
+"""The 4-bit key/value cache in float64, written from the format's definition
+(include/forgeml_b200.h), one group at a time.
+
+stands_for(x): what rows x [..., D] read back as, before the rounding to x's
+dtype.  attention(): q [B,T,QH,D] over rows 0..start+t of those numbers.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+
+def stands_for(x: torch.Tensor) -> torch.Tensor:
+    x = x.detach().cpu()
+    out = torch.empty(x.shape, dtype=torch.float64)
+    for c0 in range(0, x.shape[-1], 32):
+        g = x[..., c0:c0 + 32].double()
+        z, top = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
+        s = ((top - z) / 15).to(x.dtype).double()
+        code = ((g - z) / s.masked_fill(s == 0, 1.0)).round().clamp(0, 15)
+        code = code.masked_fill(s == 0, 0.0)
+        val = z + code * s
+        finite = g.isfinite().all(-1, keepdim=True)
+        out[..., c0:c0 + 32] = torch.where(finite, val, torch.full_like(val, math.nan))
+    return out
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts) -> torch.Tensor:
+    """k, v [B,n,H,D] float64 rows in position order; float64 [B,T,QH*D]."""
+    q = q.detach().cpu().double()
+    b, t, qh, d = q.shape
+    group = qh // k.shape[2]
+    out = torch.empty(b, t, qh, d, dtype=torch.float64)
+    for i in range(b):
+        for j in range(t):
+            n = int(starts[i]) + j + 1
+            for h in range(qh):
+                s = k[i, :n, h // group] @ q[i, j, h] / math.sqrt(d)
+                out[i, j, h] = torch.softmax(s, 0) @ v[i, :n, h // group]
+    return out.reshape(b, t, qh * d)

@@ -1,0 +1,480 @@
+"""The 4-bit key/value cache on the B200 against its definition in float64
+(oracle/kv4.py): append, read back, attention, and a run of them together.
+
+Tolerances (u = finfo(dtype).eps / 2, one rounding to the dtype):
+  read back  z + c s is formed once in fp32 and rounded to the dtype:
+             (u + 2^-24) |x|, plus half the smallest subnormal.
+  attention  see ``attention_atol``.
+"""
+
+import math
+
+import pytest
+import torch
+
+from forgeml_b200 import _native
+from forgeml_b200.nebula import (CacheError, DecoderConfig, Engine, KV4Pool, KVCache, ParallelContext, TinyDecoder,
+                                 ops)
+from oracle import kv4 as orc
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+RANGE = 4  # bit of the device error word: slot or position outside the pool
+
+
+@pytest.fixture(autouse=True)
+def clean_status(cuda):
+    _native.device_status()
+    yield
+    assert _native.device_status() == 0
+
+
+def rows(b, n, h, d, dtype, seed, offset=True):
+    g = torch.Generator().manual_seed(seed)
+    k = torch.randn(b, n, h, d, generator=g)
+    if offset:
+        k = k + 3.0 * torch.randn(h, d, generator=g)
+    return k.to(dtype), torch.randn(b, n, h, d, generator=g).to(dtype)
+
+
+def make_pool(cuda, slots, h, max_seq, d, dtype):
+    pool = KV4Pool(slots=slots, heads=h, max_seq_len=max_seq, head_dim=d, device=cuda, dtype=dtype)
+    # rows nobody wrote: codes 15, parameters NaN
+    pool.k_codes.fill_(255), pool.v_codes.fill_(255)
+    pool.k_params.fill_(math.nan), pool.v_params.fill_(math.nan)
+    return pool
+
+
+def table(values, cuda):
+    return torch.tensor(values, dtype=torch.int32, device=cuda)
+
+
+def snapshot(pool):
+    """The pool's bytes (NaN parameters compare equal to themselves)."""
+    return [t.clone().view(torch.uint8) for t in (pool.k_codes, pool.v_codes, pool.k_params, pool.v_params)]
+
+
+def check_values(got, want64, dtype):
+    got = got.cpu().double()
+    f = torch.finfo(dtype)
+    tol = (f.eps / 2 + 2.0 ** -24) * want64.abs() + f.tiny * f.eps / 2
+    assert torch.equal(got.isnan(), want64.isnan())
+    bad = (got - want64).abs() > tol
+    assert not bad.any(), (got[bad][:4], want64[bad][:4])
+
+
+def attention_atol(q, kx, vx, dtype):
+    """What the kernels may be off by, before the output's rounding u |out|.
+
+    e = 2^-24.  A score sums D products q (c + 128) (codes are fed to the
+    tensor cores as 128 + c, whose sums are at most 143 |q| s before the
+    offset is taken off again) and the minimum's share |q| |z|, in fp32:
+    (D + 8) e S with S = scale * sum |q| * (143 s + |z|).  It moves a weight by
+    twice that.  The weights' exponentials and the sum add 8 e and, over n
+    rows, (n + 32) e of 143 s + |z| of the values; the weights times s enter
+    the tensor cores in two bfloat16 parts, 2^-16 of 15 s."""
+    e, d, n = 2.0 ** -24, q.shape[-1], kx.shape[1]
+
+    def spans(x):  # largest step and largest |number|
+        step = 0.0
+        for c0 in range(0, x.shape[-1], 32):
+            g = x[..., c0:c0 + 32]
+            step = max(step, float((g.amax(-1) - g.amin(-1)).max()) / 15 * (1 + 2.0 ** -8))
+        return step, float(x.abs().max())
+
+    ks, kz = spans(kx)
+    vs, vz = spans(vx)
+    S = float(q.double().abs().sum(-1).max()) / math.sqrt(d) * (143 * ks + kz)
+    return (2 * (d + 8) * e * S + 8 * e) * (15 * vs + vz) + (n + 32) * e * (143 * vs + vz) + 2.0 ** -16 * 15 * vs
+
+
+def tc_atol(q, kx, vx, dtype):
+    """Prompts on the tensor cores: keys, values and weights are rounded to the
+    dtype (u each): a score moves by u S, a weight by twice that, and weight
+    and value add 2 u of the largest value."""
+    u = torch.finfo(dtype).eps / 2
+    S = float(q.double().abs().sum(-1).max()) / math.sqrt(q.shape[-1]) * float(kx.abs().max())
+    return (2 * u * S + 2 * u) * float(vx.abs().max())
+
+
+def check_attention(got, q, kx, vx, starts, dtype, extra=0.0):
+    want = orc.attention(q, kx, vx, starts)
+    u = torch.finfo(dtype).eps / 2
+    tol = attention_atol(q, kx, vx, dtype) + extra + u * want.abs() * (1 + 2.0 ** -10)
+    err = (got.cpu().double() - want).abs()
+    assert torch.isfinite(got).all()
+    assert (err <= tol).all(), (float((err - tol).max()), float(err.max()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,t,h,d", [(1, 1, 1, 1), (2, 3, 2, 32), (3, 1, 16, 128), (2, 17, 3, 80), (1, 130, 2, 64),
+                                     (2, 5, 5, 33), (1, 9, 1, 256), (2, 4, 3, 192), (1, 7, 2, 96), (1, 5, 2, 160),
+                                     (2, 2, 2, 224), (1, 3, 1, 255)])
+def test_rows_read_back_as_their_definition(cuda, dtype, b, t, h, d):
+    k, v = rows(b, t, h, d, dtype, seed=7 * d + t)
+    max_seq = t + 21
+    pool = make_pool(cuda, b + 2, h, max_seq, d, dtype)
+    before = snapshot(pool)
+    slots = table([(3 * i + 1) % (b + 2) for i in range(b)] if (b + 2) % 3 else list(range(b, 0, -1)), cuda)
+    starts = table([(5 * i + 4) % 22 for i in range(b)], cuda)
+    ops.kv4_append(k.to(cuda), v.to(cuda), pool, slots, starts)
+    kr, vr = ops.kv4_read(pool, slots, t, start_pos=starts)
+    check_values(kr, orc.stands_for(k).transpose(1, 2), dtype)
+    check_values(vr, orc.stands_for(v).transpose(1, 2), dtype)
+    # every row not written is as it was
+    written = torch.zeros(b + 2, max_seq + (-max_seq) % 16, dtype=torch.bool, device=cuda)
+    for i in range(b):
+        written[int(slots[i]), int(starts[i]):int(starts[i]) + t] = True
+    keep = ~written[:, None].expand(-1, h, -1)
+    for x, y in zip(before, snapshot(pool)):
+        assert torch.equal(x[keep], y[keep])
+    # from row 0, and into given tensors
+    n = int(starts.min()) + t
+    out = tuple(torch.empty(b, h, n, d, dtype=dtype, device=cuda) for _ in range(2))
+    assert ops.kv4_read(pool, slots, n, out=out)[0] is out[0]
+    for i in range(b):
+        if n > int(starts[i]):
+            torch.testing.assert_close(out[1][i, :, int(starts[i]):], vr[i, :, :n - int(starts[i])], rtol=0, atol=0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_groups_at_the_borders(cuda, dtype):
+    """Constant groups, ties, the type's extremes, subnormals, infinities, NaN."""
+    f = torch.finfo(dtype)
+    d = 64
+    k = torch.zeros(1, 10, 1, d, dtype=torch.float64)
+    k[0, 0] = 3.0  # constant: step 0
+    k[0, 1, 0] = torch.arange(d) % 32 * 0.5  # 0 .. 15.5: ties at every half
+    k[0, 2, 0] = torch.arange(d) % 16 * f.tiny * f.eps  # subnormals
+    k[0, 3, 0, 0], k[0, 3, 0, 1] = f.max, f.min  # the widest range
+    k[0, 4, 0] = torch.linspace(1000, 1001, d)  # far from zero
+    k[0, 5, 0, 3] = math.inf
+    k[0, 6, 0, 40] = math.nan
+    k[0, 7, 0, 5], k[0, 7, 0, 45] = -math.inf, math.nan
+    k[0, 8, 0] = torch.arange(d) % 31 * f.tiny
+    k[0, 9, 0] = torch.linspace(-1, 1, d) ** 3 * math.sqrt(f.max)
+    k = k.to(dtype)
+    v = k.flip(1)
+    pool = make_pool(cuda, 1, 1, 12, d, dtype)
+    z = table([0], cuda)
+    ops.kv4_append(k.to(cuda), v.to(cuda), pool, z, z)
+    kr, vr = ops.kv4_read(pool, z, 10)
+    check_values(kr, orc.stands_for(k).transpose(1, 2), dtype)
+    check_values(vr, orc.stands_for(v).transpose(1, 2), dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_append_from_strided_views(cuda, dtype):
+    """k and v as column views of one projection output, rows that are not
+    16-byte aligned, and a permuted batch."""
+    b, t, h, d = 2, 5, 3, 40
+    g = torch.Generator().manual_seed(3)
+    for off, width in ((0, 3 * h * d), (1, 3 * h * d + 3)):
+        wide = torch.randn(b * t, width, generator=g).to(dtype)
+        dev = wide.to(cuda)
+
+        def views(w):
+            return [w[:, off + i * h * d:off + (i + 1) * h * d].reshape(b, t, h, d) if not w.is_cuda
+                    else w[:, off + i * h * d:off + (i + 1) * h * d].unflatten(1, (h, d)).unflatten(0, (b, t))
+                    for i in (1, 2)]
+
+        pool = make_pool(cuda, 3, h, 16, d, dtype)
+        slots, starts = table([2, 0], cuda), table([0, 3], cuda)
+        ops.kv4_append(*views(dev), pool, slots, starts)
+        kr, vr = ops.kv4_read(pool, slots, t, start_pos=starts)
+        kc, vc = views(wide)
+        check_values(kr, orc.stands_for(kc).transpose(1, 2), dtype)
+        check_values(vr, orc.stands_for(vc).transpose(1, 2), dtype)
+        # [B, H, T, D] storage seen as [B, T, H, D]
+        perm = kc.transpose(1, 2).contiguous().to(cuda).transpose(1, 2)
+        ops.kv4_append(perm, perm, pool, slots, starts)
+        check_values(ops.kv4_read(pool, slots, t, start_pos=starts)[0], orc.stands_for(kc).transpose(1, 2), dtype)
+
+
+def fill(cuda, dtype, starts, t, h, d, seed, extra_rows=5):
+    """A pool holding each request's rows 0..start+t-1 (nothing behind them),
+    and the same rows in float64 [B, n, H, D]."""
+    b, n = len(starts), max(starts) + t
+    k, v = rows(b, n, h, d, dtype, seed)
+    pool = make_pool(cuda, b + 1, h, n + extra_rows, d, dtype)
+    slots = [(i + 1) % (b + 1) for i in range(b)]
+    for i, s in enumerate(starts):
+        m = s + t
+        ops.kv4_append(k[i:i + 1, :m].to(cuda), v[i:i + 1, :m].to(cuda), pool, table([slots[i]], cuda),
+                       table([0], cuda))
+    return pool, table(slots, cuda), table(starts, cuda), orc.stands_for(k), orc.stands_for(v)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("starts,t,h,group,d", [
+    ([0], 1, 1, 1, 128),
+    ([0, 1, 15, 16], 1, 2, 1, 128),
+    ([17, 63, 64, 127, 128, 129], 1, 3, 1, 64),
+    ([300, 5], 1, 4, 1, 80),
+    ([1023, 700, 0], 1, 2, 1, 128),
+    ([100, 31], 1, 2, 1, 32),
+    ([100, 131], 1, 2, 1, 256),
+    ([70, 9], 1, 3, 1, 96),
+    ([40, 90], 1, 1, 1, 192),
+    ([33], 1, 1, 1, 160),
+    ([64, 12], 1, 1, 1, 224),
+    ([50], 1, 2, 1, 7),
+    ([200, 3], 1, 2, 4, 128),
+    ([77, 150], 1, 2, 7, 64),
+    ([90], 1, 1, 8, 256),
+    ([33, 0, 120], 3, 2, 1, 128),
+    ([140, 61], 5, 2, 2, 64),
+    ([30], 2, 1, 3, 96),
+])
+def test_attention(cuda, dtype, starts, t, h, group, d):
+    pool, slots, st, kx, vx = fill(cuda, dtype, starts, t, h, d, seed=d + t + h)
+    q = torch.randn(len(starts), t, h * group, d, generator=torch.Generator().manual_seed(d)).to(dtype)
+    got = ops.kv4_attention(q.to(cuda), pool, slots, st)
+    assert got.shape == (len(starts), t, h * group * d)
+    extra = tc_atol(q, kx, vx, dtype) if t > 1 and dtype != torch.float32 else 0.0
+    check_attention(got, q, kx, vx, starts, dtype, extra)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("starts,t,h,group,d", [([0], 130, 1, 1, 128), ([0, 60], 129, 2, 1, 64), ([200], 33, 1, 2, 128),
+                                                ([1, 0, 255], 40, 1, 1, 80), ([127, 128], 64, 1, 1, 128),
+                                                ([5], 70, 1, 1, 256)])
+def test_attention_of_prompts(cuda, dtype, starts, t, h, group, d):
+    pool, slots, st, kx, vx = fill(cuda, dtype, starts, t, h, d, seed=d + t)
+    q = torch.randn(len(starts), t, h * group, d, generator=torch.Generator().manual_seed(t)).to(dtype)
+    got = ops.kv4_attention(q.to(cuda), pool, slots, st)
+    extra = tc_atol(q, kx, vx, dtype) if dtype != torch.float32 else 0.0
+    check_attention(got, q, kx, vx, starts, dtype, extra)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,d", [(1, 128), (1, 80), (4, 64), (40, 128)])
+def test_attention_of_sharp_scores_and_far_keys(cuda, dtype, t, d):
+    """Scores of tens whose maximum keeps moving along the rows, and channels
+    far from zero."""
+    starts = [611]
+    n = starts[0] + t
+    g = torch.Generator().manual_seed(5)
+    k = torch.randn(1, n, 2, d, generator=g) + 20.0 * (torch.rand(2, d, generator=g) > 0.9)
+    k = (k * torch.linspace(0.2, 1.5, n)[None, :, None, None]).to(dtype)
+    v = (torch.randn(1, n, 2, d, generator=g) * 1e-2 + 1.0).to(dtype)
+    pool = make_pool(cuda, 1, 2, n, d, dtype)
+    z = table([0], cuda)
+    ops.kv4_append(k.to(cuda), v.to(cuda), pool, z, z)
+    q = (torch.randn(1, t, 2, d, generator=g) * 3).to(dtype)
+    kx, vx = orc.stands_for(k), orc.stands_for(v)
+    got = ops.kv4_attention(q.to(cuda), pool, z, table(starts, cuda))
+    extra = tc_atol(q, kx, vx, dtype) if t > 1 and dtype != torch.float32 else 0.0
+    check_attention(got, q, kx, vx, starts, dtype, extra)
+
+
+def test_attention_of_strided_queries_into_out(cuda):
+    """q as column views of a projection's output, aligned and not; out given."""
+    dtype, starts, h, d = torch.bfloat16, [90, 20], 3, 64
+    pool, slots, st, kx, vx = fill(cuda, dtype, starts, 1, h, d, seed=1)
+    for off in (0, 8, 3):
+        wide = torch.randn(2, 3 * h * d + off, generator=torch.Generator().manual_seed(off)).to(dtype)
+        q = wide[:, off:off + h * d].unflatten(1, (h, d)).unsqueeze(1)
+        qd = wide.to(cuda)[:, off:off + h * d].unflatten(1, (h, d)).unsqueeze(1)
+        out = torch.full((2, 1, h * d), math.nan, dtype=dtype, device=cuda)
+        assert ops.kv4_attention(qd, pool, slots, st, out=out) is out
+        check_attention(out, q, kx, vx, starts, dtype)
+
+
+def test_a_row_that_reads_nan_reaches_only_those_who_attend_it(cuda):
+    dtype, d = torch.bfloat16, 128
+    k, v = rows(1, 40, 1, d, dtype, seed=2)
+    k[0, 30, 0, 5] = math.nan
+    pool = make_pool(cuda, 1, 1, 64, d, dtype)
+    z = table([0], cuda)
+    ops.kv4_append(k.to(cuda), v.to(cuda), pool, z, z)
+    q = torch.randn(1, 1, 1, d, device=cuda).to(dtype)
+    assert torch.isfinite(ops.kv4_attention(q, pool, z, table([29], cuda))).all()
+    assert ops.kv4_attention(q, pool, z, table([30], cuda)).isnan().all()
+
+
+@pytest.mark.parametrize("t", [1, 3, 40])
+def test_bad_slots_and_positions_raise_the_error_word(cuda, t):
+    dtype, h, d, max_seq = torch.bfloat16, 2, 64, 48
+    pool = make_pool(cuda, 3, h, max_seq, d, dtype)
+    good = rows(1, max_seq, h, d, dtype, seed=4)
+    ops.kv4_append(good[0].to(cuda), good[1].to(cuda), pool, table([1], cuda), table([0], cuda))
+    before = snapshot(pool)
+    k, v = rows(1, t, h, d, dtype, seed=5)
+    q = torch.randn(1, t, h, d).to(dtype).to(cuda)
+    for slot, start in ((-1, 0), (3, 0), (1, -1), (1, max_seq), (1, 2 ** 31 - 1), (-2 ** 31, 0)):
+        sl, st = table([slot], cuda), table([start], cuda)
+        ops.kv4_append(k.to(cuda), v.to(cuda), pool, sl, st)
+        assert _native.device_status() == RANGE
+        for x, y in zip(before, snapshot(pool)):
+            assert torch.equal(x, y)
+        assert not ops.kv4_attention(q, pool, sl, st).any()
+        assert _native.device_status() == RANGE
+        kr, vr = ops.kv4_read(pool, sl, t, start_pos=st)
+        assert not kr.any() and not vr.any()
+        assert _native.device_status() == RANGE
+    # a chunk that ends outside: the queries that fit are answered, the others are zeros
+    kx, vx = orc.stands_for(good[0]), orc.stands_for(good[1])
+    if t > 1:
+        st = table([max_seq - 1], cuda)
+        got = ops.kv4_attention(q, pool, table([1], cuda), st)
+        assert _native.device_status() == RANGE
+        check_attention(got[:, :1], q[:, :1].cpu(), kx, vx, [max_seq - 1], dtype, tc_atol(q.cpu(), kx, vx, dtype))
+        assert not got[:, 1:].any()
+
+
+def test_the_same_slot_twice_keeps_the_first(cuda):
+    dtype, h, d = torch.float16, 3, 64
+    k, v = rows(4, 6, h, d, dtype, seed=6)
+    pool = make_pool(cuda, 3, h, 32, d, dtype)
+    # requests 0 and 2 overlap in slot 1; request 3 shares the slot but not the rows
+    slots, starts = table([1, 0, 1, 1], cuda), table([4, 4, 9, 20], cuda)
+    ops.kv4_append(k.to(cuda), v.to(cuda), pool, slots, starts)
+    assert _native.device_status() == RANGE
+    kr, _ = ops.kv4_read(pool, slots, 6, start_pos=starts)
+    want = orc.stands_for(k).transpose(1, 2)
+    for i in (0, 1, 3):
+        check_values(kr[i], want[i], dtype)
+    # reading and attending the same slot twice is fine
+    q = torch.randn(2, 1, h, d).to(dtype).to(cuda)
+    two = ops.kv4_attention(q[:1].expand(2, -1, -1, -1).contiguous(), pool, table([1, 1], cuda), table([9, 9], cuda))
+    assert torch.equal(two[0], two[1]) or two.isnan().any()  # rows 0..3 were never written: NaN both times
+
+
+def test_rows_beyond_four_gigabytes(cuda):
+    """Codes at byte offsets past 32 bits (the pool's memory is mostly untouched)."""
+    dtype, h, d, max_seq, slots = torch.bfloat16, 16, 128, 8192, 530
+    pool = KV4Pool(slots=slots, heads=h, max_seq_len=max_seq, head_dim=d, device=cuda, dtype=dtype)
+    assert pool.k_codes.numel() > 1 << 32
+    n = 33
+    k, v = rows(2, n, h, d, dtype, seed=8)
+    sl = table([slots - 1, 7], cuda)
+    z = table([0, 0], cuda)
+    ops.kv4_append(k.to(cuda), v.to(cuda), pool, sl, z)
+    kx, vx = orc.stands_for(k), orc.stands_for(v)
+    check_values(ops.kv4_read(pool, sl, n)[0], kx.transpose(1, 2), dtype)
+    q = torch.randn(2, 1, h, d).to(dtype)
+    check_attention(ops.kv4_attention(q.to(cuda), pool, sl, table([n - 1] * 2, cuda)), q, kx, vx, [n - 1] * 2, dtype)
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 80)])
+def test_prefill_and_decode_together_in_a_captured_graph(cuda, dtype, d):
+    """A prompt's rows appended and attended, then decode steps whose append and
+    attention are captured once and replayed with moving positions."""
+    b, h, t0, steps = 3, 2, 21, 6
+    k, v = rows(b, t0 + steps, h, d, dtype, seed=9)
+    kx, vx = orc.stands_for(k), orc.stands_for(v)
+    q = torch.randn(b, t0 + steps, h, d, generator=torch.Generator().manual_seed(1)).to(dtype)
+    pool = make_pool(cuda, 4, h, 64, d, dtype)
+    slots, starts = table([2, 0, 3], cuda), table([0] * b, cuda)
+    kd, vd, qd = k.to(cuda), v.to(cuda), q.to(cuda)
+    ops.kv4_append(kd[:, :t0], vd[:, :t0], pool, slots, starts)
+    got = ops.kv4_attention(qd[:, :t0], pool, slots, starts)
+    extra = tc_atol(q, kx, vx, dtype) if dtype != torch.float32 else 0.0
+    check_attention(got, q[:, :t0], kx, vx, [0] * b, dtype, extra)
+    ks, vs, qs = (x[:, :1].clone() for x in (kd, vd, qd))
+    starts.fill_(t0)
+    ks.copy_(kd[:, t0:t0 + 1]), vs.copy_(vd[:, t0:t0 + 1])
+
+    def step():
+        ops.kv4_append(ks, vs, pool, slots, starts)
+        return ops.kv4_attention(qs, pool, slots, starts)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(steps):
+        ks.copy_(kd[:, t0 + i:t0 + i + 1]), vs.copy_(vd[:, t0 + i:t0 + i + 1]), qs.copy_(qd[:, t0 + i:t0 + i + 1])
+        starts.fill_(t0 + i)
+        graph.replay()
+        check_attention(out, q[:, t0 + i:t0 + i + 1], kx, vx, [t0 + i] * b, dtype)
+
+
+def test_results_repeat_bit_for_bit(cuda):
+    dtype, starts = torch.bfloat16, [900, 33, 512]
+    for t in (1, 4, 140):
+        pool, slots, st, _, _ = fill(cuda, dtype, starts, t, 2, 128, seed=t)
+        q = torch.randn(3, t, 4, 128, device=cuda).to(dtype)
+        first = ops.kv4_attention(q, pool, slots, st)
+        for _ in range(3):
+            assert torch.equal(first, ops.kv4_attention(q, pool, slots, st))
+
+
+# ------------------------------------------------------------- in the decoder
+def small_engine(**kw):
+    cfg = DecoderConfig(**{**dict(vocab_size=64, hidden_size=128, num_heads=2, num_layers=2, intermediate_size=256,
+                                  max_seq_len=96, seed=17), **kw.pop("cfg", {})})
+    return cfg, Engine(cfg, context=ParallelContext.from_env(device="cuda"), max_requests=4, init=kw.pop("init", "reference"),
+                       **kw)
+
+
+def decoder_reference(cfg, tokens, dtype):
+    """Logits [B, T, V] in float64 of the reference decoder's weights (rounded
+    to dtype) with every layer's keys and values quantised as they are written."""
+    ref = TinyDecoder(cfg).to(dtype).double()
+    x = ref.token_embedding(tokens) + ref.position_embedding(torch.arange(tokens.shape[1]))
+    b, t, h = x.shape
+    for blk in ref.blocks:
+        y = blk.ln1(x)
+        q, k, v = (f(y).view(b, t, cfg.num_heads, cfg.head_dim) for f in (blk.q, blk.k, blk.v))
+        kx, vx = (orc.stands_for(z.detach().to(dtype)) for z in (k, v))
+        x = x + blk.o(orc.attention(q, kx, vx, [0] * b))
+        x = x + blk.down(torch.nn.functional.gelu(blk.up(blk.ln2(x)), approximate="tanh"))
+    return ref.lm_head(ref.final_norm(x)).detach()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("ln", ["fold", "prologue", "kernel"])
+def test_engine_with_a_4_bit_cache(cuda, dtype, ln):
+    """Prefill, captured decode steps and per-request positions through the
+    engine, against the decoder whose keys and values are quantised in float64.
+
+    A step is at most 2^-4 of a group's span wide (15 steps, half a step either
+    side); a rounding elsewhere in the decoder moves a number across a border
+    now and then and so by one step.  The logits are therefore compared at 2e-2
+    of their scale for 16 bits, as the decoder's own tests are, and at 2e-3 for
+    fp32."""
+    cfg, eng = small_engine(dtype=dtype, kv_bits=4)
+    eng.decoder.decode_ln = ln
+    assert eng.decoder.cache.k_pool == {} and len(eng.decoder.cache.kv4_pool) == 2
+    tokens = torch.randint(0, 64, (3, 60), generator=torch.Generator().manual_seed(2))
+    want = decoder_reference(cfg, tokens, dtype)
+    rel = 2e-3 if dtype == torch.float32 else 2e-2
+    atol = rel * float(want.abs().max())
+    got = [eng.forward(tokens[:, :55], (5, 6, 7), 0)]
+    got += [eng.forward(tokens[:, i:i + 1], (5, 6, 7), i) for i in range(55, 60)]
+    torch.testing.assert_close(torch.cat([g.cpu() for g in got], 1).double(), want, rtol=0, atol=atol)
+    eng.close()
+
+
+def test_generate_with_a_4_bit_cache_eager_and_captured(cuda):
+    outs = []
+    for graphs in (True, False):
+        _, eng = small_engine(dtype=torch.bfloat16, kv_bits=4)
+        eng.decoder.use_cuda_graphs = graphs
+        outs.append((eng.generate([[1, 2, 3, 4, 5], [6, 7, 8, 9, 10]], 20),
+                     eng.generate_mixed([[1, 2, 3], [4, 5, 6, 7, 8, 9, 10], [11]], 12)))
+        eng.close()
+    assert outs[0] == outs[1]
+
+
+def test_cache_append_returns_the_prefixes_it_stands_for(cuda):
+    for dtype in DTYPES:
+        c = KVCache(layer_ids=(3, 4), num_heads=2, head_dim=48, max_seq_len=20, max_requests=3, device=cuda,
+                    dtype=dtype, kv_bits=4)
+        c.reserve((10, 11))
+        k, v = rows(2, 9, 2, 48, dtype, seed=12)
+        for lo, hi in ((0, 5), (5, 6), (6, 9)):
+            for lid in (3, 4):
+                pk, pv = c.append(lid, (10, 11), k[:, lo:hi].transpose(1, 2).to(cuda),
+                                  v[:, lo:hi].transpose(1, 2).to(cuda), lo)
+                check_values(pk, orc.stands_for(k[:, :hi]).transpose(1, 2), dtype)
+                check_values(pv, orc.stands_for(v[:, :hi]).transpose(1, 2), dtype)
+        with pytest.raises(CacheError):
+            c.append(5, (10,), k[:1, :1].transpose(1, 2).to(cuda), v[:1, :1].transpose(1, 2).to(cuda), 9)
