@@ -140,7 +140,8 @@ _SIGNATURES = {
     "neb_kv4_params_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64, _I]),
     "neb_kv4_append": (_I, [_P, _S4, _P, _S4, _KV4, _P, _P, _I64, _I64, _P]),
     "neb_kv4_read": (_I, [_KV4, _P, _P, _I64, _P, _P, _I64, _P]),
-    "neb_kv4_attention": (_I, [_P, _S4, _KV4, _P, _P, _P, _I64, _I64, _I64, _F, _P]),
+    "neb_kv4_attention": (_I, [_P, _S4, _KV4, _P, _P, _P, _I64, _I64, _I64, _F, _P, ctypes.c_size_t, _P]),
+    "neb_kv4_attention_workspace_size": (ctypes.c_size_t, [_KV4, _I64, _I64, _I64]),
     "neb_embed": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _P]),
     "neb_argmax": (_I, [_P, _I64, _I64, _I64, _P, _I, _P]),
     "neb_add": (_I, [_P, _P, _P, _I64, _I, _P]),

@@ -150,8 +150,11 @@ def kv4_attention(q: torch.Tensor, pool, slot_of: torch.Tensor, start_pos: torch
             or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {(b, t, qh * d)} tensor of q's dtype and device")
     with _on_device(pool.device):
+        need = int(_native.load().neb_kv4_attention_workspace_size(pool.handle, b, t, qh))
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
         _native.call("neb_kv4_attention", q.data_ptr(), _kv4_strides(q), pool.handle, slot_of.data_ptr(),
-                     start_pos.data_ptr(), out.data_ptr(), b, t, qh, 1.0 / math.sqrt(d), _stream(q))
+                     start_pos.data_ptr(), out.data_ptr(), b, t, qh, 1.0 / math.sqrt(d),
+                     ws.data_ptr() if need else None, need, _stream(q))
     return out
 
 

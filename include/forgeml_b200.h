@@ -280,7 +280,11 @@ FML_API int neb_kv4_read(const neb_kv4_pool* pool, const int32_t* slot_of, const
  * Scores, softmax and the sums over the rows in fp32. */
 FML_API int neb_kv4_attention(const void* q, const int64_t q_strides[4], const neb_kv4_pool* pool,
                       const int32_t* slot_of, const int32_t* start_pos, void* out,
-                      int64_t batch, int64_t t, int64_t q_heads, float scale, void* stream);
+                      int64_t batch, int64_t t, int64_t q_heads, float scale,
+                      void* workspace, size_t workspace_bytes, void* stream);
+/* Bytes of (16-byte aligned, uninitialised) device memory the call needs; one
+ * call at a time may use them. */
+FML_API size_t neb_kv4_attention_workspace_size(const neb_kv4_pool* pool, int64_t batch, int64_t t, int64_t q_heads);
 
 /* ---------------------------------------------------------------------------
  * Token + learned position embedding:

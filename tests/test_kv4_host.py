@@ -160,7 +160,7 @@ def test_c_entries_check_the_pool():
         p = None if bad is None else c_pool(**bad)
         _rejects("neb_kv4_append", code, match, FAKE, s4, FAKE, s4, p, FAKE, FAKE, 1, 1, None)
         _rejects("neb_kv4_read", code, match, p, FAKE, None, 1, FAKE, FAKE, 1, None)
-        _rejects("neb_kv4_attention", code, match, FAKE, s4, p, FAKE, FAKE, FAKE, 1, 1, 2, 0.1, None)
+        _rejects("neb_kv4_attention", code, match, FAKE, s4, p, FAKE, FAKE, FAKE, 1, 1, 2, 0.1, FAKE, 1 << 40, None)
 
 
 def test_c_entries_check_their_arguments():
@@ -177,13 +177,17 @@ def test_c_entries_check_their_arguments():
     _rejects("neb_kv4_read", EINVAL, "positive", p, FAKE, None, 0, FAKE, FAKE, 1, None)
     _rejects("neb_kv4_read", EINVAL, "exceeds max_seq", p, FAKE, None, 65, FAKE, FAKE, 1, None)
     _rejects("neb_kv4_read", EUNSUPPORTED, "too many requests", p, FAKE, None, 1, FAKE, FAKE, 1 << 25, None)
-    _rejects("neb_kv4_attention", EINVAL, "null pointer", FAKE, s4, p, FAKE, FAKE, None, 1, 1, 2, 0.1, None)
-    _rejects("neb_kv4_attention", EINVAL, "positive", FAKE, s4, p, FAKE, FAKE, FAKE, 1, 1, 0, 0.1, None)
-    _rejects("neb_kv4_attention", EINVAL, "multiple of the pool's heads", FAKE, s4, p, FAKE, FAKE, FAKE, 1, 1, 3, 0.1, None)
-    _rejects("neb_kv4_attention", EUNSUPPORTED, "innermost stride", FAKE, s5, p, FAKE, FAKE, FAKE, 1, 1, 2, 0.1, None)
-    _rejects("neb_kv4_attention", EINVAL, "exceeds max_seq", FAKE, s4, p, FAKE, FAKE, FAKE, 1, 65, 2, 0.1, None)
+    _rejects("neb_kv4_attention", EINVAL, "null pointer", FAKE, s4, p, FAKE, FAKE, None, 1, 1, 2, 0.1, FAKE, 1 << 40, None)
+    _rejects("neb_kv4_attention", EINVAL, "positive", FAKE, s4, p, FAKE, FAKE, FAKE, 1, 1, 0, 0.1, FAKE, 1 << 40, None)
+    _rejects("neb_kv4_attention", EINVAL, "multiple of the pool's heads", FAKE, s4, p, FAKE, FAKE, FAKE, 1, 1, 3, 0.1, FAKE, 1 << 40, None)
+    _rejects("neb_kv4_attention", EUNSUPPORTED, "innermost stride", FAKE, s5, p, FAKE, FAKE, FAKE, 1, 1, 2, 0.1, FAKE, 1 << 40, None)
+    _rejects("neb_kv4_attention", EINVAL, "exceeds max_seq", FAKE, s4, p, FAKE, FAKE, FAKE, 1, 65, 2, 0.1, FAKE, 1 << 40, None)
     _rejects("neb_kv4_attention", EUNSUPPORTED, "too many queries", FAKE, s4, p, FAKE, FAKE, FAKE, 1 << 24, 64, 1 << 20,
-             0.1, None)
+             0.1, FAKE, 1 << 40, None)
+    _rejects("neb_kv4_attention", 4, "workspace of", FAKE, s4, p, FAKE, FAKE, FAKE, 1, 1, 2, 0.1, None, 1 << 40, None)
+    _rejects("neb_kv4_attention", 4, "workspace of", FAKE, s4, p, FAKE, FAKE, FAKE, 1, 1, 2, 0.1, FAKE, 64, None)
+    _rejects("neb_kv4_attention", EINVAL, "16-byte aligned", FAKE, s4, p, FAKE, FAKE, FAKE, 1, 1, 2, 0.1, FAKE + 8,
+             1 << 40, None)
 
 
 def test_the_definition_on_hand_made_groups():
