@@ -518,40 +518,84 @@ __global__ void __launch_bounds__(kWarps * 32, G <= 4 ? 4 : 2) attn_row_kernel(c
 }
 
 // Joins the workers' shares of the segments that more than one of them holds,
-// in the workers' order; zeros for bad requests.  One CTA per segment.
-template <typename T>
-__global__ void __launch_bounds__(128) attn_join_kernel(const Pool p, const Problem a, long long W) {
+// in the workers' order; zeros for bad requests.  One CTA per segment: its
+// threads take the channels (times slices of the shares, so that a segment of
+// hundreds of shares is not one long chain of loads).
+constexpr int kJoinThreads = 256;
+constexpr int kJoinShares = 256;  // shares weighted at once
+
+template <typename T, int G>
+__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const Pool p, const Problem a, long long W) {
   pdl_wait();
   pdl_trigger();
+  constexpr int CH = 32 * G, SL = kJoinThreads / CH;  // channels, slices
+  __shared__ float weight[kJoinShares], sum_x[SL > 1 ? SL : 1][CH], red[kJoinThreads / 32];
+  __shared__ uint32_t place[kJoinShares];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / p.H, seg = blockIdx.x % p.H;
   const int keys = keys_of(p, a, b), units = units_of(keys);
   T* op = static_cast<T*>(a.out) + ((long long)b * a.QH + seg) * p.D;
   if (keys == 0) {
-    if (threadIdx.x == 0) raise_device_error(DEV_ERR_ATTN_RANGE);
-    for (int d = threadIdx.x; d < p.D; d += blockDim.x) op[d] = from_f32<T>(0.f);
+    if (tid == 0) raise_device_error(DEV_ERR_ATTN_RANGE);
+    for (int d = tid; d < p.D; d += kJoinThreads) op[d] = from_f32<T>(0.f);
     return;
   }
   const long long total = units_before(p, a, a.B) * p.H;
   const long long u0 = units_before(p, a, b) * p.H + (long long)seg * units, u1 = u0 + units;
-  // worker of a unit u: the largest w with total * w / W <= u
-  auto worker = [&](long long u) { return ((u + 1) * W - 1) / total; };
   W = min(W, total);
-  const long long w0 = worker(u0), w1 = worker(u1 - 1);
+  // worker of a unit u: the largest w with total * w / W <= u
+  const long long w0 = ((u0 + 1) * W - 1) / total, w1 = (u1 * W - 1) / total;
   if (w0 == w1) return;
-  const int stride = 2 + 32 * p.G;
-  auto share = [&](long long w) { return a.ws + (w * 2 + (total * w / W >= u0 ? 0 : 1)) * stride; };
-  float m = -INFINITY;
-  for (long long w = w0; w <= w1; ++w) m = fmaxf(m, share(w)[0]);
-  for (int d = threadIdx.x; d < p.D; d += blockDim.x) {
-    float x = 0.f, l = 0.f;
-    for (long long w = w0; w <= w1; ++w) {
-      const float* s = share(w);
-      const float f = ex2(s[0] - m);
-      l = fmaf(f, s[1], l);
-      x = fmaf(f, s[2 + d], x);
+  constexpr int stride = 2 + CH;
+  float m = -INFINITY, l = 0.f, x = 0.f;  // x: this thread's channel over its slice of the shares
+  const int ch = tid % CH, sl = tid / CH;
+  for (long long base = w0; base <= w1; base += kJoinShares) {
+    const int n = (int)min((long long)kJoinShares, w1 + 1 - base);
+    float mine = -INFINITY, ml = 0.f;
+    if (tid < n) {
+      const long long w = base + tid;
+      const uint32_t at = (uint32_t)(w * 2 + (total * w / W >= u0 ? 0 : 1));
+      place[tid] = at;
+      mine = a.ws[(long long)at * stride];
+      ml = a.ws[(long long)at * stride + 1];
     }
-    op[d] = from_f32<T>(x / l);
+    float mx = mine;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    __syncthreads();  // the previous round's weights are read
+    if (lane == 0) red[warp] = mx;
+    __syncthreads();
+    mx = m;
+#pragma unroll
+    for (int i = 0; i < kJoinThreads / 32; ++i) mx = fmaxf(mx, red[i]);
+    const float alpha = m == -INFINITY ? 0.f : ex2(m - mx);
+    m = mx;
+    const float f = tid < n ? ex2(mine - m) : 0.f;
+    weight[tid] = f;
+    float part = f * ml;
+    if (tid >= n) part = 0.f;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) part += __shfl_xor_sync(0xffffffffu, part, off);
+    __syncthreads();
+    if (lane == 0) red[warp] = part;
+    __syncthreads();
+    l *= alpha;
+#pragma unroll
+    for (int i = 0; i < kJoinThreads / 32; ++i) l += red[i];
+    x *= alpha;
+    if (sl < SL) {
+#pragma unroll 4
+      for (int i = sl; i < n; i += SL) x = fmaf(weight[i], a.ws[(long long)place[i] * stride + 2 + ch], x);
+    }
   }
+  if (SL > 1) {
+    if (sl < SL) sum_x[sl][ch] = x;
+    __syncthreads();
+    x = 0.f;
+#pragma unroll
+    for (int i = 0; i < SL; ++i) x += sum_x[i][ch];
+  }
+  if (sl == 0 && ch < p.D) op[ch] = from_f32<T>(x / l);
 }
 
 template <typename T, int G>
@@ -568,7 +612,7 @@ static int launch_row(const Pool& p, const Problem& a, int grid, cudaStream_t st
   cudaError_t e = launch_pdl(attn_row_kernel<T, G>, dim3((unsigned)grid), dim3(kWarps * 32), smem, st, 1, p, a);
   count_launch();
   if (e != cudaSuccess) return check_cuda(e, "neb_kv4_attention launch");
-  e = launch_pdl(attn_join_kernel<T>, dim3((unsigned)(a.B * p.H)), dim3(128), 0, st, 1, p, a,
+  e = launch_pdl(attn_join_kernel<T, G>, dim3((unsigned)(a.B * p.H)), dim3(kJoinThreads), 0, st, 1, p, a,
                  (long long)grid * kWarps);
   count_launch();
   return check_cuda(e, "neb_kv4_attention join launch");
