@@ -81,10 +81,7 @@ class neb_kv4_pool(ctypes.Structure):
     """One layer's 4-bit key/value pool (include/forgeml_b200.h)."""
 
     _fields_ = [
-        ("k_codes", ctypes.c_void_p),
-        ("v_codes", ctypes.c_void_p),
-        ("k_params", ctypes.c_void_p),
-        ("v_params", ctypes.c_void_p),
+        ("data", ctypes.c_void_p),
         ("slots", ctypes.c_int64),
         ("heads", ctypes.c_int64),
         ("max_seq", ctypes.c_int64),
@@ -136,8 +133,7 @@ _SIGNATURES = {
     ),
     "neb_attention": (_I, [_P, _S4, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _F, _I, _P]),
     "neb_kv_append": (_I, [_P, _S4, _P, _S4, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _P]),
-    "neb_kv4_codes_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64]),
-    "neb_kv4_params_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64, _I]),
+    "neb_kv4_pool_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64, _I]),
     "neb_kv4_append": (_I, [_P, _S4, _P, _S4, _KV4, _P, _P, _I64, _I64, _P]),
     "neb_kv4_read": (_I, [_KV4, _P, _P, _I64, _P, _P, _I64, _P]),
     "neb_kv4_attention": (_I, [_P, _S4, _KV4, _P, _P, _P, _I64, _I64, _I64, _F, _P, ctypes.c_size_t, _P]),

@@ -132,7 +132,8 @@ __global__ void __launch_bounds__(256)
       continue;
     }
     const int pos = start + t;
-    const long long r = live ? head_row(p, slot, h) + pos : 0;
+    uint8_t* const tile = live ? head_tiles(p, slot, h) + (long long)(pos / kTile) * (2 * p.half) : nullptr;
+    const int r = pos % kTile;
     float x[2][8];
     if (n > 0) {
       load8<T, VEC>(k + b * ks0 + t * ks1 + h * ks2, c0, p.D, x[0]);
@@ -143,14 +144,14 @@ __global__ void __launch_bounds__(256)
       float s, z;
       const uint32_t w = quantise8<T>(x[kv], n, s, z);
       if (live && quarter == 0) {
-        T* pr = static_cast<T*>(kv ? p.vp : p.kp) + (r * p.G + g) * 2;
+        T* pr = reinterpret_cast<T*>(tile + kv * p.half + kTile * 16 * p.G) + (r * p.G + g) * 2;
         pr[0] = from_f32<T>(s);
         pr[1] = from_f32<T>(z);
       }
       if (kv == 0) {
-        if (live) *reinterpret_cast<uint32_t*>(p.kc + r * 16 * p.G + k_byte(p.G, c0)) = w;
+        if (live) *reinterpret_cast<uint32_t*>(tile + r * 16 * p.G + k_byte(p.G, c0)) = w;
       } else if (live) {
-        uint8_t* vr = p.vc + r * 16 * p.G;
+        uint8_t* vr = tile + p.half + r * 16 * p.G;
         *reinterpret_cast<uint16_t*>(vr + v_byte(p.G, c0, pos)) = (uint16_t)w;
         *reinterpret_cast<uint16_t*>(vr + v_byte(p.G, c0 + 4, pos)) = (uint16_t)(w >> 16);
       }
@@ -190,20 +191,21 @@ __global__ void __launch_bounds__(256)
     const bool ok = slot >= 0 && slot < p.slots && start >= 0 && start <= p.max_seq - 1 - i;
     if (!ok) raise_device_error(DEV_ERR_ATTN_RANGE);
     const int pos = ok ? start + i : 0;
-    const long long r = ok ? head_row(p, slot, h) + pos : 0;
+    const uint8_t* const tile = ok ? head_tiles(p, slot, h) + (long long)(pos / kTile) * (2 * p.half) : nullptr;
+    const int r = pos % kTile;
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
       T* out = (kv ? vo : ko) + o * p.D;
       float s = 0.f, z = 0.f;
       uint32_t w = 0;
       if (ok) {
-        const T* pr = static_cast<const T*>(kv ? p.vp : p.kp) + (r * p.G + g) * 2;
+        const T* pr = reinterpret_cast<const T*>(tile + kv * p.half + kTile * 16 * p.G) + (r * p.G + g) * 2;
         s = to_f32<T>(pr[0]);
         z = to_f32<T>(pr[1]);
         if (kv == 0) {
-          w = *reinterpret_cast<const uint32_t*>(p.kc + r * 16 * p.G + k_byte(p.G, c0));
+          w = *reinterpret_cast<const uint32_t*>(tile + r * 16 * p.G + k_byte(p.G, c0));
         } else {
-          const uint8_t* vr = p.vc + r * 16 * p.G;
+          const uint8_t* vr = tile + p.half + r * 16 * p.G;
           w = *reinterpret_cast<const uint16_t*>(vr + v_byte(p.G, c0, pos)) |
               (uint32_t) * reinterpret_cast<const uint16_t*>(vr + v_byte(p.G, c0 + 4, pos)) << 16;
         }
@@ -219,26 +221,22 @@ int pool_from(const neb_kv4_pool* pool, const char* who, Pool* p) {
   const std::string name(who);
   if (!pool) return fail(FML_EINVAL, name + ": null pool");
   if (!valid_dtype(pool->dtype)) return fail(FML_EINVAL, name + ": bad dtype");
-  if (!pool->k_codes || !pool->v_codes || !pool->k_params || !pool->v_params)
+  if (!pool->data)
     return fail(FML_EINVAL, name + ": null pointer");
   if (pool->slots <= 0 || pool->heads <= 0 || pool->max_seq <= 0 || pool->head_dim <= 0)
     return fail(FML_EINVAL, name + ": sizes must be positive");
   if (pool->head_dim > kMaxD) return fail(FML_EUNSUPPORTED, name + ": head_dim > 256");
   if (pool->slots > (1 << 30) || pool->heads > (1 << 20) || pool->max_seq > (1 << 30))
     return fail(FML_EUNSUPPORTED, name + ": pool too large");
-  for (const void* q : {(const void*)pool->k_codes, (const void*)pool->v_codes, (const void*)pool->k_params,
-                        (const void*)pool->v_params})
-    if (reinterpret_cast<uintptr_t>(q) & 15) return fail(FML_EINVAL, name + ": pool tensors must be 16-byte aligned");
-  p->kc = static_cast<uint8_t*>(pool->k_codes);
-  p->vc = static_cast<uint8_t*>(pool->v_codes);
-  p->kp = pool->k_params;
-  p->vp = pool->v_params;
-  p->rows = (pool->max_seq + kRowPad - 1) / kRowPad * kRowPad;
+  if (reinterpret_cast<uintptr_t>(pool->data) & 127) return fail(FML_EINVAL, name + ": the pool must be 128-byte aligned");
+  p->data = static_cast<uint8_t*>(pool->data);
+  p->tiles = (pool->max_seq + kTile - 1) / kTile;
   p->slots = (int)pool->slots;
   p->H = (int)pool->heads;
   p->max_seq = (int)pool->max_seq;
   p->D = (int)pool->head_dim;
   p->G = groups_of(p->D);
+  p->half = kTile * p->G * (16 + 2 * (int)dtype_size(pool->dtype));
   return FML_OK;
 }
 
@@ -283,15 +281,11 @@ static int read(const Pool& p, const int32_t* slot_of, const int32_t* start_pos,
 
 using namespace fml;
 
-extern "C" size_t neb_kv4_codes_bytes(int64_t slots, int64_t heads, int64_t max_seq, int64_t head_dim) {
-  if (slots <= 0 || heads <= 0 || max_seq <= 0 || head_dim <= 0 || head_dim > kv4::kMaxD) return 0;
-  const size_t rows = (size_t)((max_seq + kv4::kRowPad - 1) / kv4::kRowPad * kv4::kRowPad);
-  return (size_t)slots * (size_t)heads * rows * 16 * (size_t)kv4::groups_of((int)head_dim);
-}
-
-extern "C" size_t neb_kv4_params_bytes(int64_t slots, int64_t heads, int64_t max_seq, int64_t head_dim, int dtype) {
-  if (!valid_dtype(dtype)) return 0;
-  return neb_kv4_codes_bytes(slots, heads, max_seq, head_dim) / 16 * 2 * dtype_size(dtype);
+extern "C" size_t neb_kv4_pool_bytes(int64_t slots, int64_t heads, int64_t max_seq, int64_t head_dim, int dtype) {
+  if (slots <= 0 || heads <= 0 || max_seq <= 0 || head_dim <= 0 || head_dim > kv4::kMaxD || !valid_dtype(dtype)) return 0;
+  const size_t tiles = (size_t)((max_seq + kv4::kTile - 1) / kv4::kTile);
+  return (size_t)slots * (size_t)heads * tiles * 2 * kv4::kTile * (size_t)kv4::groups_of((int)head_dim) *
+         (16 + 2 * dtype_size(dtype));
 }
 
 extern "C" int neb_kv4_append(const void* k, const int64_t k_strides[4], const void* v, const int64_t v_strides[4],

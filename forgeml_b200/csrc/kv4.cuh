@@ -11,11 +11,10 @@
 // holds an infinity or a NaN has s = z = NaN and reads back as NaN, as loudly
 // as a 16-bit cache would.  Unused channels of a short group hold code 0.
 //
-// Memory of a layer (keys and values alike, a tensor each):
-//   codes   [slots][heads][rows][16 G bytes]
-//   params  [slots][heads][rows][G][2]  (s, z) in T
-// rows = max_seq rounded up to 16, so every head's run of rows starts on a
-// 16-byte boundary and a copy of whole 16-row tiles stays inside it.
+// Memory of a layer: [slots][heads][tiles], a tile being 32 positions of one
+// head in one piece, so that a kernel fetches it with one copy:
+//   keys' codes [32][16 G bytes], keys' parameters [32][G][2] (s, z) in T,
+//   values' codes, values' parameters.
 //
 // Order of the codes within a row.  The attention kernel feeds codes straight
 // to mma.sync.m16n8k16 fragments; the order makes a thread's codes of all
@@ -36,20 +35,20 @@ namespace kv4 {
 
 constexpr int kGroup = 32;
 constexpr int kMaxD = 256;
-constexpr int kRowPad = 16;
+constexpr int kTile = 32;  // positions of a tile
 
 struct Pool {
-  uint8_t *kc, *vc;
-  void *kp, *vp;
-  long long rows;  // padded rows of one (slot, head)
+  uint8_t* data;
+  long long tiles;  // of one (slot, head)
   int slots, H, max_seq, D, G;
+  int half;  // bytes of a tile's keys (and of its values)
 };
 
 __host__ __device__ __forceinline__ int groups_of(int d) { return (d + kGroup - 1) / kGroup; }
 
-// First row of a (slot, head), counted in rows of the whole tensor.
-__device__ __forceinline__ long long head_row(const Pool& p, int slot, int h) {
-  return ((long long)slot * p.H + h) * p.rows;
+// The first tile of a (slot, head).
+__device__ __forceinline__ uint8_t* head_tiles(const Pool& p, int slot, int h) {
+  return p.data + ((long long)slot * p.H + h) * p.tiles * (2 * p.half);
 }
 
 __device__ __forceinline__ int v_swizzle(int G, int pos) {

@@ -21,6 +21,8 @@
 // bits, for fp16 and fp32, whose outputs keep more bits than bf16's).  Scores,
 // maxima, sums and outputs are fp32.
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 #include <string>
 #include <type_traits>
 
@@ -29,15 +31,25 @@
 namespace fml {
 namespace kv4 {
 
-// Each warp is a worker with its own contiguous share of all (request, query
-// row) segments of the batch, counted in units of 32 positions, so the work is
-// even whatever the lengths are.  A worker streams its units through its own
-// ring of shared memory with cp.async and keeps a running maximum, sum and
-// output; a segment that it holds whole is written out, the others leave
-// (maximum, sum, output) in the workspace for the join kernel.
-constexpr int kUnit = 32;
-constexpr int kWarps = 4;
-constexpr int kStages = 2;
+// The batch's segments (a request's query rows) are laid end to end and counted
+// in units of 32 positions; one CTA per SM takes an equal, contiguous share of
+// them and every warp an equal part of that, so the work is even whatever the
+// lengths are and no warp waits for another one while it streams.  (Where no
+// segment is long, a CTA takes the whole segments that begin in its share.)  A
+// warp copies its units into its own stages of shared memory (a bulk copy each:
+// four small ones a unit bound the kernel to 30 ns apiece per SM) and keeps a
+// running maximum, sum and output; a segment that it holds
+// whole is written out.  At its end the CTA joins the segments that several of
+// its warps hold, and a segment that several CTAs hold is finished by the last
+// of them to arrive: each leaves (maximum, sum, output) in the workspace and
+// takes a ticket, and the one that takes the last ticket joins them, in the
+// shares' order, so the result does not depend on who that was.  Nobody waits
+// for another CTA.  (A second kernel for this took 5 to 15 us.)
+constexpr int kUnit = kTile;
+// Longest segment (units) for which the CTAs take whole segments: their unequal
+// ends then cost less than the join through memory (about 3 us, in which a CTA
+// streams some 25 units).
+constexpr int kWholeUnits = 24;
 
 template <typename T> struct Parts { static constexpr int p = 3; };
 template <> struct Parts<__nv_bfloat16> { static constexpr int p = 2; };
@@ -47,26 +59,47 @@ struct Unit {
   static constexpr int SETS = (G + 3) / 4;           // groups are handled four at a time
   static constexpr int CR = 16 * G;                  // bytes of a row's codes
   static constexpr int PR = 2 * G * (int)sizeof(T);  // bytes of a row's parameters
-  static constexpr int kc = 0, vc = kUnit * CR, kp = 2 * kUnit * CR, vp = kp + kUnit * PR;
-  static constexpr int bytes = vp + kUnit * PR;
-  // A warp's shared memory: the ring, the scores' parts [set][8][36] fp32 (36:
-  // distinct banks), the weights' digits [set][8 or 16][32].
-  static constexpr int dots = kStages * bytes;
+  static constexpr int kc = 0, kp = kUnit * CR, vc = kUnit * (CR + PR), vp = vc + kUnit * CR;
+  static constexpr int bytes = 2 * vc;
+  // A warp's shared memory beside its stages: the scores' parts [set][8][36]
+  // fp32 (36: distinct banks), the weights' digits [set][8 or 16][32], an mbarrier
+  // per stage, its shares of the segments
+  // that it holds in part (the first and the last).
+  static constexpr int share = 4 + 32 * G;
+  static constexpr int dots = 0;
   static constexpr int digits = dots + SETS * 8 * 36 * 4;
-  static constexpr int warp_bytes = digits + SETS * (Parts<T>::p == 3 ? 16 : 8) * 32;
-  // CTAs per SM, by registers: the sums of every group (of three digits twice).
-  static constexpr int resident = G > 4 ? 2 : G == 4 && Parts<T>::p == 3 ? 3 : 4;
-  static_assert(resident * (kWarps * warp_bytes + 1024) <= 227 * 1024, "shared memory");
+  static constexpr int bars = digits + SETS * (Parts<T>::p == 3 ? 16 : 8) * 32;
+  static constexpr int parts = bars + 64;
+  static constexpr int stages_at = (parts + 2 * share * 4 + 127) / 128 * 128;
+  static constexpr int room = 227 * 1024 - 2048;
+  // Warps: by registers (the sums of every group, of three digits twice, beside
+  // the query: 168 for twelve warps) and by shared memory for two stages.
+  static constexpr int by_regs = G > 4 || (G == 4 && Parts<T>::p == 3) ? 8 : 12;
+  static constexpr int by_smem = room / (stages_at + 2 * bytes);
+  static constexpr int warps = by_regs < by_smem ? by_regs : by_smem;
+  static constexpr int fit = (room / warps - stages_at) / bytes;
+  static constexpr int stages = fit < 4 ? fit : 4;
+  static constexpr int warp_bytes = stages_at + stages * bytes;
+  static constexpr int cta_bytes = warps * warp_bytes;
+  static_assert(stages >= 2, "shared memory");
 };
 
 struct Problem {
   const int32_t *slot_of, *start_pos;
   int B, tq, QH, group;  // group: query heads of a key/value head
+  int segs;              // segments of a request: tq * QH
   long long qs0, qs1, qs2;
+  bool q_vec, out_vec;  // 16-byte loads of q, 8-byte stores of the output
   float scale_log2;  // softmax scale * log2(e)
   const void* q;
   void* out;
-  float* ws;  // [worker][first / last segment][4 + 32 G]: maximum, sum, -, -, output
+  // Workspace: [CTA][first / last segment][4 + 32 G] fp32 (maximum, sum, -, -,
+  // output), then a ticket per CTA for the segment that starts in its share and
+  // ends in another's: 48 bits that name the launch (a word of any other launch
+  // counts as empty; the last taker clears it) and the tickets taken.
+  float* ws;
+  unsigned long long* tickets;
+  unsigned long long launch;
 };
 
 // Positions that request b's last query attends; 0 for a bad slot or position.
@@ -77,12 +110,11 @@ __device__ __forceinline__ int keys_of(const Pool& p, const Problem& a, int b) {
 }
 __device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / kUnit; }
 
-// Where a worker is.  A request's segments are its query rows, (head, token)
-// in this order, each of all the request's units (an earlier token's last
-// units may be masked whole).
+// Where a warp is: a request, one of its segments (query rows: head, then the
+// head's rows, tokens innermost), a unit of it.  Every segment of a request has
+// all of the request's units (an earlier token's last ones may be masked whole).
 struct Cursor {
   int b, seg, unit, keys, units;
-  int segs;  // segments of a request
   __device__ __forceinline__ void request(const Pool& p, const Problem& a, int nb) {
     b = nb;
     keys = units = 0;
@@ -93,90 +125,109 @@ struct Cursor {
       ++b;
     }
   }
-  __device__ __forceinline__ void next(const Pool& p, const Problem& a) {
-    if (++unit < units) return;
+  __device__ __forceinline__ void next_segment(const Pool& p, const Problem& a) {
     unit = 0;
-    if (++seg < segs) return;
-    seg = 0;
-    request(p, a, b + 1);
+    if (++seg == a.segs) {
+      seg = 0;
+      request(p, a, b + 1);
+    }
+  }
+  // The next unit; true when it opens another segment.
+  __device__ __forceinline__ bool next(const Pool& p, const Problem& a) {
+    if (unit + 1 < units) {
+      ++unit;
+      return false;
+    }
+    next_segment(p, a);
+    return true;
+  }
+  // n units on.
+  __device__ __forceinline__ void skip(const Pool& p, const Problem& a, unsigned n) {
+    n += unit;
+    while (b < a.B) {
+      const unsigned here = (unsigned)(a.segs - seg) * units;
+      if (n < here) {
+        const unsigned k = n / (unsigned)units;
+        seg += k;
+        unit = n - k * units;
+        return;
+      }
+      n -= here;
+      seg = 0;
+      request(p, a, b + 1);
+    }
   }
 };
 
-// Units of the whole batch; the whole warp calls.
-__device__ __forceinline__ long long all_units(const Pool& p, const Problem& a, int segs) {
-  long long n = 0;
-  for (int i = threadIdx.x & 31; i < a.B; i += 32) n += units_of(keys_of(p, a, i));
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
-  return n * segs;
-}
+// Contiguous shares of `total` units: part w of W begins at unit total * w / W.
+struct Shares {
+  unsigned total, each, W, extra;
+  __device__ __forceinline__ Shares(unsigned total_, unsigned parts) : total(total_), W(parts) {
+    each = total / W;
+    extra = total - each * W;
+  }
+  // extra * w stays below W * W
+  __device__ __forceinline__ unsigned begin(unsigned w) const { return each * w + extra * w / W; }
+  // The part that holds unit u, from part w on up or down.
+  __device__ __forceinline__ unsigned holder(unsigned u, unsigned w) const {
+    while (begin(w) > u) --w;
+    while (w + 1 < W && begin(w + 1) <= u) ++w;
+    return w;
+  }
+};
 
-// The unit at place `at` of the batch's order (request, segment, unit); the
-// whole warp calls, 0 <= at < all_units.
-__device__ __forceinline__ Cursor seek(const Pool& p, const Problem& a, int segs, long long at) {
-  Cursor c;
-  c.segs = segs;
-  const int lane = threadIdx.x & 31;
-  long long before = 0;
-  for (int base = 0; base < a.B; base += 32) {
-    const int i = base + lane;
-    const long long mine = i < a.B ? (long long)units_of(keys_of(p, a, i)) * segs : 0;
-    long long incl = mine;
+// The batch in front of a warp: its units, and the place of any of them.
+struct Plan {
+  unsigned total;
+  int longest;
+  unsigned units, incl;  // of the request of this lane's number: units, units up to its end
+  __device__ __forceinline__ static unsigned scan(unsigned u) {
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const long long o = __shfl_up_sync(0xffffffffu, incl, off);
-      if (lane >= off) incl += o;
+      const unsigned o = __shfl_up_sync(0xffffffffu, u, off);
+      if ((int)(threadIdx.x & 31) >= off) u += o;
     }
-    const unsigned past = __ballot_sync(0xffffffffu, before + incl > at);
-    if (past) {
-      const int l = __ffs(past) - 1;
-      const long long rest = at - before - __shfl_sync(0xffffffffu, incl - mine, l);
-      c.request(p, a, base + l);
-      c.seg = (int)(rest / c.units);
-      c.unit = (int)(rest - (long long)c.seg * c.units);
-      return c;
-    }
-    before += __shfl_sync(0xffffffffu, incl, 31);
+    return u;
   }
-  c.b = a.B;
-  c.seg = c.unit = c.keys = c.units = 0;
-  return c;
-}
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-// Copies a unit's first nk rows into a stage (the rest of the stage keeps what
-// it held and is masked).  Copies are whole 16 bytes: up to 15 rows' worth of
-// parameters past nk, inside the head's padded rows.
-template <typename T, int G>
-__device__ __forceinline__ void load_unit(const Pool& p, long long row, int nk, uint32_t dst) {
-  using U = Unit<T, G>;
-  const int lane = threadIdx.x & 31;
-  const uint8_t* kc = p.kc + row * U::CR + lane * 16;
-  const uint8_t* vc = p.vc + row * U::CR + lane * 16;
-  const uint8_t* kp = static_cast<const uint8_t*>(p.kp) + row * U::PR + lane * 16;
-  const uint8_t* vp = static_cast<const uint8_t*>(p.vp) + row * U::PR + lane * 16;
-  dst += lane * 16;
-#pragma unroll
-  for (int i = 0; i < G; ++i)
-    if (i * 512 + lane * 16 < nk * U::CR) {
-      cp_async16(dst + U::kc + i * 512, kc + i * 512);
-      cp_async16(dst + U::vc + i * 512, vc + i * 512);
+  __device__ __forceinline__ Plan(const Pool& p, const Problem& a) {
+    const int lane = threadIdx.x & 31;
+    units = lane < a.B ? units_of(keys_of(p, a, lane)) : 0;
+    incl = scan(units);
+    unsigned sum = 0, most = units;
+    for (int i = lane + 32; i < a.B; i += 32) {
+      const unsigned u = units_of(keys_of(p, a, i));
+      sum += u;
+      most = max(most, u);
     }
-#pragma unroll
-  for (int i = 0; i < (kUnit * U::PR + 511) / 512; ++i)
-    if (i * 512 + lane * 16 < nk * U::PR) {
-      cp_async16(dst + U::kp + i * 512, kp + i * 512);
-      cp_async16(dst + U::vp + i * 512, vp + i * 512);
+    if (a.B > 32) sum = __reduce_add_sync(0xffffffffu, sum);
+    total = (sum + __shfl_sync(0xffffffffu, incl, 31)) * a.segs;
+    longest = __reduce_max_sync(0xffffffffu, most);
+  }
+  // The unit at place `at` < total of the batch's order.
+  __device__ __forceinline__ Cursor seek(const Pool& p, const Problem& a, unsigned at) const {
+    const int lane = threadIdx.x & 31;
+    Cursor c;
+    c.b = c.seg = c.unit = c.keys = c.units = 0;
+    unsigned mine = units, upto = incl;
+    for (int base = 0; base < a.B; base += 32) {
+      if (base > 0) {
+        mine = base + lane < a.B ? units_of(keys_of(p, a, base + lane)) : 0;
+        upto = scan(mine);
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, upto * a.segs > at);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        at -= (__shfl_sync(0xffffffffu, upto, l) - __shfl_sync(0xffffffffu, mine, l)) * a.segs;
+        c.request(p, a, base + l);
+        c.seg = at / (unsigned)c.units;
+        c.unit = at - c.seg * c.units;
+        return c;
+      }
+      at -= __shfl_sync(0xffffffffu, upto, 31) * a.segs;
     }
-}
+    return c;
+  }
+};
 
 // d = a b + c: a 16 x 32 signed or unsigned bytes, b 32 x 8 unsigned bytes.
 __device__ __forceinline__ void mma_s8u8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -185,12 +236,50 @@ __device__ __forceinline__ void mma_s8u8(int (&c)[4], const uint32_t (&a)[4], ui
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_s8u8_zero(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+}
 __device__ __forceinline__ void mma_u8u8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// A ticket word of this launch: zero (clean) or whatever another launch or other
+// use of the memory left becomes this launch's, with no tickets taken.  Every
+// CTA that will take a ticket calls this first, early on.
+__device__ __forceinline__ void open_tickets(unsigned long long* word, unsigned long long launch) {
+  unsigned long long seen = *reinterpret_cast<volatile unsigned long long*>(word);
+  if (seen >> 16 != launch) atomicCAS(word, seen, launch << 16);  // fails only where another CTA did it
+}
+// Takes a ticket; returns the tickets taken so far.  What the warp wrote before is
+// visible to whoever takes a later one.
+__device__ __forceinline__ unsigned take_ticket(unsigned long long* word) {
+  unsigned long long was;
+  asm volatile("atom.acq_rel.gpu.global.add.u64 %0, [%1], 1;" : "=l"(was) : "l"(word) : "memory");
+  return (unsigned)(was & 0xffff) + 1;
+}
+// Waits for a phase of an mbarrier; try_wait suspends the warp for a while, which
+// leaves the issue slots to the others.  Bounded (a few seconds): false and the
+// device error word when it gives up.
+__device__ __forceinline__ bool wait_copies(uint32_t bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
+    if (clock64() - t0 > kWaitBudgetCycles) break;
+  }
+  raise_device_error(DEV_ERR_ATTN_TIMEOUT);
+  return false;
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -239,14 +328,17 @@ __device__ __forceinline__ void lds_halves(const uint8_t* s, uint32_t* w) {
     }
   }
 }
-// A row's parameters, (s, z) per group; zeros unless ok.
+// A row's parameters, (s, z) per group; zeros unless ok (looked at where the
+// unit is `part`ial).
 template <typename T, int G>
-__device__ __forceinline__ void lds_params(const uint8_t* s, bool ok, float (&step)[G], float (&low)[G]) {
+__device__ __forceinline__ void lds_params(const uint8_t* s, bool part, bool ok, float (&step)[G], float (&low)[G]) {
   constexpr int N = 2 * G * (int)sizeof(T) / 4;
   uint32_t w[N];
   lds_words<N>(s, w);
+  if (part) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) w[i] = ok ? w[i] : 0u;
+    for (int i = 0; i < N; ++i) w[i] = ok ? w[i] : 0u;
+  }
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     if constexpr (std::is_same<T, float>::value) {
@@ -263,12 +355,26 @@ __device__ __forceinline__ void lds_params(const uint8_t* s, bool ok, float (&st
   }
 }
 
-// Balanced base-256 digit d (0: lowest) of x, |x| <= 127 (2^24 + 2^16 + 2^8 + 1).
-__device__ __forceinline__ uint32_t digit(int x, int d) {
-  // Adding 128 to every lower digit carries into the ones above as needed.
-  const uint32_t biased = (uint32_t)x + 0x00808080u;
-  const uint32_t byte = (biased >> (8 * d)) & 0xffu;
-  return d == 3 ? byte : byte ^ 0x80u;  // take the 128 off again, modulo 256
+// The four balanced base-256 digits of x, |x| <= 127 (2^24 + 2^16 + 2^8 + 1), a
+// signed byte each: adding 128 to the lower three carries into the ones above
+// as needed, and the 128s are taken off again modulo 256.
+__device__ __forceinline__ uint32_t digits_of(int x) { return ((uint32_t)x + 0x00808080u) ^ 0x00808080u; }
+
+// Eight consecutive channels of a row as they lie; channels past D give 0.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int c0, int D, bool vec, uint4 (&raw)[sizeof(T) / 2]) {
+  constexpr int N = (int)sizeof(T) / 2;
+  if (vec) {  // D a multiple of 8, rows 16-byte aligned
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      raw[i] = c0 < D ? reinterpret_cast<const uint4*>(p + c0)[i] : make_uint4(0, 0, 0, 0);
+  } else {
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = c0 + i < D ? p[c0 + i] : from_f32<T>(0.f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) raw[i] = reinterpret_cast<const uint4*>(e)[i];
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -294,53 +400,141 @@ __device__ __forceinline__ uint32_t digit(int x, int d) {
 // the rows that a quarter or half of the warp reads at once lie in distinct
 // banks (kv4.cuh).
 // ---------------------------------------------------------------------------
+// A running (maximum, sum, output) of a warp, V float4s of channels a lane, and
+// another share of the same segment.  One that saw no position counts nothing.
+template <int V>
+struct Running {
+  float m = -INFINITY, l = 0.f;
+  float4 x[V];
+  __device__ __forceinline__ Running() {
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __device__ __forceinline__ void add(float om, float ol, const float4 (&y)[V]) {
+    if (om == -INFINITY && ol == 0.f) return;
+    const float mn = fmaxf(m, om), fa = m == -INFINITY ? 0.f : ex2(m - mn), fb = ex2(om - mn);
+    m = mn;
+    l = fmaf(l, fa, fb * ol);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      x[v].x = fmaf(x[v].x, fa, fb * y[v].x);
+      x[v].y = fmaf(x[v].y, fa, fb * y[v].y);
+      x[v].z = fmaf(x[v].z, fa, fb * y[v].z);
+      x[v].w = fmaf(x[v].w, fa, fb * y[v].w);
+    }
+  }
+};
+// Four channels of an output row.
+template <typename T>
+__device__ __forceinline__ void store4(T* op, int c, int D, bool vec, float4 f) {
+  if (vec && sizeof(T) == 2) {  // D a multiple of 4, rows 8-byte aligned
+    if (c < D) {
+      T e[4] = {from_f32<T>(f.x), from_f32<T>(f.y), from_f32<T>(f.z), from_f32<T>(f.w)};
+      *reinterpret_cast<uint2*>(op + c) = *reinterpret_cast<const uint2*>(e);
+    }
+  } else {
+    if (c < D) op[c] = from_f32<T>(f.x);
+    if (c + 1 < D) op[c + 1] = from_f32<T>(f.y);
+    if (c + 2 < D) op[c + 2] = from_f32<T>(f.z);
+    if (c + 3 < D) op[c + 3] = from_f32<T>(f.w);
+  }
+}
+
 constexpr int kFlush = 1000;
 constexpr float kQMax = 1.2e8f;  // |16 q0 - q1| stays within four digits
 
 template <typename T, int G>
-__global__ void __launch_bounds__(kWarps * 32, Unit<T, G>::resident) attn_row_kernel(const Pool p, const Problem a) {
+__global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(const Pool p, const Problem a) {
   using U = Unit<T, G>;
-  constexpr int PP = Parts<T>::p, SETS = U::SETS;
+  constexpr int PP = Parts<T>::p, SETS = U::SETS, kWarps = U::warps, kStages = U::stages;
   constexpr float kPMax = PP == 3 ? 8388600.f : 65530.f;
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  uint8_t* ring = smem + warp * U::warp_bytes;
+  uint8_t* mem = smem + warp * U::warp_bytes;
+  uint8_t* ring = mem + U::stages_at;
   const uint32_t ring_u32 = smem_u32(ring);
-  float* dots = reinterpret_cast<float*>(ring + U::dots);
-  uint8_t* digits = ring + U::digits;
+  float* dots = reinterpret_cast<float*>(mem + U::dots);
+  uint8_t* digits = mem + U::digits;
   T* const out = static_cast<T*>(a.out);
   pdl_wait();
   pdl_trigger();
 
-  const int segs = a.QH * a.tq;
-  const long long w = (long long)blockIdx.x * kWarps + warp, nw = (long long)gridDim.x * kWarps;
-  // zeros for queries without a place in the pool
-  for (long long b = w; b < a.B; b += nw) {
-    const int keys = keys_of(p, a, (int)b), good = keys == 0 ? 0 : min(a.tq, keys - a.start_pos[b]);
+  const Plan plan(p, a);
+  const unsigned total = plan.total;
+  const bool by_segment = plan.longest <= kWholeUnits;
+  // a share of a few units at least: an empty one could not be joined
+  const Shares shares(total, by_segment ? gridDim.x : min(gridDim.x, (total + 3) / 4));
+  unsigned cta_begin = total, cta_end = total;
+  if (blockIdx.x < shares.W) {
+    cta_begin = shares.begin(blockIdx.x);
+    cta_end = shares.begin(blockIdx.x + 1);
+  }
+  Cursor cur = plan.seek(p, a, min(cta_begin, max(total, 1u) - 1));
+  if (by_segment && total > 0) {  // the segments that begin in the share
+    const Cursor tail = plan.seek(p, a, min(cta_end, total - 1));
+    if (cta_begin < total && cur.unit > 0) {
+      cta_begin += cur.units - cur.unit;
+      cur.next_segment(p, a);
+    }
+    if (cta_end < total && tail.unit > 0) cta_end += tail.units - tail.unit;
+    cta_end = max(cta_end, cta_begin);
+  }
+  const unsigned cta_units = cta_end - cta_begin;
+  const unsigned begin = cta_begin + cta_units * warp / kWarps;
+  int left = (int)(cta_begin + cta_units * (warp + 1) / kWarps - begin), ahead = left;
+  const int share_units = left;
+  const unsigned end = begin + left;
+  const bool busy = left > 0;
+  const Cursor cta_cur = cur;
+  if (busy) cur.skip(p, a, begin - cta_begin);
+  Cursor pre = cur;
+  const uint32_t bars = smem_u32(mem + U::bars);
+  const uint8_t* pre_head = nullptr;  // tiles of the head that `pre` is in
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(bars + 8 * i, 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+  // Copies the next unit's tile (rows past the last one are masked).
+  auto copy = [&](int stage) {
+    if (ahead == 0) return;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(bars + 8 * stage, U::bytes);
+      bulk_load(ring_u32 + stage * U::bytes, pre_head + (long long)pre.unit * U::bytes, U::bytes, bars + 8 * stage);
+    }
+    --ahead;
+    if (pre.next(p, a) && ahead > 0) pre_head = head_tiles(p, a.slot_of[pre.b], pre.seg / (a.group * a.tq));
+  };
+  if (busy) pre_head = head_tiles(p, a.slot_of[pre.b], pre.seg / (a.group * a.tq));
+#pragma unroll 1
+  for (int i = 0; i < kStages; ++i) copy(i);
+
+  // The segments that the share begins and ends in are other CTAs' too where they
+  // reach past it: their tickets' words.
+  if (!by_segment && cta_units > 0 && warp == 0) {
+    Cursor c = cta_cur;
+    unsigned at = cta_begin;
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+      const unsigned seg0 = at - c.unit;
+      if (seg0 < cta_begin || seg0 + c.units > cta_end) {
+        const unsigned word = shares.holder(seg0, blockIdx.x);
+        if (lane == 0) open_tickets(a.tickets + word, a.launch);
+      }
+      c.skip(p, a, cta_units - 1);
+      at += cta_units - 1;
+    }
+  }
+  // Zeros for queries without a place in the pool.
+  for (int b = blockIdx.x * kWarps + warp; b < a.B; b += gridDim.x * kWarps) {
+    const int keys = keys_of(p, a, b), good = keys == 0 ? 0 : min(a.tq, keys - a.start_pos[b]);
     if (good == a.tq) continue;
     if (lane == 0) raise_device_error(DEV_ERR_ATTN_RANGE);
     const long long n = (long long)(a.tq - good) * a.QH * p.D;
-    for (long long i = lane; i < n; i += 32) out[(b * a.tq + good) * a.QH * p.D + i] = from_f32<T>(0.f);
+    T* bad = out + ((long long)b * a.tq + good) * a.QH * p.D;
+    for (long long i = lane; i < n; i += 32) bad[i] = from_f32<T>(0.f);
   }
-  const long long total = all_units(p, a, segs);
-  const long long W = min(nw, total);
-  if (w >= W) return;  // every worker holds a unit
-  const long long begin = total * w / W, end = total * (w + 1) / W;
-  Cursor cur = seek(p, a, segs, begin), pre = cur;
-  long long left = end - begin, ahead = left;
-  auto prefetch = [&](int stage) {
-    if (ahead > 0) {
-      const int h = pre.seg / a.tq / a.group;
-      const long long row = head_row(p, a.slot_of[pre.b], h) + pre.unit * kUnit;
-      load_unit<T, G>(p, row, min(kUnit, pre.keys - pre.unit * kUnit), ring_u32 + stage * U::bytes);
-      pre.next(p, a);
-      --ahead;
-    }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) prefetch(i);
 
   // Offsets of this lane's reads within a stage.
   const int krow = (g & 1) ? 4 + ((g >> 1) ^ 1) : (g >> 1);  // position (of 8) that column g of a product stands for
@@ -356,8 +550,16 @@ __global__ void __launch_bounds__(kWarps * 32, Unit<T, G>::resident) attn_row_ke
   int accm[G][4], accr[G][4];                                // sums of P lo and of P (lo + 16 hi)
   int accm3[PP == 3 ? G : 1][4], accr3[PP == 3 ? G : 1][4];  // third digits
   float o[G][4], zacc[G], bound[G], to_int[G], m = -INFINITY, l = 0.f;
-  int stage = 0, since = 0, row_keys = 0;
-  bool fresh = true;
+  int stage = 0, since = 0;
+  uint32_t parity = 0;
+  bool live = true;
+  // The segments that this warp holds in part: the first and last of its share.
+  float* const parts = reinterpret_cast<float*>(mem + U::parts);
+  __shared__ unsigned part_seg0[kWarps][2];  // place of the segment's first unit
+  __shared__ int part_units[kWarps][2];      // its units; 0: none
+  __shared__ T* part_op[kWarps][2];
+  if (lane < 2) part_units[warp][lane] = 0;
+  __syncwarp();
 
   // Takes the integer sums over into o (channels 32 gi + 4 g .. + 3, valid in
   // the lanes whose columns are group gi's).
@@ -387,66 +589,96 @@ __global__ void __launch_bounds__(kWarps * 32, Unit<T, G>::resident) attn_row_ke
     since = 0;
   };
 
-  while (left > 0) {
-    if (fresh) {  // a segment begins: its query, empty sums
-      const int qh = cur.seg / a.tq, tok = cur.seg - qh * a.tq;
-      const T* qp = static_cast<const T*>(a.q) + cur.b * a.qs0 + tok * a.qs1 + qh * a.qs2;
-      row_keys = a.start_pos[cur.b] + tok + 1;
-      float x[G][8], big = 0.f;
-#pragma unroll
-      for (int gi = 0; gi < G; ++gi)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int c = gi * 32 + 8 * t + i;
-          x[gi][i] = c < p.D ? to_f32<T>(qp[c]) : 0.f;
-          big = fmaxf(big, fabsf(x[gi][i]));
-          if (!(fabsf(x[gi][i]) <= 3.402823466e38f)) big = INFINITY;
-        }
-      big = warp_max(big);
-      const bool sound = big <= 3.402823466e38f;
-      const float to_q = big > 0.f && sound ? fminf(kQMax / big, 1e37f) : 0.f;
-      // scores = (integer sums / 16) * unit_q + minima's share, in log2 units
-      unit_q = sound ? (to_q > 0.f ? 0.0625f / to_q * a.scale_log2 : 0.f) : NAN;
-#pragma unroll
-      for (int gi = 0; gi < G; ++gi) {
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum += x[gi][i];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        qsum[gi] = sum * a.scale_log2;
-        uint32_t r[4] = {0u, 0u, 0u, 0u};
-        if ((gi & 3) == (g & 3)) {
-          const int hi = g < 4 ? 3 : 1;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int q0 = __float2int_rn(x[gi][2 * i] * to_q), q1 = __float2int_rn(x[gi][2 * i + 1] * to_q);
-            const int q01 = 16 * q0 - q1;
-            r[0] |= digit(q01, hi) << (8 * i);
-            r[1] |= digit(q01, hi - 1) << (8 * i);
-            r[2] |= digit(q1, hi) << (8 * i);
-            r[3] |= digit(q1, hi - 1) << (8 * i);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          qa[gi][i] = r[i];
-          accm[gi][i] = accr[gi][i] = 0;
-          if constexpr (PP == 3) accm3[gi][i] = accr3[gi][i] = 0;
-          o[gi][i] = 0.f;
-        }
-        zacc[gi] = bound[gi] = to_int[gi] = 0.f;
-      }
-      m = -INFINITY;
-      l = 0.f;
-      since = 0;
-      fresh = false;
+  // A segment's query, as it lies: lane (g, t) holds channels 8 t .. 8 t + 7 of
+  // its own groups, every channel of the row in two lanes.  The next segment's
+  // is loaded a segment ahead.
+  uint4 q_raw[SETS][sizeof(T) / 2];
+  T* op = nullptr;
+  int row_keys = 0;
+  auto load_query = [&](const Cursor& c) {
+    int qh = c.seg, tok = 0;
+    if (a.tq > 1) {
+      qh = c.seg / a.tq;
+      tok = c.seg - qh * a.tq;
     }
-    cp_async_wait<kStages - 2>();
-    __syncwarp();
-    prefetch(stage == 0 ? kStages - 1 : stage - 1);
+    op = out + (((long long)c.b * a.tq + tok) * a.QH + qh) * p.D;
+    row_keys = a.start_pos[c.b] + tok + 1;
+    const T* qp = static_cast<const T*>(a.q) + c.b * a.qs0 + tok * a.qs1 + qh * a.qs2;
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) load8<T>(qp, (4 * s + (g & 3)) * 32 + 8 * t, p.D, a.q_vec, q_raw[s]);
+  };
+  if (busy) load_query(cur);
+
+  while (left > 0) {  // the share's segments
+    const int n_units = min(cur.units - cur.unit, left);
+    T* const seg_op = op;
+    const int seg_keys = row_keys;
+    float big = 0.f, x[SETS][8];
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) {
+      const T* e = reinterpret_cast<const T*>(q_raw[s]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[s][i] = to_f32<T>(e[i]);
+        big = fmaxf(big, fabsf(x[s][i]));
+        if (!(fabsf(x[s][i]) <= 3.402823466e38f)) big = INFINITY;
+      }
+    }
+    Cursor nxt = cur;
+    nxt.next_segment(p, a);
+    if (n_units < left) load_query(nxt);
+    big = warp_max(big);
+    const bool sound = big <= 3.402823466e38f;
+    const float to_q = big > 0.f && sound ? fminf(kQMax / big, 1e37f) : 0.f;
+    // scores = (integer sums / 16) * unit_q + minima's share, in log2 units
+    unit_q = sound ? (to_q > 0.f ? 0.0625f / to_q * a.scale_log2 : 0.f) : NAN;
+    const int hi = g < 4 ? 3 : 1;
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += x[s][i];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sum *= a.scale_log2;
+      uint32_t r[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int q0 = __float2int_rn(x[s][2 * i] * to_q), q1 = __float2int_rn(x[s][2 * i + 1] * to_q);
+        const uint32_t d0 = digits_of(16 * q0 - q1), d1 = digits_of(q1);
+        r[0] |= (d0 >> (8 * hi) & 0xffu) << (8 * i);
+        r[1] |= (d0 >> (8 * hi - 8) & 0xffu) << (8 * i);
+        r[2] |= (d1 >> (8 * hi) & 0xffu) << (8 * i);
+        r[3] |= (d1 >> (8 * hi - 8) & 0xffu) << (8 * i);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int gi = 4 * s + k;
+        if (gi < G) {
+          qsum[gi] = __shfl_sync(0xffffffffu, sum, 4 * k);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) qa[gi][i] = (g & 3) == k ? r[i] : 0u;
+        }
+      }
+    }
+#pragma unroll
+    for (int gi = 0; gi < G; ++gi) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        accm[gi][i] = accr[gi][i] = 0;
+        if constexpr (PP == 3) accm3[gi][i] = accr3[gi][i] = 0;
+        o[gi][i] = 0.f;
+      }
+      zacc[gi] = bound[gi] = to_int[gi] = 0.f;
+    }
+    m = -INFINITY;
+    l = 0.f;
+    since = 0;
+    for (int i = 0; i < n_units && live; ++i) {
+    live = __all_sync(0xffffffffu, wait_copies(bars + 8 * stage, parity >> stage & 1));
+    if (!live) break;
     const uint8_t* st = ring + stage * U::bytes;
-    const int nk = row_keys - cur.unit * kUnit;  // positions of the unit that the row attends
+    const int nk = seg_keys - (cur.unit + i) * kUnit;  // positions of the unit that the row attends
     if (nk > 0) {
       // ---- scores
       int c[SETS][4][4];
@@ -455,11 +687,10 @@ __global__ void __launch_bounds__(kWarps * 32, Unit<T, G>::resident) attn_row_ke
         uint32_t kw[G];
         lds_words<G>(st + k_off + nt * 8 * U::CR, kw);
 #pragma unroll
-        for (int s = 0; s < SETS; ++s)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) c[s][nt][e] = 0;
-#pragma unroll
-        for (int gi = 0; gi < G; ++gi) mma_s8u8(c[gi / 4][nt], qa[gi], kw[gi] & 0x0f0f0f0fu, kw[gi]);
+        for (int gi = 0; gi < G; ++gi) {
+          if (gi % 4 == 0) mma_s8u8_zero(c[gi / 4][nt], qa[gi], kw[gi] & 0x0f0f0f0fu, kw[gi]);
+          else mma_s8u8(c[gi / 4][nt], qa[gi], kw[gi] & 0x0f0f0f0fu, kw[gi]);
+        }
       }
 #pragma unroll
       for (int s = 0; s < SETS; ++s)
@@ -473,9 +704,9 @@ __global__ void __launch_bounds__(kWarps * 32, Unit<T, G>::resident) attn_row_ke
           *reinterpret_cast<float4*>(dots + s * 8 * 36 + g * 36 + t * 8 + 4 * i) = f;
         }
       __syncwarp();
-      const bool valid = my_pos < nk;
+      const bool part = nk < kUnit, valid = my_pos < nk;
       float step[G], low[G];
-      lds_params<T, G>(st + U::kp + my_pos * U::PR, valid, step, low);
+      lds_params<T, G>(st + U::kp + my_pos * U::PR, part, valid, step, low);
       float x = 0.f, y = 0.f;
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) {
@@ -485,7 +716,7 @@ __global__ void __launch_bounds__(kWarps * 32, Unit<T, G>::resident) attn_row_ke
       }
       const float sc = valid ? fmaf(x, unit_q, y) : -INFINITY;
       const float mx = warp_max(sc);
-      lds_params<T, G>(st + U::vp + my_pos * U::PR, valid, step, low);
+      lds_params<T, G>(st + U::vp + my_pos * U::PR, part, valid, step, low);
       bool grow = mx > m, over = false;
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) over |= step[gi] > bound[gi];
@@ -578,188 +809,179 @@ __global__ void __launch_bounds__(kWarps * 32, Unit<T, G>::resident) attn_row_ke
         }
       }
     }
+    __syncwarp();  // the stage is read
+    copy(stage);
+    parity ^= 1u << stage;
     stage = stage == kStages - 1 ? 0 : stage + 1;
-    --left;
-    const bool last = cur.unit + 1 == cur.units;
-    if (last || left == 0) {  // the segment, or this worker's share, ends here
-      const long long seg0 = end - left - 1 - cur.unit;  // place of the segment's first unit
-      const bool whole = last && seg0 >= begin;
-      flush();
-      l = warp_sum(l);
-      const int qh = cur.seg / a.tq, tok = cur.seg - qh * a.tq;
-      T* op = out + (((long long)cur.b * a.tq + tok) * a.QH + qh) * p.D;
-      float* wp = a.ws + (w * 2 + (seg0 <= begin ? 0 : 1)) * (4 + 32 * G);
-      if (!whole && lane == 0) {
-        wp[0] = m;
-        wp[1] = l;
-      }
-      const float inv = 1.0f / l;
-      const bool store = !whole || row_keys <= cur.keys;
+    }
+
+    // ---- the segment, or this share of it, ends
+    flush();
+    l = warp_sum(l);
+    const bool whole = n_units == cur.units;
+    const int which = left == share_units ? 0 : 1;
+    float* own = parts + which * U::share;
+    if (!whole && lane == 0) {
+      own[0] = m;
+      own[1] = l;
+      part_seg0[warp][which] = end - left - cur.unit;
+      part_units[warp][which] = cur.units;
+      part_op[warp][which] = seg_keys <= cur.keys ? seg_op : nullptr;  // null: a token outside the pool, zeros already
+    }
+    const float inv = 1.0f / l;
 #pragma unroll
-      for (int gi = 0; gi < G; ++gi) {
-        const float z = warp_sum(zacc[gi]);
-        float4 f;
-        f.x = o[gi][0] + __shfl_xor_sync(0xffffffffu, o[gi][0], 2) + z;
-        f.y = o[gi][1] + __shfl_xor_sync(0xffffffffu, o[gi][1], 2) + z;
-        f.z = o[gi][2] + __shfl_xor_sync(0xffffffffu, o[gi][2], 2) + z;
-        f.w = o[gi][3] + __shfl_xor_sync(0xffffffffu, o[gi][3], 2) + z;
-        if (t == (gi & 3) >> 1 && store) {
-          const int c = 32 * gi + 4 * g;
-          if (!whole) {
-            *reinterpret_cast<float4*>(wp + 4 + c) = f;
-          } else {
-            if (c < p.D) op[c] = from_f32<T>(f.x * inv);
-            if (c + 1 < p.D) op[c + 1] = from_f32<T>(f.y * inv);
-            if (c + 2 < p.D) op[c + 2] = from_f32<T>(f.z * inv);
-            if (c + 3 < p.D) op[c + 3] = from_f32<T>(f.w * inv);
-          }
+    for (int gi = 0; gi < G; ++gi) {
+      const float z = warp_sum(zacc[gi]);
+      float4 f;
+      f.x = o[gi][0] + __shfl_xor_sync(0xffffffffu, o[gi][0], 2) + z;
+      f.y = o[gi][1] + __shfl_xor_sync(0xffffffffu, o[gi][1], 2) + z;
+      f.z = o[gi][2] + __shfl_xor_sync(0xffffffffu, o[gi][2], 2) + z;
+      f.w = o[gi][3] + __shfl_xor_sync(0xffffffffu, o[gi][3], 2) + z;
+      if (t == (gi & 3) >> 1) {
+        const int c = 32 * gi + 4 * g;
+        if (!whole) {
+          *reinterpret_cast<float4*>(own + 4 + c) = f;
+        } else if (seg_keys <= cur.keys) {
+          f.x *= inv;
+          f.y *= inv;
+          f.z *= inv;
+          f.w *= inv;
+          store4<T>(seg_op, c, p.D, a.out_vec, f);
         }
       }
-      fresh = true;
     }
-    cur.next(p, a);
-    __syncwarp();
+    left -= n_units;
+    cur = nxt;
+    if (!live) break;
   }
-  cp_async_wait<0>();
+  // a wait gave up: let the copies in flight land before the warp exits
+  if (!live)
+    for (int i = 0; i < kStages; ++i) wait_copies(bars + 8 * i, parity >> i & 1);
+
+  // ---- segments held in part.  A warp joins those whose first share in this CTA
+  // is its own.
+  __syncthreads();
+  constexpr int V = (G + 3) / 4;  // float4s of a share per lane
+  // a share's float4 number v of this lane
+  auto in_share = [&](int v) { return v * 128 + lane * 4 < 32 * G; };
+#pragma unroll 1
+  for (int mine = 0; mine < 2; ++mine) {
+    const int units = part_units[warp][mine];
+    if (units == 0) continue;
+    const unsigned seg0 = part_seg0[warp][mine];
+    // begun in an earlier warp's part of the share: joined there
+    if (seg0 < begin && begin > cta_begin) continue;
+    T* const dest = part_op[warp][mine];
+    Running<V> run;
+    for (int w = warp; w < kWarps; ++w) {
+      const int k = w == warp ? mine : 0;
+      if (part_units[w][k] == 0 || part_seg0[w][k] != seg0) continue;
+      const float* sh = reinterpret_cast<const float*>(smem + w * U::warp_bytes + U::parts) + k * U::share;
+      float4 y[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        y[v] = in_share(v) ? reinterpret_cast<const float4*>(sh + 4)[v * 32 + lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+      run.add(sh[0], sh[1], y);
+    }
+    if (seg0 < cta_begin || seg0 + units > cta_end) {  // other CTAs hold parts of it
+      const unsigned w0 = shares.holder(seg0, blockIdx.x), w1 = shares.holder(seg0 + units - 1, blockIdx.x);
+      float* sh = a.ws + ((long long)blockIdx.x * 2 + (seg0 <= cta_begin ? 0 : 1)) * U::share;
+      if (lane == 0) __stcg(reinterpret_cast<float4*>(sh), make_float4(run.m, run.l, 0.f, 0.f));
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (in_share(v)) __stcg(reinterpret_cast<float4*>(sh + 4) + v * 32 + lane, run.x[v]);
+      __syncwarp();
+      unsigned taken = 0;
+      if (lane == 0) {
+        taken = take_ticket(a.tickets + w0);
+        if (taken == w1 - w0 + 1) a.tickets[w0] = 0;  // clean for the next launch
+      }
+      taken = __shfl_sync(0xffffffffu, taken, 0);
+      if (taken != w1 - w0 + 1) continue;
+      constexpr int kBatch = G > 4 ? 6 : 12;  // shares in flight
+      run = Running<V>();
+      for (unsigned w = w0; w <= w1; w += kBatch) {
+        float4 ml[kBatch], y[kBatch][V];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const unsigned wk = w + k;
+          // the segment is the last of the share that it starts in, the first of the others
+          const float* o2 = a.ws + ((long long)wk * 2 + (wk == w0 && shares.begin(wk) < seg0 ? 1 : 0)) * U::share;
+          const bool in = wk <= w1;
+          ml[k] = in ? __ldcg(reinterpret_cast<const float4*>(o2)) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            y[k][v] = in && in_share(v) ? __ldcg(reinterpret_cast<const float4*>(o2 + 4) + v * 32 + lane)
+                                        : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) run.add(ml[k].x, ml[k].y, y[k]);
+      }
+    }
+    if (dest == nullptr) continue;
+    const float inv = 1.0f / run.l;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      run.x[v].x *= inv;
+      run.x[v].y *= inv;
+      run.x[v].z *= inv;
+      run.x[v].w *= inv;
+      store4<T>(dest, v * 128 + lane * 4, p.D, a.out_vec, run.x[v]);
+    }
+  }
 }
 
-// Joins the workers' shares of a segment that more than one of them holds, in
-// the workers' order.  One CTA per worker: the one whose share begins inside a
-// segment, the first to do so, joins that segment.  Its threads take the
-// channels (times slices of the shares, so that a segment of hundreds of
-// shares is not one long chain of loads).
-constexpr int kJoinThreads = 256;
-constexpr int kJoinShares = 256;  // shares weighted at once
-
-template <typename T, int G>
-__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const Pool p, const Problem a, long long W) {
-  pdl_wait();
-  pdl_trigger();
-  constexpr int CH = 32 * G, SL = kJoinThreads / CH;  // channels, slices
-  __shared__ float weight[kJoinShares], sum_x[SL > 1 ? SL : 1][CH], red[kJoinThreads / 32];
-  __shared__ uint32_t place[kJoinShares];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int segs = a.QH * a.tq;
-  const long long total = all_units(p, a, segs);
-  W = min(W, total);
-  const long long mid = blockIdx.x + 1;  // the worker whose begin is looked at
-  if (mid >= W) return;
-  const Cursor c = seek(p, a, segs, total * mid / W);
-  const long long u0 = total * mid / W - c.unit, u1 = u0 + c.units;
-  if (c.unit == 0 || total * (mid - 1) / W > u0) return;
-  const long long w0 = mid - 1, w1 = (u1 * W - 1) / total;  // the worker of a unit u: the last with total * w / W <= u
-  const int qh = c.seg / a.tq, tok = c.seg - qh * a.tq;
-  if (a.start_pos[c.b] + tok >= p.max_seq) return;  // zeros already
-  T* op = static_cast<T*>(a.out) + (((long long)c.b * a.tq + tok) * a.QH + qh) * p.D;
-  constexpr int stride = 4 + CH;
-  float m = -INFINITY, l = 0.f, x = 0.f;  // x: this thread's channel over its slice of the shares
-  const int ch = tid % CH, sl = tid / CH;
-  for (long long base = w0; base <= w1; base += kJoinShares) {
-    const int n = (int)min((long long)kJoinShares, w1 + 1 - base);
-    float mine = -INFINITY, ml = 0.f;
-    if (tid < n) {
-      const long long w = base + tid;
-      const uint32_t at = (uint32_t)(w * 2 + (total * w / W >= u0 ? 0 : 1));
-      place[tid] = at;
-      mine = a.ws[(long long)at * stride];
-      ml = a.ws[(long long)at * stride + 1];
-    }
-    float mx = warp_max(mine);
-    __syncthreads();  // the previous round's weights are read
-    if (lane == 0) red[warp] = mx;
-    __syncthreads();
-    mx = m;
-#pragma unroll
-    for (int i = 0; i < kJoinThreads / 32; ++i) mx = fmaxf(mx, red[i]);
-    const float alpha = m == -INFINITY ? 0.f : ex2(m - mx);
-    m = mx;
-    // a share whose units are all masked has maximum -inf and counts nothing
-    const float f = tid < n && !(mine == -INFINITY && ml == 0.f) ? ex2(mine - m) : 0.f;
-    weight[tid] = f;
-    const float part = warp_sum(tid < n ? f * ml : 0.f);
-    __syncthreads();
-    if (lane == 0) red[warp] = part;
-    __syncthreads();
-    l *= alpha;
-#pragma unroll
-    for (int i = 0; i < kJoinThreads / 32; ++i) l += red[i];
-    x *= alpha;
-    if (sl < SL) {
-#pragma unroll 4
-      for (int i = sl; i < n; i += SL) x = fmaf(weight[i], a.ws[(long long)place[i] * stride + 4 + ch], x);
-    }
-  }
-  if (SL > 1) {
-    if (sl < SL) sum_x[sl][ch] = x;
-    __syncthreads();
-    x = 0.f;
-#pragma unroll
-    for (int i = 0; i < SL; ++i) x += sum_x[i][ch];
-  }
-  if (sl == 0 && ch < p.D) op[ch] = from_f32<T>(x / l);
+// A number that no other launch of this process uses, 48 bits, never 0; they
+// start at a place that memory written by others will hardly hold.
+static unsigned long long launch_number() {
+  static std::atomic<unsigned long long> next{
+      (unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count() * 0x9e3779b97f4a7c15ull};
+  unsigned long long n;
+  do n = next.fetch_add(1, std::memory_order_relaxed) & 0xffffffffffffull;
+  while (n == 0);
+  return n;
 }
 
 template <typename T, int G>
 static int launch_row(const Pool& p, const Problem& a, int grid, cudaStream_t st) {
-  constexpr int smem = kWarps * Unit<T, G>::warp_bytes;
-  static bool attr_set[64] = {};
+  static std::atomic<bool> ready[64] = {};
   const int dev = current_device();
-  if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(attn_row_kernel<T, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (dev < 0 || dev >= 64) return fail(FML_EUNSUPPORTED, "neb_kv4_attention: device index out of range");
+  if (!ready[dev].load()) {
+    const cudaError_t e = cudaFuncSetAttribute(attn_row_kernel<T, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               Unit<T, G>::cta_bytes);
     if (e != cudaSuccess) return check_cuda(e, "neb_kv4_attention smem attribute");
-    attr_set[dev] = true;
+    ready[dev].store(true);
   }
-  cudaError_t e = launch_pdl(attn_row_kernel<T, G>, dim3((unsigned)grid), dim3(kWarps * 32), smem, st, 1, p, a);
+  const cudaError_t e = launch_pdl(attn_row_kernel<T, G>, dim3((unsigned)grid), dim3(Unit<T, G>::warps * 32),
+                                   Unit<T, G>::cta_bytes, st, 1, p, a);
   count_launch();
-  if (e != cudaSuccess) return check_cuda(e, "neb_kv4_attention launch");
-  const long long W = (long long)grid * kWarps;
-  if (W < 2) return FML_OK;
-  e = launch_pdl(attn_join_kernel<T, G>, dim3((unsigned)(W - 1)), dim3(kJoinThreads), 0, st, 1, p, a, W);
-  count_launch();
-  return check_cuda(e, "neb_kv4_attention join launch");
+  return check_cuda(e, "neb_kv4_attention launch");
 }
 
-// The row kernel's grid: a whole number of resident CTAs per SM, no more
-// workers than the longest batch has units.
-template <typename T, int G>
-static int row_grid(const Pool& p, long long segments) {
-  const long long units = segments * ((p.max_seq + kUnit - 1) / kUnit);
-  return (int)std::min<long long>((long long)Unit<T, G>::resident * num_sms(current_device()), (units + kWarps - 1) / kWarps);
-}
-
-#define KV4_GROUPS(CALL) \
-  switch (p.G) {         \
-    case 1: CALL(1);     \
-    case 2: CALL(2);     \
-    case 3: CALL(3);     \
-    case 4: CALL(4);     \
-    case 5: CALL(5);     \
-    case 6: CALL(6);     \
-    case 7: CALL(7);     \
-    default: CALL(8);    \
-  }
-
-template <typename T>
-static int grid_of(const Pool& p, long long segments) {
-#define CALL(G) return row_grid<T, G>(p, segments)
-  KV4_GROUPS(CALL)
-#undef CALL
-}
-
-static size_t workspace_bytes(const Pool& p, int dtype, int64_t batch, int64_t t, int64_t q_heads) {
-  const long long segs = batch * t * q_heads;
-  const int grid = dtype == FML_F32 ? grid_of<float>(p, segs)
-                   : dtype == FML_F16 ? grid_of<__half>(p, segs) : grid_of<__nv_bfloat16>(p, segs);
-  return (size_t)grid * kWarps * 2 * (4 + 32 * p.G) * sizeof(float);
+// The row kernel's CTAs: one per SM.  The workspace holds the shares of every
+// CTA, then the tickets.
+static int row_grid() { return num_sms(current_device()); }
+static size_t shares_bytes(const Pool& p) { return (size_t)row_grid() * 2 * (4 + 32 * p.G) * sizeof(float); }
+static size_t workspace_bytes(const Pool& p) {
+  return shares_bytes(p) + (size_t)row_grid() * sizeof(unsigned long long);
 }
 
 template <typename T>
-static int attention(const Pool& p, const Problem& a, cudaStream_t st) {
-  const int grid = grid_of<T>(p, (long long)a.B * a.tq * a.QH);
-#define CALL(G) return launch_row<T, G>(p, a, grid, st)
-  KV4_GROUPS(CALL)
-#undef CALL
+static int attention(const Pool& p, Problem a, cudaStream_t st) {
+  const int grid = row_grid();
+  a.tickets = reinterpret_cast<unsigned long long*>(reinterpret_cast<uint8_t*>(a.ws) + shares_bytes(p));
+  a.launch = launch_number();
+  switch (p.G) {
+    case 1: return launch_row<T, 1>(p, a, grid, st);
+    case 2: return launch_row<T, 2>(p, a, grid, st);
+    case 3: return launch_row<T, 3>(p, a, grid, st);
+    case 4: return launch_row<T, 4>(p, a, grid, st);
+    case 5: return launch_row<T, 5>(p, a, grid, st);
+    case 6: return launch_row<T, 6>(p, a, grid, st);
+    case 7: return launch_row<T, 7>(p, a, grid, st);
+    default: return launch_row<T, 8>(p, a, grid, st);
+  }
 }
 
 }  // namespace kv4
@@ -771,7 +993,7 @@ extern "C" size_t neb_kv4_attention_workspace_size(const neb_kv4_pool* pool, int
                                                    int64_t q_heads) {
   kv4::Pool p;
   if (kv4::pool_from(pool, "neb_kv4_attention_workspace_size", &p) || batch <= 0 || t <= 0 || q_heads <= 0) return 0;
-  return kv4::workspace_bytes(p, pool->dtype, batch, t, q_heads);
+  return kv4::workspace_bytes(p);
 }
 
 extern "C" int neb_kv4_attention(const void* q, const int64_t q_strides[4], const neb_kv4_pool* pool,
@@ -787,27 +1009,40 @@ extern "C" int neb_kv4_attention(const void* q, const int64_t q_strides[4], cons
   if (t > p.max_seq) return fail(FML_EINVAL, "neb_kv4_attention: t exceeds max_seq");
   if (batch > (1 << 24) || q_heads > (1 << 20) || batch * t > (1ll << 31) / q_heads / 8)
     return fail(FML_EUNSUPPORTED, "neb_kv4_attention: too many queries");
-  const size_t need = kv4::workspace_bytes(p, pool->dtype, batch, t, q_heads);
+  const size_t need = kv4::workspace_bytes(p);
   if (workspace_bytes < need || (need && !workspace))
     return fail(FML_EWORKSPACE, "neb_kv4_attention: workspace of " + std::to_string(need) + " bytes needed");
   if (reinterpret_cast<uintptr_t>(workspace) & 15)
     return fail(FML_EINVAL, "neb_kv4_attention: workspace must be 16-byte aligned");
   kv4::Problem a = {};
-  a.slot_of = slot_of;
-  a.start_pos = start_pos;
-  a.B = (int)batch;
   a.tq = (int)t;
   a.QH = (int)q_heads;
   a.group = (int)(q_heads / p.H);
+  a.segs = (int)(t * q_heads);
   a.qs0 = q_strides[0];
   a.qs1 = q_strides[1];
   a.qs2 = q_strides[2];
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.q = q;
-  a.out = out;
+  const size_t es = dtype_size(pool->dtype);
+  a.q_vec = p.D % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_strides[0] * es % 16 == 0 &&
+            q_strides[1] * es % 16 == 0 && q_strides[2] * es % 16 == 0;
+  a.out_vec = p.D % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0;
   a.ws = static_cast<float*>(workspace);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (pool->dtype == FML_F32) return kv4::attention<float>(p, a, st);
-  if (pool->dtype == FML_BF16) return kv4::attention<__nv_bfloat16>(p, a, st);
-  return kv4::attention<__half>(p, a, st);
+  // Units are counted in 31 bits: a larger batch goes in slices of requests.
+  const int64_t per_request = t * q_heads * ((p.max_seq + kv4::kUnit - 1) / kv4::kUnit);
+  const int64_t slice = std::min<int64_t>(batch, ((1ll << 31) - 1) / per_request);
+  if (slice == 0) return fail(FML_EUNSUPPORTED, "neb_kv4_attention: too many queries");
+  for (int64_t b = 0; b < batch; b += slice) {
+    a.B = (int)std::min(slice, batch - b);
+    a.slot_of = slot_of + b;
+    a.start_pos = start_pos + b;
+    a.q = static_cast<const uint8_t*>(q) + b * q_strides[0] * (int64_t)es;
+    a.out = static_cast<uint8_t*>(out) + b * t * q_heads * p.D * (int64_t)es;
+    const int rc = pool->dtype == FML_F32    ? kv4::attention<float>(p, a, st)
+                   : pool->dtype == FML_BF16 ? kv4::attention<__nv_bfloat16>(p, a, st)
+                                             : kv4::attention<__half>(p, a, st);
+    if (rc != FML_OK) return rc;
+  }
+  return FML_OK;
 }

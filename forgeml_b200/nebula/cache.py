@@ -109,20 +109,15 @@ class KV4Pool:
             device = torch.device("cuda", torch.cuda.current_device())
         self.slots, self.heads, self.max_seq_len, self.head_dim = slots, heads, max_seq_len, head_dim
         self.device, self.dtype = device, dtype
-        groups, rows = -(-head_dim // 32), -(-max_seq_len // 16) * 16
-        codes, params = (slots, heads, rows, 16 * groups), (slots, heads, rows, groups, 2)
-        self.k_codes = torch.empty(codes, device=device, dtype=torch.uint8)
-        self.v_codes = torch.empty(codes, device=device, dtype=torch.uint8)
-        self.k_params = torch.empty(params, device=device, dtype=dtype)
-        self.v_params = torch.empty(params, device=device, dtype=dtype)
-        self._struct = _native.neb_kv4_pool(
-            self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_params.data_ptr(), self.v_params.data_ptr(),
-            slots, heads, max_seq_len, head_dim, _native.dtype_code(dtype))
+        code = _native.dtype_code(dtype)
+        self.data = torch.empty(_native.load().neb_kv4_pool_bytes(slots, heads, max_seq_len, head_dim, code),
+                                device=device, dtype=torch.uint8)
+        self._struct = _native.neb_kv4_pool(self.data.data_ptr(), slots, heads, max_seq_len, head_dim, code)
         self.handle = ctypes.byref(self._struct)
 
     @property
     def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.k_codes, self.v_codes, self.k_params, self.v_params))
+        return self.data.numel()
 
 
 class KVCache:

@@ -238,11 +238,10 @@ FML_API int neb_kv_append(const void* k, const int64_t k_strides[4],
  * c = rint((x - z) / s) in 0..15 (ties to even; 0 where s is 0), and stands
  * for z + c * s.  A group that holds an infinity or a NaN reads back as NaN.
  *
- * One layer's pool: codes [slots, heads, rows, 16 G] bytes and params
- * [slots, heads, rows, G, 2] (s, z) in dtype, for keys and for values, with
- * G = ceil(head_dim / 32) and rows = max_seq rounded up to 16; each tensor
- * 16-byte aligned, neb_kv4_codes_bytes / neb_kv4_params_bytes long.  The
- * order of the codes within a row is the kernels' own.
+ * One layer's pool is one piece of memory of neb_kv4_pool_bytes, 128-byte
+ * aligned: [slots, heads, ceil(max_seq / 32)] tiles of 32 positions.  The
+ * order of codes and parameters within a tile is the kernels' own
+ * (csrc/kv4.cuh).
  *
  * Request b of a batch holds slot slot_of[b] (int32, device) and its rows
  * begin at start_pos[b] (int32, device).  A slot or position outside the pool
@@ -250,16 +249,12 @@ FML_API int neb_kv_append(const void* k, const int64_t k_strides[4],
  * its outputs are zeros (read, attention).  head_dim <= 256.
  * ------------------------------------------------------------------------- */
 typedef struct neb_kv4_pool {
-  void* k_codes;
-  void* v_codes;
-  void* k_params;
-  void* v_params;
+  void* data;
   int64_t slots, heads, max_seq, head_dim;
   int32_t dtype;
 } neb_kv4_pool;
 
-FML_API size_t neb_kv4_codes_bytes(int64_t slots, int64_t heads, int64_t max_seq, int64_t head_dim);
-FML_API size_t neb_kv4_params_bytes(int64_t slots, int64_t heads, int64_t max_seq, int64_t head_dim, int dtype);
+FML_API size_t neb_kv4_pool_bytes(int64_t slots, int64_t heads, int64_t max_seq, int64_t head_dim, int dtype);
 /* Quantise k and v [B,T,H,D] (dtype of the pool, element strides, innermost 1)
  * into rows start_pos[b] .. start_pos[b]+T-1.  The requests of a batch hold
  * distinct slots; where a later one's rows overlap an earlier one's in the

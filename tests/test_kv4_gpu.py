@@ -40,9 +40,7 @@ def rows(b, n, h, d, dtype, seed, offset=True):
 
 def make_pool(cuda, slots, h, max_seq, d, dtype):
     pool = KV4Pool(slots=slots, heads=h, max_seq_len=max_seq, head_dim=d, device=cuda, dtype=dtype)
-    # rows nobody wrote: codes 15, parameters NaN
-    pool.k_codes.fill_(255), pool.v_codes.fill_(255)
-    pool.k_params.fill_(math.nan), pool.v_params.fill_(math.nan)
+    pool.data.fill_(255)  # rows nobody wrote: codes 15, parameters NaN
     return pool
 
 
@@ -51,8 +49,12 @@ def table(values, cuda):
 
 
 def snapshot(pool):
-    """The pool's bytes (NaN parameters compare equal to themselves)."""
-    return [t.clone().view(torch.uint8) for t in (pool.k_codes, pool.v_codes, pool.k_params, pool.v_params)]
+    """The pool's bytes: keys' codes and parameters, values' codes and parameters,
+    [slots, heads, rows, bytes] each."""
+    groups, es = -(-pool.head_dim // 32), torch.finfo(pool.dtype).bits // 8
+    widths = [16 * groups, 2 * groups * es] * 2
+    tiles = pool.data.clone().view(pool.slots, pool.heads, -1, 32 * sum(widths))
+    return [x.reshape(pool.slots, pool.heads, -1, w) for x, w in zip(tiles.split([32 * w for w in widths], -1), widths)]
 
 
 def check_values(got, want64, dtype):
@@ -123,7 +125,7 @@ def test_rows_read_back_as_their_definition(cuda, dtype, b, t, h, d):
     check_values(kr, orc.stands_for(k).transpose(1, 2), dtype)
     check_values(vr, orc.stands_for(v).transpose(1, 2), dtype)
     # every row not written is as it was
-    written = torch.zeros(b + 2, max_seq + (-max_seq) % 16, dtype=torch.bool, device=cuda)
+    written = torch.zeros(b + 2, max_seq + (-max_seq) % 32, dtype=torch.bool, device=cuda)
     for i in range(b):
         written[int(slots[i]), int(starts[i]):int(starts[i]) + t] = True
     keep = ~written[:, None].expand(-1, h, -1)
@@ -346,7 +348,7 @@ def test_rows_beyond_four_gigabytes(cuda):
     """Codes at byte offsets past 32 bits (the pool's memory is mostly untouched)."""
     dtype, h, d, max_seq, slots = torch.bfloat16, 16, 128, 8192, 530
     pool = KV4Pool(slots=slots, heads=h, max_seq_len=max_seq, head_dim=d, device=cuda, dtype=dtype)
-    assert pool.k_codes.numel() > 1 << 32
+    assert pool.nbytes > 1 << 33
     n = 33
     k, v = rows(2, n, h, d, dtype, seed=8)
     sl = table([slots - 1, 7], cuda)

@@ -128,17 +128,16 @@ def test_read_refuses_bad_counts_and_out(count, out, match):
 def test_pool_sizes():
     lib = _native.load()
     for slots, heads, seq, d in ((1, 1, 1, 1), (3, 2, 17, 80), (32, 16, 2048, 128), (2, 1, 100, 256)):
-        n = slots * heads * -(-seq // 16) * 16 * -(-d // 32)
-        assert lib.neb_kv4_codes_bytes(slots, heads, seq, d) == 16 * n
-        assert lib.neb_kv4_params_bytes(slots, heads, seq, d, BF16) == 4 * n
-        assert lib.neb_kv4_params_bytes(slots, heads, seq, d, F32) == 8 * n
+        n = slots * heads * -(-seq // 32) * 32 * -(-d // 32)  # groups of all rows: keys and values, codes and (s, z)
+        assert lib.neb_kv4_pool_bytes(slots, heads, seq, d, BF16) == 2 * n * (16 + 4)
+        assert lib.neb_kv4_pool_bytes(slots, heads, seq, d, F32) == 2 * n * (16 + 8)
     for bad in ((0, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), (1, 1, 1, 0), (1, 1, 1, 257)):
-        assert lib.neb_kv4_codes_bytes(*bad) == 0
-    assert lib.neb_kv4_params_bytes(1, 1, 1, 1, 9) == 0
+        assert lib.neb_kv4_pool_bytes(*bad, BF16) == 0
+    assert lib.neb_kv4_pool_bytes(1, 1, 1, 1, 9) == 0
 
 
 def c_pool(**kw):
-    f = dict(k_codes=FAKE, v_codes=FAKE, k_params=FAKE, v_params=FAKE, slots=4, heads=2, max_seq=64, head_dim=64,
+    f = dict(data=FAKE, slots=4, heads=2, max_seq=64, head_dim=64,
              dtype=BF16)
     return ctypes.byref(_native.neb_kv4_pool(**{**f, **kw}))
 
@@ -152,11 +151,11 @@ def _rejects(name, code, match, *args):
 def test_c_entries_check_the_pool():
     s4 = _native.strides4((128, 128, 64, 1))
     for bad, code, match in ((None, EINVAL, "null pool"), (dict(dtype=7), EINVAL, "bad dtype"),
-                             (dict(v_params=None), EINVAL, "null pointer"), (dict(slots=0), EINVAL, "positive"),
+                             (dict(data=None), EINVAL, "null pointer"), (dict(slots=0), EINVAL, "positive"),
                              (dict(heads=-2), EINVAL, "positive"), (dict(max_seq=0), EINVAL, "positive"),
                              (dict(head_dim=300), EUNSUPPORTED, "head_dim > 256"),
                              (dict(max_seq=1 << 31), EUNSUPPORTED, "too large"),
-                             (dict(k_params=FAKE + 8), EINVAL, "16-byte aligned")):
+                             (dict(data=FAKE + 16), EINVAL, "128-byte aligned")):
         p = None if bad is None else c_pool(**bad)
         _rejects("neb_kv4_append", code, match, FAKE, s4, FAKE, s4, p, FAKE, FAKE, 1, 1, None)
         _rejects("neb_kv4_read", code, match, p, FAKE, None, 1, FAKE, FAKE, 1, None)
