@@ -63,13 +63,15 @@ struct Unit {
   static constexpr int bytes = 2 * vc;
   // A warp's shared memory beside its stages: the scores' parts [set][8][36]
   // fp32 (36: distinct banks), the weights' digits [set][8 or 16][32], an mbarrier
-  // per stage, its shares of the segments
+  // per stage, the fp32 output [4 G][32 lanes] that the integer sums are taken over
+  // into, its shares of the segments
   // that it holds in part (the first and the last).
   static constexpr int share = 4 + 32 * G;
   static constexpr int dots = 0;
   static constexpr int digits = dots + SETS * 8 * 36 * 4;
   static constexpr int bars = digits + SETS * (Parts<T>::p == 3 ? 16 : 8) * 32;
-  static constexpr int parts = bars + 64;
+  static constexpr int out = bars + 64;
+  static constexpr int parts = out + 4 * G * 32 * 4;
   static constexpr int stages_at = (parts + 2 * share * 4 + 127) / 128 * 128;
   static constexpr int room = 227 * 1024 - 2048;
   // Warps: by registers (the sums of every group, of three digits twice, beside
@@ -441,6 +443,7 @@ __device__ __forceinline__ void store4(T* op, int c, int D, bool vec, float4 f) 
 }
 
 constexpr int kFlush = 1000;
+constexpr float kToInt0 = 1e37f;  // before any weight was seen: the first one of any size is over the bound
 constexpr float kQMax = 1.2e8f;  // |16 q0 - q1| stays within four digits
 
 template <typename T, int G>
@@ -506,9 +509,22 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
     --ahead;
     if (pre.next(p, a) && ahead > 0) pre_head = head_tiles(p, a.slot_of[pre.b], pre.seg / (a.group * a.tq));
   };
+  // The first stages at once, a lane each.
   if (busy) pre_head = head_tiles(p, a.slot_of[pre.b], pre.seg / (a.group * a.tq));
+  {
+    const uint8_t* first = nullptr;
 #pragma unroll 1
-  for (int i = 0; i < kStages; ++i) copy(i);
+    for (int i = 0; i < kStages && ahead > 0; ++i) {
+      if (lane == i) first = pre_head + (long long)pre.unit * U::bytes;
+      --ahead;
+      if (pre.next(p, a) && ahead > 0) pre_head = head_tiles(p, a.slot_of[pre.b], pre.seg / (a.group * a.tq));
+    }
+    if (first != nullptr) {
+      mbar_arrive_expect_tx(bars + 8 * lane, U::bytes);
+      bulk_load(ring_u32 + lane * U::bytes, first, U::bytes, bars + 8 * lane);
+    }
+  }
+  __syncwarp();
 
   // The segments that the share begins and ends in are other CTAs' too where they
   // reach past it: their tickets' words.
@@ -549,7 +565,8 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
   float qsum[G], unit_q = 0.f;
   int accm[G][4], accr[G][4];                                // sums of P lo and of P (lo + 16 hi)
   int accm3[PP == 3 ? G : 1][4], accr3[PP == 3 ? G : 1][4];  // third digits
-  float o[G][4], zacc[G], bound[G], to_int[G], m = -INFINITY, l = 0.f;
+  float zacc[G], to_int[G], m = -INFINITY, l = 0.f;
+  float* const o = reinterpret_cast<float*>(mem + U::out) + lane;  // channel 32 gi + 4 g + i: o[(4 gi + i) * 32]
   int stage = 0, since = 0;
   uint32_t parity = 0;
   bool live = true;
@@ -561,24 +578,27 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
   if (lane < 2) part_units[warp][lane] = 0;
   __syncwarp();
 
-  // Takes the integer sums over into o (channels 32 gi + 4 g .. + 3, valid in
-  // the lanes whose columns are group gi's).
-  auto flush = [&]() {
+  // Takes the integer sums over into the output, times `scale` (channels 32 gi +
+  // 4 g .. + 3, valid in the lanes whose columns are group gi's).
+  auto flush = [&](float scale) {
 #pragma unroll
     for (int gi = 0; gi < G; ++gi) {
-      const float u = bound[gi] * (1.0f / kPMax);
+      const float u = __fdividef(scale, to_int[gi]);
       const float d1 = t < 2 ? (PP == 3 ? 65536.f : 256.f) * u : (PP == 3 ? 256.f : 1.f) * u;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int e = 2 * h + (gi & 1);
-        o[gi][2 * h] = fmaf((float)accm[gi][e], d1, o[gi][2 * h]);
-        o[gi][2 * h + 1] = fmaf((float)(accr[gi][e] - accm[gi][e]), d1 * 0.0625f, o[gi][2 * h + 1]);
+        float* const x = o + (4 * gi + 2 * h) * 32;
+        float x0 = fmaf((float)accm[gi][e], d1, x[0] * scale);
+        float x1 = fmaf((float)(accr[gi][e] - accm[gi][e]), d1 * 0.0625f, x[32] * scale);
         if constexpr (PP == 3) {
           if (t < 2) {
-            o[gi][2 * h] = fmaf((float)accm3[gi][e], u, o[gi][2 * h]);
-            o[gi][2 * h + 1] = fmaf((float)(accr3[gi][e] - accm3[gi][e]), u * 0.0625f, o[gi][2 * h + 1]);
+            x0 = fmaf((float)accm3[gi][e], u, x0);
+            x1 = fmaf((float)(accr3[gi][e] - accm3[gi][e]), u * 0.0625f, x1);
           }
         }
+        x[0] = x0;
+        x[32] = x1;
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -586,7 +606,6 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
         if constexpr (PP == 3) accm3[gi][e] = accr3[gi][e] = 0;
       }
     }
-    since = 0;
   };
 
   // A segment's query, as it lies: lane (g, t) holds channels 8 t .. 8 t + 7 of
@@ -629,9 +648,9 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
     if (n_units < left) load_query(nxt);
     big = warp_max(big);
     const bool sound = big <= 3.402823466e38f;
-    const float to_q = big > 0.f && sound ? fminf(kQMax / big, 1e37f) : 0.f;
+    const float to_q = big > 0.f && sound ? fminf(__fdividef(kQMax, big), 1e37f) : 0.f;
     // scores = (integer sums / 16) * unit_q + minima's share, in log2 units
-    unit_q = sound ? (to_q > 0.f ? 0.0625f / to_q * a.scale_log2 : 0.f) : NAN;
+    unit_q = sound ? (to_q > 0.f ? __fdividef(0.0625f, to_q) * a.scale_log2 : 0.f) : NAN;
     const int hi = g < 4 ? 3 : 1;
 #pragma unroll
     for (int s = 0; s < SETS; ++s) {
@@ -667,19 +686,26 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
       for (int i = 0; i < 4; ++i) {
         accm[gi][i] = accr[gi][i] = 0;
         if constexpr (PP == 3) accm3[gi][i] = accr3[gi][i] = 0;
-        o[gi][i] = 0.f;
+        o[(4 * gi + i) * 32] = 0.f;
       }
-      zacc[gi] = bound[gi] = to_int[gi] = 0.f;
+      zacc[gi] = 0.f;
+      to_int[gi] = kToInt0;
     }
     m = -INFINITY;
     l = 0.f;
-    since = 0;
+    since = -1;
     for (int i = 0; i < n_units && live; ++i) {
     live = __all_sync(0xffffffffu, wait_copies(bars + 8 * stage, parity >> stage & 1));
     if (!live) break;
     const uint8_t* st = ring + stage * U::bytes;
     const int nk = seg_keys - (cur.unit + i) * kUnit;  // positions of the unit that the row attends
     if (nk > 0) {
+      // The values' codes, loaded ahead of the scores: the exchange of their bytes
+      // fills the scores' waits.
+      uint32_t vw[8][(G + 1) / 2];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        lds_halves<G>(st + ((i & 1) ? v_off1 : v_off0) + (16 * (i >> 2) + 8 * ((i >> 1) & 1)) * U::CR, vw[i]);
       // ---- scores
       int c[SETS][4][4];
 #pragma unroll
@@ -717,50 +743,52 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
       const float sc = valid ? fmaf(x, unit_q, y) : -INFINITY;
       const float mx = warp_max(sc);
       lds_params<T, G>(st + U::vp + my_pos * U::PR, part, valid, step, low);
-      bool grow = mx > m, over = false;
+      // ---- weights, as integers up to kPMax
+      const float mn = fmaxf(m, mx);
+      const float pr = valid ? ex2(sc - mn) : 0.f;
+      float n[G];
+      bool over = false;
 #pragma unroll
-      for (int gi = 0; gi < G; ++gi) over |= step[gi] > bound[gi];
+      for (int gi = 0; gi < G; ++gi) {
+        n[gi] = fmaf(pr * step[gi], to_int[gi], 8388608.f);
+        over |= n[gi] > 8388608.f + kPMax;
+      }
       over = __any_sync(0xffffffffu, over);
-      if (grow || over || since == kFlush) {  // the same in every lane
-        flush();
+      if (mx > m || over || since == kFlush) {  // the same in every lane
+        const float alpha = ex2(m - mn);
+        m = mn;
+        if (since >= 0) {  // not the segment's first unit
+          flush(alpha);
+          l *= alpha;
+#pragma unroll
+          for (int gi = 0; gi < G; ++gi) zacc[gi] *= alpha;
+        }
+        since = 0;
         if (over) {
 #pragma unroll
           for (int gi = 0; gi < G; ++gi) {
             // a quarter of headroom, so that it moves seldom
-            const float s = warp_max(step[gi]);
-            if (s > bound[gi]) bound[gi] = fmaxf(1.25f * s, 1e-32f);
-            to_int[gi] = bound[gi] > 0.f ? kPMax / bound[gi] : 0.f;
-          }
-        }
-        if (grow) {
-          const float alpha = ex2(m - mx);
-          m = mx;
-          l *= alpha;
-#pragma unroll
-          for (int gi = 0; gi < G; ++gi) {
-            zacc[gi] *= alpha;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[gi][e] *= alpha;
+            const float big = 1.25f * warp_max(pr * step[gi]);
+            to_int[gi] = fminf(to_int[gi], __fdividef(kPMax, fmaxf(big, 1e-32f)));
+            n[gi] = fmaf(pr * step[gi], to_int[gi], 8388608.f);
           }
         }
       }
       ++since;
-
-      // ---- weights
-      const float pr = valid ? ex2(sc - m) : 0.f;
       l += pr;
 #pragma unroll
+      for (int gi = 0; gi < G; ++gi) zacc[gi] = fmaf(pr, low[gi], zacc[gi]);
+#pragma unroll
       for (int gi = 0; gi < G; ++gi) {
-        zacc[gi] = fmaf(pr, low[gi], zacc[gi]);
-        const uint32_t n = __float_as_uint(fmaf(pr * step[gi], to_int[gi], 8388608.f));
+        const uint32_t w = __float_as_uint(n[gi]);
         uint8_t* d = digits + (gi / 4) * (PP == 3 ? 16 : 8) * 32 + (gi & 3) * 32 + lane;
         if constexpr (PP == 3) {
-          d[0] = (uint8_t)((n >> 16) & 0x7f);
-          d[4 * 32] = (uint8_t)(n >> 8);
-          d[8 * 32] = (uint8_t)n;
+          d[0] = (uint8_t)((w >> 16) & 0x7f);
+          d[4 * 32] = (uint8_t)(w >> 8);
+          d[8 * 32] = (uint8_t)w;
         } else {
-          d[0] = (uint8_t)(n >> 8);
-          d[4 * 32] = (uint8_t)n;
+          d[0] = (uint8_t)(w >> 8);
+          d[4 * 32] = (uint8_t)w;
         }
       }
       __syncwarp();
@@ -773,10 +801,6 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
       }
 
       // ---- output: per word (two groups) the bytes of four rows change places
-      uint32_t vw[8][(G + 1) / 2];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        lds_halves<G>(st + ((i & 1) ? v_off1 : v_off0) + (16 * (i >> 2) + 8 * ((i >> 1) & 1)) * U::CR, vw[i]);
 #pragma unroll
       for (int wi = 0; wi < (G + 1) / 2; ++wi) {
         uint32_t by[2][4];  // [rows 0-3 / 4-7][byte of the word]
@@ -816,7 +840,7 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
     }
 
     // ---- the segment, or this share of it, ends
-    flush();
+    flush(1.f);
     l = warp_sum(l);
     const bool whole = n_units == cur.units;
     const int which = left == share_units ? 0 : 1;
@@ -828,15 +852,19 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
       part_units[warp][which] = cur.units;
       part_op[warp][which] = seg_keys <= cur.keys ? seg_op : nullptr;  // null: a token outside the pool, zeros already
     }
-    const float inv = 1.0f / l;
+    const float inv = __frcp_rn(l);
 #pragma unroll
     for (int gi = 0; gi < G; ++gi) {
       const float z = warp_sum(zacc[gi]);
       float4 f;
-      f.x = o[gi][0] + __shfl_xor_sync(0xffffffffu, o[gi][0], 2) + z;
-      f.y = o[gi][1] + __shfl_xor_sync(0xffffffffu, o[gi][1], 2) + z;
-      f.z = o[gi][2] + __shfl_xor_sync(0xffffffffu, o[gi][2], 2) + z;
-      f.w = o[gi][3] + __shfl_xor_sync(0xffffffffu, o[gi][3], 2) + z;
+      f.x = o[(4 * gi + 0) * 32];
+      f.x += __shfl_xor_sync(0xffffffffu, f.x, 2) + z;
+      f.y = o[(4 * gi + 1) * 32];
+      f.y += __shfl_xor_sync(0xffffffffu, f.y, 2) + z;
+      f.z = o[(4 * gi + 2) * 32];
+      f.z += __shfl_xor_sync(0xffffffffu, f.z, 2) + z;
+      f.w = o[(4 * gi + 3) * 32];
+      f.w += __shfl_xor_sync(0xffffffffu, f.w, 2) + z;
       if (t == (gi & 3) >> 1) {
         const int c = 32 * gi + 4 * g;
         if (!whole) {
