@@ -1,95 +1,156 @@
 // 4-bit key/value cache: rows quantised as they are written (neb_kv4_append)
 // and read back (neb_kv4_read).  Format: kv4.cuh.
+#include <algorithm>
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 #include "kv4.cuh"
 
 namespace fml {
 namespace kv4 {
 
-// Eight consecutive channels of one row as floats; channels past D give 0 and
-// ok[i] false.
+// Eight consecutive channels of a row as they lie; those past D repeat the
+// last real one (a thread without any repeats channel 0 of its group's first
+// thread, which changes neither minimum nor maximum).
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int c0, int D, float (&x)[8]) {
-  if (VEC) {
-    constexpr int N = (int)sizeof(T) / 2;  // 16-byte loads: 1 for 16-bit, 2 for fp32
-    uint4 raw[N];
+struct Row8 {
+  uint4 raw[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p, int c0, int D) {
+    if (VEC) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) raw[i] = reinterpret_cast<const uint4*>(p + c0)[i];
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = __ldcs(reinterpret_cast<const uint4*>(p + min(c0, D - 8)) + i);
+    } else {
+      T e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = p[min(c0 + i, D - 1)];
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const uint4*>(e)[i];
+    }
+  }
+  __device__ __forceinline__ void floats(float (&x)[8]) const {
     const T* e = reinterpret_cast<const T*>(raw);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(e[i]);
-  } else {
+  }
+};
+
+// Minimum and maximum of a group over its four neighbouring lanes; NaN where the
+// group holds one.  The 16-bit types compare two numbers at once, and maximum
+// and negated minimum travel together.
+__device__ __forceinline__ __nv_bfloat162 max2(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmax2_nan(a, b); }
+__device__ __forceinline__ __nv_bfloat162 min2(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmin2_nan(a, b); }
+__device__ __forceinline__ __half2 max2(__half2 a, __half2 b) { return __hmax2_nan(a, b); }
+__device__ __forceinline__ __half2 min2(__half2 a, __half2 b) { return __hmin2_nan(a, b); }
+template <typename T2, bool VEC, typename T>
+__device__ __forceinline__ void range16(const Row8<T, VEC>& r, float& lo, float& hi) {
+  const T2* e = reinterpret_cast<const T2*>(r.raw);
+  const T2 mx = max2(max2(e[0], e[1]), max2(e[2], e[3])), mn = min2(min2(e[0], e[1]), min2(e[2], e[3]));
+  // (maximum, -minimum) of the two halves
+  T2 both;
+  both.x = __hmax_nan(mx.x, mx.y);
+  both.y = __hneg(__hmin_nan(mn.x, mn.y));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = c0 + i < D ? to_f32<T>(p[c0 + i]) : 0.f;
+  for (int off = 1; off <= 2; off <<= 1) {
+    const uint32_t o = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<uint32_t*>(&both), off);
+    both = max2(both, *reinterpret_cast<const T2*>(&o));
+  }
+  hi = to_f32<T>(both.x);
+  lo = -to_f32<T>(both.y);
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void range(const Row8<T, VEC>& r, const float (&x)[8], float& lo, float& hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    range16<__nv_bfloat162>(r, lo, hi);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    range16<__half2>(r, lo, hi);
+  } else {
+    lo = hi = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      lo = fminf(lo, x[i]);
+      hi = fmaxf(hi, x[i]);
+    }
+    float sum = 0.f;  // NaN and infinities stay in it
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], 0.f, sum);
+    if (sum != sum) hi = INFINITY;
+#pragma unroll
+    for (int off = 1; off <= 2; off <<= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+    }
   }
 }
 
-// Codes of eight channels (n of them real) of a group whose four threads are
-// neighbouring lanes: the group's s and z, and the codes as eight nibbles.
+// Codes of eight channels of a group, as eight nibbles, and the group's s and z.
 //
 // Quotients.  d = (x - z) / 2 and u = s / 2 (halved so that the widest range
-// stays finite; scaled by a power of two when s is tiny so that 1 / u does):
-// with y = RN(1 / u), q0 = RN(d y), r = d - q0 u (exact), RN(q0 + r y) is the
-// correctly rounded d / u (Markstein 1990).  Numerators of at most 20 bits
-// and steps of at most 11 cannot round onto a border k + 1/2 that they do not
-// hit, so adding 1.5 * 2^23 (round to nearest even) gives the code of the
-// exact quotient for the 16-bit types.  For fp32 the exact remainder,
-// including what x - z lost, decides the borders.
-template <typename T>
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], int n, float& s_out, float& z_out) {
-  float lo = INFINITY, hi = -INFINITY;
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (i < n) {
-      lo = fminf(lo, x[i]);
-      hi = fmaxf(hi, x[i]);
-      bad |= !(fabsf(x[i]) <= 3.402823466e38f);
-    }
-  }
-  if (bad) hi = INFINITY;
-#pragma unroll
-  for (int off = 1; off <= 2; off <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-  }
-  const float half_range = fmaf(0.5f, hi, -0.5f * lo);
+// stays finite; scaled by a power of two when s is tiny so that 1 / u does).
+// With y near 1 / u, q0 = d y, r = d - q0 u (exact) and q = q0 + r y rounded
+// once, q is the quotient rounded to fp32 but for 2^-44 of it (Markstein's
+// correction step).  For the 16-bit types a quotient that is not itself a border
+// k + 1/2 is at least 2^-20 of it away from one, so q falls on a border only
+// where the quotient does, and adding 1.5 * 2^23 (to nearest, ties to even) gives
+// its code.  For fp32 the exact remainder, with what x - z lost, decides.
+constexpr float kRound = 12582912.f;  // 1.5 * 2^23
+template <typename T> __device__ __forceinline__ float smallest_normal();
+template <> __device__ __forceinline__ float smallest_normal<float>() { return 1.17549435e-38f; }
+template <> __device__ __forceinline__ float smallest_normal<__half>() { return 6.103515625e-05f; }
+template <> __device__ __forceinline__ float smallest_normal<__nv_bfloat16>() { return 1.17549435e-38f; }
+
+template <typename T, bool VEC>
+__device__ __forceinline__ uint32_t quantise8(const Row8<T, VEC>& row, float& s, float& z) {
+  float x[8], hi;
+  row.floats(x);
+  range(row, x, z, hi);
+  const float half_range = fmaf(0.5f, hi, -0.5f * z);
   if (!(half_range <= 3.402823466e38f)) {  // an infinity or a NaN in the group
-    s_out = z_out = NAN;
+    s = z = NAN;
     return 0u;
   }
-  // (max - min) / 15 rounded to T: for the 16-bit types the difference has few
-  // enough bits for one fp32 division; fp32 takes the 64-bit quotient.
-  float s;
-  if (sizeof(T) == 4) s = (float)(((double)hi - (double)lo) / 15.0);
-  else s = to_f32<T>(from_f32<T>(__fdiv_rn(half_range, 7.5f)));
-  s_out = s;
-  z_out = lo;
+  // s = (max - min) / 15 rounded to T.  The 16-bit types' differences have few
+  // enough bits for one fp32 quotient (by the same correction step, with the
+  // constant 1 / 7.5); fp32 takes the 64-bit one.
+  if constexpr (sizeof(T) == 4) {
+    s = (float)(((double)hi - (double)z) / 15.0);
+  } else {
+    constexpr float y = 1.0f / 7.5f;
+    const float q0 = half_range * y;
+    s = fmaf(fmaf(-q0, 7.5f, half_range), y, q0);
+    if (half_range < 1e-30f) s = __fdiv_rn(half_range, 7.5f);  // the remainder would underflow
+    s = to_f32<T>(from_f32<T>(s));
+  }
   if (s == 0.f) return 0u;
-  const float scale = s < 8.6736174e-19f ? 0.5f * 1.1529215e18f : 0.5f;  // 2^-60, 2^60
-  const float u = s * scale, y = __frcp_rn(u), z = -lo * scale;
-  uint32_t w = 0;
+  float scale = 0.5f;
+  if (s < 8.6736174e-19f) scale = 0.5f * 1.1529215e18f;  // 2^-60, 2^60
+  const float u = s * scale, zs = -z * scale;
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(u));
+  float q[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float d = fmaf(x[i], scale, z);
-    const float q0 = d * y;
-    float q = fmaf(fmaf(-q0, u, d), y, q0);
-    if (sizeof(T) == 4) {
-      float c = rintf(q);
+    const float d = fmaf(x[i], scale, zs), q0 = d * y;
+    q[i] = fmaf(fmaf(-q0, u, d), y, q0);
+    if constexpr (sizeof(T) == 4) {
+      float c = rintf(q[i]);
       const float xs = x[i] * scale, b = d - xs;
-      const float lost = (xs - (d - b)) + (z - b);  // x - z = d + lost exactly
+      const float lost = (xs - (d - b)) + (zs - b);  // x - z = d + lost exactly
       const float r = fmaf(-c, u, d) + lost, h = 0.5f * u;
       const bool odd = ((int)c & 1) != 0;
       if (r > h || (r == h && odd)) c += 1.f;
       else if (r < -h || (r == -h && odd)) c -= 1.f;
-      q = c;
+      q[i] = c;
     }
-    q = fminf(q, 15.f);
-    const uint32_t code = __float_as_uint(q + 12582912.f) & 0xfu;
-    if (i < n) w |= code << (4 * i);
   }
+  if (s < smallest_normal<T>()) {  // a step without all its bits: quotients may pass 15.5
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = fminf(q[i], 15.f);
+  }
+  // bits of kRound + code are those of kRound plus the code: 16^i of each, summed
+  uint32_t w = 0u - 0x4b400000u * 0x11111111u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w += __float_as_uint(q[i] + kRound) << (4 * i);
   return w;
 }
 
@@ -106,113 +167,174 @@ __device__ __forceinline__ bool written_before(const int32_t* slot_of, const int
   return __any_sync(0xffffffffu, dup);
 }
 
-// One thread: eight channels of one head of one token, keys and values.
-// blockIdx.y * blockDim.x + threadIdx.x = (head, group, quarter); tokens are
-// dealt to blockIdx.x.
+// The values' codes of a group's quarter q (channels 8 q .. 8 q + 7) are the half
+// words 2 q and 2 q + 1 of the row's order.  With an even number of groups two
+// neighbouring groups (lanes 4 apart) exchange one each, so that both move a
+// whole word: the even group's half words 2 q, the odd group's 2 q + 1.
+__device__ __forceinline__ uint32_t swap_halves(uint32_t w, bool odd) {
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? w : w >> 16, 4);  // low half counts
+  return odd ? __byte_perm(other, w, 0x7610) : __byte_perm(w, other, 0x5410);
+}
+
+// One thread: eight channels of one head, keys and values, of a run of a
+// request's tokens.  threadIdx.x (and blockIdx.y) = (head, group, quarter);
+// blockIdx.x = (request, run).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
     append_kernel(const T* __restrict__ k, long long ks0, long long ks1, long long ks2, const T* __restrict__ v,
                   long long vs0, long long vs1, long long vs2, const Pool p, const int32_t* __restrict__ slot_of,
-                  const int32_t* __restrict__ start_pos, int tq, int tokens) {
+                  const int32_t* __restrict__ start_pos, int tq, int run, int runs) {
   pdl_wait();
   pdl_trigger();
+  const int b = blockIdx.x / runs, t0 = (blockIdx.x - b * runs) * run;
+  const int slot = slot_of[b], start = start_pos[b];
+  // the run's tokens that have a place
+  int t1 = min(tq, t0 + run);
+  if (slot < 0 || slot >= p.slots || start < 0 || written_before(slot_of, start_pos, b, slot, start, tq)) t1 = t0;
+  else t1 = min(t1, max(t0, p.max_seq - min(start, p.max_seq)));
+  if (t1 < min(tq, t0 + run) && threadIdx.x == 0) raise_device_error(DEV_ERR_ATTN_RANGE);
   const int per_head = 4 * p.G;
   const int j = blockIdx.y * blockDim.x + threadIdx.x;
-  const int h = j / per_head;
-  const bool live = h < p.H;
-  const int part = j - h * per_head, g = part >> 2, quarter = part & 3;
-  const int c0 = g * kGroup + quarter * 8;
-  const int n = live ? max(0, min(8, p.D - c0)) : 0;
-  for (int row = blockIdx.x; row < tokens; row += gridDim.x) {
-    const int b = row / tq, t = row - b * tq;
-    const int slot = slot_of[b], start = start_pos[b];
-    if (slot < 0 || slot >= p.slots || start < 0 || start > p.max_seq - 1 - t ||
-        written_before(slot_of, start_pos, b, slot, start, tq)) {
-      if (threadIdx.x == 0) raise_device_error(DEV_ERR_ATTN_RANGE);
-      continue;
-    }
-    const int pos = start + t;
-    uint8_t* const tile = live ? head_tiles(p, slot, h) + (long long)(pos / kTile) * (2 * p.half) : nullptr;
-    const int r = pos % kTile;
-    float x[2][8];
-    if (n > 0) {
-      load8<T, VEC>(k + b * ks0 + t * ks1 + h * ks2, c0, p.D, x[0]);
-      load8<T, VEC>(v + b * vs0 + t * vs1 + h * vs2, c0, p.D, x[1]);
-    }
-#pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      float s, z;
-      const uint32_t w = quantise8<T>(x[kv], n, s, z);
-      if (live && quarter == 0) {
-        T* pr = reinterpret_cast<T*>(tile + kv * p.half + kTile * 16 * p.G) + (r * p.G + g) * 2;
-        pr[0] = from_f32<T>(s);
-        pr[1] = from_f32<T>(z);
+  const bool live = j < p.H * per_head;
+  const int h = live ? j / per_head : 0, part = live ? j - h * per_head : 0, g = part >> 2, quarter = part & 3;
+  const int c0 = g * kGroup + quarter * 8, n = min(8, max(0, p.D - c0));
+  const uint32_t real = n == 8 ? 0xffffffffu : (1u << (4 * n)) - 1;  // codes of real channels
+  const int src_c = n > 0 ? c0 : g * kGroup;  // a quarter without channels looks at its group's first
+  const T* kr = k + b * ks0 + t0 * ks1 + h * ks2;
+  const T* vr = v + b * vs0 + t0 * vs1 + h * vs2;
+  uint8_t* const tiles = head_tiles(p, max(slot, 0), h);
+  const bool pairs = (p.G & 1) == 0, odd = (g & 1) != 0;
+  const int k_at = k_byte(p.G, c0), v_at = v_byte(p.G, pairs ? (g & ~1) * kGroup + quarter * 8 + (odd ? 4 : 0) : c0, 0);
+#pragma unroll 2
+  for (int t = t0; t < t1; ++t, kr += ks1, vr += vs1) {
+    Row8<T, VEC> kx, vx;
+    kx.load(kr, src_c, p.D);
+    vx.load(vr, src_c, p.D);
+    const int pos = start + t, r = pos % kTile;
+    uint8_t* const tile = tiles + (long long)(pos / kTile) * (2 * p.half);
+    float ks, kz, vs, vz;
+    const uint32_t kw = quantise8(kx, ks, kz) & real;
+    const uint32_t vw = quantise8(vx, vs, vz) & real;
+    uint8_t* const vrow = tile + p.half + r * 16 * p.G;
+    const uint32_t vx2 = pairs ? swap_halves(vw, odd) : 0u;
+    if (live) {
+      *reinterpret_cast<uint32_t*>(tile + r * 16 * p.G + k_at) = kw;
+      if (pairs) {
+        *reinterpret_cast<uint32_t*>(vrow + (v_at ^ v_swizzle(p.G, pos))) = vx2;
+      } else {
+        *reinterpret_cast<uint16_t*>(vrow + v_at) = (uint16_t)vw;
+        *reinterpret_cast<uint16_t*>(vrow + v_at + 2 * p.G) = (uint16_t)(vw >> 16);
       }
-      if (kv == 0) {
-        if (live) *reinterpret_cast<uint32_t*>(tile + r * 16 * p.G + k_byte(p.G, c0)) = w;
-      } else if (live) {
-        uint8_t* vr = tile + p.half + r * 16 * p.G;
-        *reinterpret_cast<uint16_t*>(vr + v_byte(p.G, c0, pos)) = (uint16_t)w;
-        *reinterpret_cast<uint16_t*>(vr + v_byte(p.G, c0 + 4, pos)) = (uint16_t)(w >> 16);
+      if (quarter < 2) {  // the first lane writes the keys' parameters, the second the values'
+        T sz[2] = {from_f32<T>(quarter ? vs : ks), from_f32<T>(quarter ? vz : kz)};
+        uint8_t* at = tile + quarter * p.half + kTile * 16 * p.G + (r * p.G + g) * 2 * (int)sizeof(T);
+        if (sizeof(T) == 4) *reinterpret_cast<uint2*>(at) = *reinterpret_cast<uint2*>(sz);
+        else *reinterpret_cast<uint32_t*>(at) = *reinterpret_cast<uint32_t*>(sz);
       }
     }
   }
 }
 
 // z + c * s rounded to T, within T's finite range (a rounded-up step can carry
-// code 15 of the widest groups past it); NaN stays.
+// code 15 of the widest groups past it); NaN stays.  Eight channels of a group.
+// The 16-bit types work on pairs: a code under the exponent of 128 (or 1024) is
+// 128 + c, exact in both, and one fused product rounds once.
 template <typename T>
-__device__ __forceinline__ float largest();
-template <> __device__ __forceinline__ float largest<float>() { return 3.402823466e38f; }
-template <> __device__ __forceinline__ float largest<__half>() { return 65504.f; }
-template <> __device__ __forceinline__ float largest<__nv_bfloat16>() { return 3.3895313892515355e38f; }
-template <typename T>
-__device__ __forceinline__ float value_of(uint32_t code, float s, float z) {
-  const float x = fmaf((float)code, s, z);
-  return x > largest<T>() ? largest<T>() : x;
+__device__ __forceinline__ void values8(uint32_t w, T s, T z, uint4 (&out)[sizeof(T) / 2]) {
+  if constexpr (sizeof(T) == 4) {
+    float e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = fmaf((float)((w >> (4 * i)) & 0xf), s, z);
+      e[i] = x > 3.402823466e38f ? 3.402823466e38f : x;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) out[i] = reinterpret_cast<const uint4*>(e)[i];
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    const uint32_t exponent = kHalf ? 0x64006400u : 0x43004300u, top = kHalf ? 0x7bff7bffu : 0x7f7f7f7fu;
+    const T2 base = *reinterpret_cast<const T2*>(&exponent), most = *reinterpret_cast<const T2*>(&top);
+    T2 s2, z2;
+    s2.x = s2.y = s;
+    z2.x = z2.y = z;
+    uint32_t e[4];  // channels i and i + 4
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t c = ((w >> (4 * i)) & 0x000f000fu) | exponent;
+      const T2 x = min2(__hfma2(__hsub2(*reinterpret_cast<const T2*>(&c), base), s2, z2), most);
+      e[i] = *reinterpret_cast<const uint32_t*>(&x);
+    }
+    out[0] = make_uint4(__byte_perm(e[0], e[1], 0x5410), __byte_perm(e[2], e[3], 0x5410),
+                        __byte_perm(e[0], e[1], 0x7632), __byte_perm(e[2], e[3], 0x7632));
+  }
 }
 
-// out[b, h, i, :] = the numbers that row start + i of request b stands for.
-template <typename T>
+// out[b, h, i, :] = the numbers that row start + i of request b stands for.  A
+// thread: eight channels of one row, keys and values; blockIdx.y = (request,
+// head), the block's rows side by side, blockIdx.x and steps along the rows.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
     read_kernel(const Pool p, const int32_t* __restrict__ slot_of, const int32_t* __restrict__ start_pos, int count,
-                T* __restrict__ ko, T* __restrict__ vo, long long total) {
+                T* __restrict__ ko, T* __restrict__ vo, int heads_first) {
   pdl_wait();
   pdl_trigger();
-  const int per_row = 4 * p.G;
-  for (long long idx = (long long)blockIdx.x * blockDim.x + threadIdx.x; idx < total;
-       idx += (long long)gridDim.x * blockDim.x) {
-    const int part = (int)(idx % per_row), g = part >> 2;
-    const long long o = idx / per_row;  // output row: (b, h, i)
-    const int i = (int)(o % count);
-    const int h = (int)((o / count) % p.H), b = (int)(o / count / p.H);
-    const int c0 = g * kGroup + (part & 3) * 8;
-    const int slot = slot_of[b], start = start_pos ? start_pos[b] : 0;
-    const bool ok = slot >= 0 && slot < p.slots && start >= 0 && start <= p.max_seq - 1 - i;
-    if (!ok) raise_device_error(DEV_ERR_ATTN_RANGE);
-    const int pos = ok ? start + i : 0;
-    const uint8_t* const tile = ok ? head_tiles(p, slot, h) + (long long)(pos / kTile) * (2 * p.half) : nullptr;
-    const int r = pos % kTile;
+  const int per_row = 4 * p.G, rows = blockDim.x / per_row;
+  const int bh = blockIdx.y + heads_first, b = bh / p.H, h = bh - b * p.H;
+  const int sub = threadIdx.x / per_row, part = threadIdx.x - sub * per_row, g = part >> 2, quarter = part & 3;
+  const int slot = slot_of[b], start = start_pos ? start_pos[b] : 0;
+  const bool in_pool = slot >= 0 && slot < p.slots && start >= 0;
+  const uint8_t* const tiles = head_tiles(p, in_pool ? slot : 0, h);
+  const int c0 = g * kGroup + quarter * 8;
+  const bool pairs = (p.G & 1) == 0, odd = (g & 1) != 0;
+  const int k_at = k_byte(p.G, c0), v_at = v_byte(p.G, pairs ? (g & ~1) * kGroup + quarter * 8 + (odd ? 4 : 0) : c0, 0);
+#pragma unroll 2
+  for (int i0 = blockIdx.x * rows; i0 < count; i0 += gridDim.x * rows) {
+    const int i = i0 + sub;
+    const bool live = sub < rows && i < count;
+    const bool ok = in_pool && live && start <= p.max_seq - 1 - i;
+    if (live && !ok) raise_device_error(DEV_ERR_ATTN_RANGE);
+    const int pos = ok ? start + i : 0, r = pos % kTile;
+    const uint8_t* const tile = tiles + (long long)(pos / kTile) * (2 * p.half);
+    const int at = kTile * 16 * p.G + (r * p.G + g) * 2 * (int)sizeof(T);
+    uint32_t kw = 0, vw = 0;
+    T kp[2], vp[2];
+    kp[0] = kp[1] = vp[0] = vp[1] = from_f32<T>(0.f);
+    if (ok) {
+      const uint8_t* const vrow = tile + p.half + r * 16 * p.G;
+      kw = __ldcs(reinterpret_cast<const uint32_t*>(tile + r * 16 * p.G + k_at));
+      if (pairs)
+        vw = __ldcs(reinterpret_cast<const uint32_t*>(vrow + (v_at ^ v_swizzle(p.G, pos))));
+      else
+        vw = *reinterpret_cast<const uint16_t*>(vrow + v_at) |
+             (uint32_t) * reinterpret_cast<const uint16_t*>(vrow + v_at + 2 * p.G) << 16;
+      if (sizeof(T) == 4) {
+        *reinterpret_cast<uint2*>(kp) = *reinterpret_cast<const uint2*>(tile + at);
+        *reinterpret_cast<uint2*>(vp) = *reinterpret_cast<const uint2*>(tile + p.half + at);
+      } else {
+        *reinterpret_cast<uint32_t*>(kp) = *reinterpret_cast<const uint32_t*>(tile + at);
+        *reinterpret_cast<uint32_t*>(vp) = *reinterpret_cast<const uint32_t*>(tile + p.half + at);
+      }
+    }
+    if (pairs) vw = swap_halves(vw, odd);  // its own inverse
+    uint4 kx[sizeof(T) / 2], vx[sizeof(T) / 2];
+    values8<T>(kw, kp[0], kp[1], kx);
+    values8<T>(vw, vp[0], vp[1], vx);
+    if (!live) continue;
+    const long long o = ((long long)bh * count + i) * p.D + c0;
+    if (VEC) {
+      if (c0 < p.D) {
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      T* out = (kv ? vo : ko) + o * p.D;
-      float s = 0.f, z = 0.f;
-      uint32_t w = 0;
-      if (ok) {
-        const T* pr = reinterpret_cast<const T*>(tile + kv * p.half + kTile * 16 * p.G) + (r * p.G + g) * 2;
-        s = to_f32<T>(pr[0]);
-        z = to_f32<T>(pr[1]);
-        if (kv == 0) {
-          w = *reinterpret_cast<const uint32_t*>(tile + r * 16 * p.G + k_byte(p.G, c0));
-        } else {
-          const uint8_t* vr = tile + p.half + r * 16 * p.G;
-          w = *reinterpret_cast<const uint16_t*>(vr + v_byte(p.G, c0, pos)) |
-              (uint32_t) * reinterpret_cast<const uint16_t*>(vr + v_byte(p.G, c0 + 4, pos)) << 16;
+        for (int e = 0; e < (int)sizeof(T) / 2; ++e) {
+          __stcs(reinterpret_cast<uint4*>(ko + o) + e, kx[e]);
+          __stcs(reinterpret_cast<uint4*>(vo + o) + e, vx[e]);
         }
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c0 + e < p.D) out[c0 + e] = from_f32<T>(value_of<T>((w >> (4 * e)) & 0xf, s, z));
+    } else {
+      for (int e = 0; e < 8 && c0 + e < p.D; ++e) {
+        ko[o + e] = reinterpret_cast<const T*>(kx)[e];
+        vo[o + e] = reinterpret_cast<const T*>(vx)[e];
+      }
     }
   }
 }
@@ -226,7 +348,7 @@ int pool_from(const neb_kv4_pool* pool, const char* who, Pool* p) {
   if (pool->slots <= 0 || pool->heads <= 0 || pool->max_seq <= 0 || pool->head_dim <= 0)
     return fail(FML_EINVAL, name + ": sizes must be positive");
   if (pool->head_dim > kMaxD) return fail(FML_EUNSUPPORTED, name + ": head_dim > 256");
-  if (pool->slots > (1 << 30) || pool->heads > (1 << 20) || pool->max_seq > (1 << 30))
+  if (pool->slots > (1 << 30) || pool->heads > (1 << 18) || pool->max_seq > (1 << 30))
     return fail(FML_EUNSUPPORTED, name + ": pool too large");
   if (reinterpret_cast<uintptr_t>(pool->data) & 127) return fail(FML_EINVAL, name + ": the pool must be 128-byte aligned");
   p->data = static_cast<uint8_t*>(pool->data);
@@ -243,21 +365,23 @@ int pool_from(const neb_kv4_pool* pool, const char* who, Pool* p) {
 template <typename T>
 static int append(const void* k, const int64_t* ks, const void* v, const int64_t* vs, const Pool& p,
                   const int32_t* slot_of, const int32_t* start_pos, int64_t batch, int64_t t, cudaStream_t st) {
-  const int per_head = 4 * p.G;
-  const int lanes = p.H * per_head;
+  const int lanes = p.H * 4 * p.G;
   const int block = lanes >= 256 ? 256 : (lanes + 31) / 32 * 32;
-  const long long tokens = batch * t;
-  const unsigned gy = (unsigned)((lanes + block - 1) / block);
-  const long long gx = std::min<long long>(tokens, std::max<long long>(1, 148LL * 64 / gy));
-  constexpr int W = 8;
+  const long long gy = (lanes + block - 1) / block;
+  // Tokens per block: one while blocks are few, up to 16 where they are many
+  // (the request's look-ups and addresses are made once a block).
+  const long long spread = 148LL * 16;
+  const int run = (int)std::min<long long>(16, std::max<long long>(1, batch * t * gy / spread));
+  const long long runs = (t + run - 1) / run;
   auto addressable = [&](const void* x, const int64_t* s) {
-    return p.D % W == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && s[0] * sizeof(T) % 16 == 0 &&
+    return p.D % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && s[0] * sizeof(T) % 16 == 0 &&
            s[1] * sizeof(T) % 16 == 0 && s[2] * sizeof(T) % 16 == 0;
   };
   auto go = [&](auto kernel) {
-    return launch_pdl(kernel, dim3((unsigned)gx, gy), dim3(block), 0, st, 1, static_cast<const T*>(k),
-                      (long long)ks[0], (long long)ks[1], (long long)ks[2], static_cast<const T*>(v), (long long)vs[0],
-                      (long long)vs[1], (long long)vs[2], p, slot_of, start_pos, (int)t, (int)tokens);
+    return launch_pdl(kernel, dim3((unsigned)(batch * runs), (unsigned)gy), dim3(block), 0, st, 1,
+                      static_cast<const T*>(k), (long long)ks[0], (long long)ks[1], (long long)ks[2],
+                      static_cast<const T*>(v), (long long)vs[0], (long long)vs[1], (long long)vs[2], p, slot_of,
+                      start_pos, (int)t, run, (int)runs);
   };
   const bool vec = addressable(k, ks) && addressable(v, vs);
   const cudaError_t e = vec ? go(append_kernel<T, true>) : go(append_kernel<T, false>);
@@ -268,12 +392,25 @@ static int append(const void* k, const int64_t* ks, const void* v, const int64_t
 template <typename T>
 static int read(const Pool& p, const int32_t* slot_of, const int32_t* start_pos, int64_t count, void* ko, void* vo,
                 int64_t batch, cudaStream_t st) {
-  const long long total = batch * p.H * count * 4 * p.G;
-  const long long blocks = std::min<long long>((total + 255) / 256, 148LL * 64);
-  const cudaError_t e = launch_pdl(read_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, 1, p, slot_of, start_pos,
-                                   (int)count, static_cast<T*>(ko), static_cast<T*>(vo), total);
-  count_launch();
-  return check_cuda(e, "neb_kv4_read launch");
+  const int per_row = 4 * p.G;
+  const int rows = 256 / per_row;
+  const int block = (rows * per_row + 31) / 32 * 32;
+  const bool vec = p.D % 8 == 0 && reinterpret_cast<uintptr_t>(ko) % 16 == 0 && reinterpret_cast<uintptr_t>(vo) % 16 == 0;
+  const long long heads = batch * p.H;
+  for (long long first = 0; first < heads; first += 65535) {  // grid.y
+    const long long gy = std::min<long long>(65535, heads - first);
+    // up to four steps along the rows a block, where that leaves blocks enough
+    const long long steps = (count + rows - 1) / rows;
+    const long long gx = std::max<long long>(1, std::min(steps, std::max((steps + 3) / 4, 148LL * 16 / gy)));
+    auto go = [&](auto kernel) {
+      return launch_pdl(kernel, dim3((unsigned)gx, (unsigned)gy), dim3(block), 0, st, 1, p, slot_of, start_pos,
+                        (int)count, static_cast<T*>(ko), static_cast<T*>(vo), (int)first);
+    };
+    const cudaError_t e = vec ? go(read_kernel<T, true>) : go(read_kernel<T, false>);
+    count_launch();
+    if (e != cudaSuccess) return check_cuda(e, "neb_kv4_read launch");
+  }
+  return FML_OK;
 }
 
 }  // namespace kv4
