@@ -24,7 +24,7 @@ OUT_DIR = PKG / "_lib"
 OBJ_DIR = OUT_DIR / "obj"
 LIB_NAME = "libforgeml_b200.so"
 SOURCES = ["common.cu", "gemm.cu", "layernorm.cu", "attention.cu", "sdpa_tc.cu", "nebula_ops.cu", "allreduce.cu",
-           "kv4.cu", "kv4_attention.cu"]
+           "kv4.cu", "kv4_attention.cu", "kv4_tc.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

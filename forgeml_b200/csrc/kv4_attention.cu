@@ -22,11 +22,10 @@
 // maxima, sums and outputs are fp32.
 #include <algorithm>
 #include <atomic>
-#include <chrono>
 #include <string>
 #include <type_traits>
 
-#include "kv4.cuh"
+#include "kv4_attention.cuh"
 
 namespace fml {
 namespace kv4 {
@@ -86,151 +85,6 @@ struct Unit {
   static_assert(stages >= 2, "shared memory");
 };
 
-struct Problem {
-  const int32_t *slot_of, *start_pos;
-  int B, tq, QH, group;  // group: query heads of a key/value head
-  int segs;              // segments of a request: tq * QH
-  long long qs0, qs1, qs2;
-  bool q_vec, out_vec;  // 16-byte loads of q, 8-byte stores of the output
-  float scale_log2;  // softmax scale * log2(e)
-  const void* q;
-  void* out;
-  // Workspace: [CTA][first / last segment][4 + 32 G] fp32 (maximum, sum, -, -,
-  // output), then a ticket per CTA for the segment that starts in its share and
-  // ends in another's: 48 bits that name the launch (a word of any other launch
-  // counts as empty; the last taker clears it) and the tickets taken.
-  float* ws;
-  unsigned long long* tickets;
-  unsigned long long launch;
-};
-
-// Positions that request b's last query attends; 0 for a bad slot or position.
-__device__ __forceinline__ int keys_of(const Pool& p, const Problem& a, int b) {
-  const int slot = a.slot_of[b], start = a.start_pos[b];
-  if (slot < 0 || slot >= p.slots || start < 0 || start >= p.max_seq) return 0;
-  return min(start + a.tq, p.max_seq);
-}
-__device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / kUnit; }
-
-// Where a warp is: a request, one of its segments (query rows: head, then the
-// head's rows, tokens innermost), a unit of it.  Every segment of a request has
-// all of the request's units (an earlier token's last ones may be masked whole).
-struct Cursor {
-  int b, seg, unit, keys, units;
-  __device__ __forceinline__ void request(const Pool& p, const Problem& a, int nb) {
-    b = nb;
-    keys = units = 0;
-    while (b < a.B) {
-      keys = keys_of(p, a, b);
-      units = units_of(keys);
-      if (units > 0) break;
-      ++b;
-    }
-  }
-  __device__ __forceinline__ void next_segment(const Pool& p, const Problem& a) {
-    unit = 0;
-    if (++seg == a.segs) {
-      seg = 0;
-      request(p, a, b + 1);
-    }
-  }
-  // The next unit; true when it opens another segment.
-  __device__ __forceinline__ bool next(const Pool& p, const Problem& a) {
-    if (unit + 1 < units) {
-      ++unit;
-      return false;
-    }
-    next_segment(p, a);
-    return true;
-  }
-  // n units on.
-  __device__ __forceinline__ void skip(const Pool& p, const Problem& a, unsigned n) {
-    n += unit;
-    while (b < a.B) {
-      const unsigned here = (unsigned)(a.segs - seg) * units;
-      if (n < here) {
-        const unsigned k = n / (unsigned)units;
-        seg += k;
-        unit = n - k * units;
-        return;
-      }
-      n -= here;
-      seg = 0;
-      request(p, a, b + 1);
-    }
-  }
-};
-
-// Contiguous shares of `total` units: part w of W begins at unit total * w / W.
-struct Shares {
-  unsigned total, each, W, extra;
-  __device__ __forceinline__ Shares(unsigned total_, unsigned parts) : total(total_), W(parts) {
-    each = total / W;
-    extra = total - each * W;
-  }
-  // extra * w stays below W * W
-  __device__ __forceinline__ unsigned begin(unsigned w) const { return each * w + extra * w / W; }
-  // The part that holds unit u, from part w on up or down.
-  __device__ __forceinline__ unsigned holder(unsigned u, unsigned w) const {
-    while (begin(w) > u) --w;
-    while (w + 1 < W && begin(w + 1) <= u) ++w;
-    return w;
-  }
-};
-
-// The batch in front of a warp: its units, and the place of any of them.
-struct Plan {
-  unsigned total;
-  int longest;
-  unsigned units, incl;  // of the request of this lane's number: units, units up to its end
-  __device__ __forceinline__ static unsigned scan(unsigned u) {
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const unsigned o = __shfl_up_sync(0xffffffffu, u, off);
-      if ((int)(threadIdx.x & 31) >= off) u += o;
-    }
-    return u;
-  }
-  __device__ __forceinline__ Plan(const Pool& p, const Problem& a) {
-    const int lane = threadIdx.x & 31;
-    units = lane < a.B ? units_of(keys_of(p, a, lane)) : 0;
-    incl = scan(units);
-    unsigned sum = 0, most = units;
-    for (int i = lane + 32; i < a.B; i += 32) {
-      const unsigned u = units_of(keys_of(p, a, i));
-      sum += u;
-      most = max(most, u);
-    }
-    if (a.B > 32) sum = __reduce_add_sync(0xffffffffu, sum);
-    total = (sum + __shfl_sync(0xffffffffu, incl, 31)) * a.segs;
-    longest = __reduce_max_sync(0xffffffffu, most);
-  }
-  // The unit at place `at` < total of the batch's order.
-  __device__ __forceinline__ Cursor seek(const Pool& p, const Problem& a, unsigned at) const {
-    const int lane = threadIdx.x & 31;
-    Cursor c;
-    c.b = c.seg = c.unit = c.keys = c.units = 0;
-    unsigned mine = units, upto = incl;
-    for (int base = 0; base < a.B; base += 32) {
-      if (base > 0) {
-        mine = base + lane < a.B ? units_of(keys_of(p, a, base + lane)) : 0;
-        upto = scan(mine);
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, upto * a.segs > at);
-      if (past) {
-        const int l = __ffs(past) - 1;
-        at -= (__shfl_sync(0xffffffffu, upto, l) - __shfl_sync(0xffffffffu, mine, l)) * a.segs;
-        c.request(p, a, base + l);
-        c.seg = at / (unsigned)c.units;
-        c.unit = at - c.seg * c.units;
-        return c;
-      }
-      at -= __shfl_sync(0xffffffffu, upto, 31) * a.segs;
-    }
-    return c;
-  }
-};
-
 // d = a b + c: a 16 x 32 signed or unsigned bytes, b 32 x 8 unsigned bytes.
 __device__ __forceinline__ void mma_s8u8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -250,43 +104,6 @@ __device__ __forceinline__ void mma_u8u8(int (&c)[4], uint32_t a0, uint32_t a1, 
       "mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// A ticket word of this launch: zero (clean) or whatever another launch or other
-// use of the memory left becomes this launch's, with no tickets taken.  Every
-// CTA that will take a ticket calls this first, early on.
-__device__ __forceinline__ void open_tickets(unsigned long long* word, unsigned long long launch) {
-  unsigned long long seen = *reinterpret_cast<volatile unsigned long long*>(word);
-  if (seen >> 16 != launch) atomicCAS(word, seen, launch << 16);  // fails only where another CTA did it
-}
-// Takes a ticket; returns the tickets taken so far.  What the warp wrote before is
-// visible to whoever takes a later one.
-__device__ __forceinline__ unsigned take_ticket(unsigned long long* word) {
-  unsigned long long was;
-  asm volatile("atom.acq_rel.gpu.global.add.u64 %0, [%1], 1;" : "=l"(was) : "l"(word) : "memory");
-  return (unsigned)(was & 0xffff) + 1;
-}
-// Waits for a phase of an mbarrier; try_wait suspends the warp for a while, which
-// leaves the issue slots to the others.  Bounded (a few seconds): false and the
-// device error word when it gives up.
-__device__ __forceinline__ bool wait_copies(uint32_t bar, uint32_t parity) {
-  const long long t0 = clock64();
-  while (true) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    if (ok) return true;
-    if (clock64() - t0 > kWaitBudgetCycles) break;
-  }
-  raise_device_error(DEV_ERR_ATTN_TIMEOUT);
-  return false;
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 __device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll
@@ -463,7 +280,7 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
   pdl_wait();
   pdl_trigger();
 
-  const Plan plan(p, a);
+  const Plan<kUnit> plan(p, a);
   const unsigned total = plan.total;
   const bool by_segment = plan.longest <= kWholeUnits;
   // a share of a few units at least: an empty one could not be joined
@@ -473,9 +290,9 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
     cta_begin = shares.begin(blockIdx.x);
     cta_end = shares.begin(blockIdx.x + 1);
   }
-  Cursor cur = plan.seek(p, a, min(cta_begin, max(total, 1u) - 1));
+  Cursor<kUnit> cur = plan.seek(p, a, min(cta_begin, max(total, 1u) - 1));
   if (by_segment && total > 0) {  // the segments that begin in the share
-    const Cursor tail = plan.seek(p, a, min(cta_end, total - 1));
+    const Cursor<kUnit> tail = plan.seek(p, a, min(cta_end, total - 1));
     if (cta_begin < total && cur.unit > 0) {
       cta_begin += cur.units - cur.unit;
       cur.next_segment(p, a);
@@ -489,9 +306,9 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
   const int share_units = left;
   const unsigned end = begin + left;
   const bool busy = left > 0;
-  const Cursor cta_cur = cur;
+  const Cursor<kUnit> cta_cur = cur;
   if (busy) cur.skip(p, a, begin - cta_begin);
-  Cursor pre = cur;
+  Cursor<kUnit> pre = cur;
   const uint32_t bars = smem_u32(mem + U::bars);
   const uint8_t* pre_head = nullptr;  // tiles of the head that `pre` is in
   if (lane == 0) {
@@ -529,7 +346,7 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
   // The segments that the share begins and ends in are other CTAs' too where they
   // reach past it: their tickets' words.
   if (!by_segment && cta_units > 0 && warp == 0) {
-    Cursor c = cta_cur;
+    Cursor<kUnit> c = cta_cur;
     unsigned at = cta_begin;
 #pragma unroll 1
     for (int i = 0; i < 2; ++i) {
@@ -614,7 +431,7 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
   uint4 q_raw[SETS][sizeof(T) / 2];
   T* op = nullptr;
   int row_keys = 0;
-  auto load_query = [&](const Cursor& c) {
+  auto load_query = [&](const Cursor<kUnit>& c) {
     int qh = c.seg, tok = 0;
     if (a.tq > 1) {
       qh = c.seg / a.tq;
@@ -643,7 +460,7 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
         if (!(fabsf(x[s][i]) <= 3.402823466e38f)) big = INFINITY;
       }
     }
-    Cursor nxt = cur;
+    Cursor<kUnit> nxt = cur;
     nxt.next_segment(p, a);
     if (n_units < left) load_query(nxt);
     big = warp_max(big);
@@ -959,17 +776,6 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
   }
 }
 
-// A number that no other launch of this process uses, 48 bits, never 0; they
-// start at a place that memory written by others will hardly hold.
-static unsigned long long launch_number() {
-  static std::atomic<unsigned long long> next{
-      (unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count() * 0x9e3779b97f4a7c15ull};
-  unsigned long long n;
-  do n = next.fetch_add(1, std::memory_order_relaxed) & 0xffffffffffffull;
-  while (n == 0);
-  return n;
-}
-
 template <typename T, int G>
 static int launch_row(const Pool& p, const Problem& a, int grid, cudaStream_t st) {
   static std::atomic<bool> ready[64] = {};
@@ -1021,6 +827,8 @@ extern "C" size_t neb_kv4_attention_workspace_size(const neb_kv4_pool* pool, int
                                                    int64_t q_heads) {
   kv4::Pool p;
   if (kv4::pool_from(pool, "neb_kv4_attention_workspace_size", &p) || batch <= 0 || t <= 0 || q_heads <= 0) return 0;
+  if (q_heads % p.H == 0 && kv4::tc_covers(p, pool->dtype, t, q_heads / p.H))
+    return kv4::tc_workspace_bytes(p, batch, t, q_heads / p.H);
   return kv4::workspace_bytes(p);
 }
 
@@ -1037,7 +845,8 @@ extern "C" int neb_kv4_attention(const void* q, const int64_t q_strides[4], cons
   if (t > p.max_seq) return fail(FML_EINVAL, "neb_kv4_attention: t exceeds max_seq");
   if (batch > (1 << 24) || q_heads > (1 << 20) || batch * t > (1ll << 31) / q_heads / 8)
     return fail(FML_EUNSUPPORTED, "neb_kv4_attention: too many queries");
-  const size_t need = kv4::workspace_bytes(p);
+  const bool tc = kv4::tc_covers(p, pool->dtype, t, q_heads / p.H);
+  const size_t need = tc ? kv4::tc_workspace_bytes(p, batch, t, q_heads / p.H) : kv4::workspace_bytes(p);
   if (workspace_bytes < need || (need && !workspace))
     return fail(FML_EWORKSPACE, "neb_kv4_attention: workspace of " + std::to_string(need) + " bytes needed");
   if (reinterpret_cast<uintptr_t>(workspace) & 15)
@@ -1057,6 +866,15 @@ extern "C" int neb_kv4_attention(const void* q, const int64_t q_strides[4], cons
   a.out_vec = p.D % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0;
   a.ws = static_cast<float*>(workspace);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (tc) {
+    a.B = (int)batch;
+    a.slot_of = slot_of;
+    a.start_pos = start_pos;
+    a.q = q;
+    a.out = out;
+    a.out_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0;
+    return kv4::tc_attention(p, a, pool->dtype, st);
+  }
   // Units are counted in 31 bits: a larger batch goes in slices of requests.
   const int64_t per_request = t * q_heads * ((p.max_seq + kv4::kUnit - 1) / kv4::kUnit);
   const int64_t slice = std::min<int64_t>(batch, ((1ll << 31) - 1) / per_request);

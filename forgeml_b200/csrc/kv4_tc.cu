@@ -1,0 +1,696 @@
+// Attention of several query rows over the 4-bit key/value cache on the tcgen05
+// tensor cores: a prompt's tokens, a few drafted ones, query heads that share a
+// key/value head (16-bit types, head dim 64 or 128).
+//
+// A segment is a request's key/value head with up to 128 of its query rows (row =
+// token * group + query head within the group: UMMA M, the TMEM lanes).  Its
+// positions go by in blocks of 128, flash-attention schedule, warp-specialised:
+//
+//   warp 9     copies the cache's tiles (32 positions, one bulk copy each) into a
+//              ring;
+//   warps 4-7  turn a tile each into 16-bit operands: a lane takes a position's
+//              codes and writes z + c s, rounded once, into the swizzled key and
+//              value blocks (two of each).  A code under the exponent of 128 (fp16:
+//              1024) is a 16-bit number, two at a time; the channels of every eight
+//              stay in the order 0 4 1 5 2 6 3 7 that this leaves, in the queries
+//              too, and are put right where the output is written;
+//   warp 8     TMEM owner and single-thread UMMA issuer: S = Q K^T of block j + 1
+//              into the other of two TMEM score blocks while block j's softmax
+//              runs, O += P V into TMEM;
+//   warps 0-3  queries, softmax and epilogue, one row per thread.
+//
+// Rounded below fp32: the operands (keys, values) and P, to the cache's dtype, as
+// attention over a 16-bit cache rounds them.
+//
+// Work: either one segment per CTA (prompts: enough segments), or, for few
+// segments, equal shares of all blocks per CTA with the split segments joined by
+// the last CTA to arrive (kv4_attention.cuh).
+//
+// Every wait is bounded (DEV_ERR_ATTN_TIMEOUT); a CTA that gives up lets its
+// copies land and frees its TMEM before it exits.
+#include <string>
+#include <type_traits>
+
+#include "kv4_attention.cuh"
+
+namespace fml {
+namespace kv4 {
+namespace tc {
+
+constexpr int kRows = 128;   // query rows of a segment
+constexpr int kBlock = 128;  // positions of a block
+constexpr int kThreads = 320;
+constexpr int kDequant = 4, kMma = 8, kCopy = 9;  // first warps of the roles
+constexpr int kRing = 6;                          // tiles
+constexpr uint32_t kTmemCols = 512;               // two score blocks, the output
+
+template <int D>
+struct Smem {
+  static constexpr int G = D / 32, kSlabs = D / 64;  // 128-byte slabs along the head dim
+  static constexpr uint32_t kTileBytes = 2 * kTile * G * (16 + 4);
+  static constexpr uint32_t kOperand = kRows * D * 2;
+  static constexpr uint32_t q = 0, k = kOperand, v = 3 * kOperand, p = 5 * kOperand;
+  static constexpr uint32_t raw = p + kRows * kBlock * 2;
+  static constexpr uint32_t bars = raw + kRing * kTileBytes;
+  static constexpr uint32_t total = bars + 256 + 1024;  // 1024: alignment of the base
+  static_assert(total <= 227 * 1024, "shared memory");
+};
+enum Bar : int {
+  kQFull = 0, kRawFull = 1, kRawEmpty = kRawFull + kRing, kKFull = kRawEmpty + kRing, kKEmpty = kKFull + 2,
+  kVFull = kKEmpty + 2, kVEmpty = kVFull + 2, kSFull = kVEmpty + 2, kPFull = kSFull + 2, kOFull, kTogether, kNumBars
+};
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void sts4(uint32_t at, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// A word of eight codes as eight 16-bit numbers z + c s, in the order 0 4 1 5 2 6 3 7.
+// (fp16 stays within its finite range where a rounded-up step would leave it.)
+template <typename T>
+__device__ __forceinline__ uint4 operand8(uint32_t w, uint32_t sz) {
+  using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  const uint32_t exponent = kHalf ? 0x64006400u : 0x43004300u, top = 0x7bff7bffu;
+  const uint32_t ss = __byte_perm(sz, sz, 0x1010), zz = __byte_perm(sz, sz, 0x3232);
+  uint32_t e[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t c = ((w >> (4 * i)) & 0x000f000fu) | exponent;
+    T2 x = __hfma2(__hsub2(*reinterpret_cast<const T2*>(&c), *reinterpret_cast<const T2*>(&exponent)),
+                   *reinterpret_cast<const T2*>(&ss), *reinterpret_cast<const T2*>(&zz));
+    if constexpr (kHalf) x = __hmin2_nan(x, *reinterpret_cast<const T2*>(&top));
+    e[i] = *reinterpret_cast<const uint32_t*>(&x);
+  }
+  return make_uint4(e[0], e[1], e[2], e[3]);
+}
+
+// A part of a segment: its blocks [lo, hi) (those that its rows attend at all).
+struct Part {
+  int b, h, row0, rows;  // rows of the request's head: row0 .. row0 + rows - 1
+  int start, kend;       // request's first position; positions that some row attends
+  int lo, hi;
+  bool whole;
+  unsigned seg0, units;  // in the batch's order: the segment's first unit, its units
+  int which;             // first or last part of the CTA's share
+};
+using BlockCursor = Cursor<kBlock>;
+// The parts that this CTA works through, in order; every role walks alike.
+struct Walk {
+  bool shared;
+  int row_tiles, left;
+  unsigned at, begin;
+  BlockCursor cur;
+  __device__ __forceinline__ bool next(const Pool& p, const Problem& a, Part& o) {
+    if (left == 0) return false;
+    const int n = shared ? min(cur.units - cur.unit, left) : 1;
+    const int rows = a.group * a.tq;
+    o.b = cur.b;
+    o.h = cur.seg / row_tiles;
+    o.row0 = (cur.seg - o.h * row_tiles) * kRows;
+    o.rows = min(kRows, rows - o.row0);
+    o.start = a.start_pos[cur.b];
+    o.kend = min(cur.keys, o.start + (o.row0 + o.rows - 1) / a.group + 1);
+    const int blocks = (o.kend + kBlock - 1) / kBlock;
+    o.lo = shared ? cur.unit : 0;
+    o.hi = shared ? max(o.lo, min(cur.unit + n, blocks)) : blocks;
+    o.whole = !shared || n == cur.units;
+    o.units = cur.units;
+    o.which = at == begin ? 0 : 1;
+    o.seg0 = at - cur.unit;
+    left -= n;
+    at += n;
+    if (shared) {
+      cur.unit += n;
+      if (cur.unit == cur.units) cur.next_segment(p, a);
+    }
+    return true;
+  }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_tc_kernel(const Pool p, const Problem a, const int row_tiles, const int shared_blocks) {
+  using L = Smem<D>;
+  constexpr int G = L::G;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const mem = smem_raw + (base - smem_u32(smem_raw));
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  auto bar = [&](int i) { return base + L::bars + 8u * (uint32_t)i; };
+  const uint32_t tmem_holder = base + L::bars + 8u * kNumBars;
+  if (threadIdx.x == 0) {
+    mbar_init(bar(kQFull), 4);
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(bar(kRawFull + i), 1);
+      mbar_init(bar(kRawEmpty + i), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(kKFull + i), 4);
+      mbar_init(bar(kKEmpty + i), 1);
+      mbar_init(bar(kVFull + i), 4);
+      mbar_init(bar(kVEmpty + i), 1);
+      mbar_init(bar(kSFull + i), 1);
+    }
+    mbar_init(bar(kPFull), 4);
+    mbar_init(bar(kTogether), 4);
+    mbar_init(bar(kOFull), 1);
+    fence_mbar_init();
+  }
+  if (warp == kMma) {
+    tmem_alloc(tmem_holder, kTmemCols);
+    tmem_relinquish();
+  }
+  pdl_wait();
+  pdl_trigger();
+  // ---- this CTA's work
+  Walk walk;
+  walk.shared = shared_blocks != 0;
+  walk.row_tiles = row_tiles;
+  walk.begin = walk.at = 0;
+  Shares shares(1, 1);
+  if (walk.shared) {
+    const Plan<kBlock> plan(p, a);
+    // a share of a few blocks at least: an empty one could not be joined
+    shares = Shares(plan.total, min(gridDim.x, (plan.total + 1) / 2));
+    walk.left = 0;
+    if (plan.total > 0 && blockIdx.x < shares.W) {
+      walk.begin = walk.at = shares.begin(blockIdx.x);
+      walk.left = (int)(shares.begin(blockIdx.x + 1) - walk.begin);
+      walk.cur = plan.seek(p, a, walk.begin);
+    }
+  } else {
+    // one segment; the longest (a head's last rows) of every request first
+    const int per_tile = gridDim.x / row_tiles, tile = blockIdx.x / per_tile, bh = blockIdx.x - tile * per_tile;
+    walk.cur.b = bh / p.H;
+    walk.cur.seg = (bh - walk.cur.b * p.H) * row_tiles + (row_tiles - 1 - tile);
+    walk.cur.unit = 0;
+    walk.cur.keys = keys_of(p, a, walk.cur.b);
+    walk.cur.units = 1;
+    walk.left = walk.cur.keys > 0 ? 1 : 0;
+  }
+  // Zeros for queries without a place in the pool.
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    const int keys = keys_of(p, a, b), good = keys == 0 ? 0 : min(a.tq, keys - a.start_pos[b]);
+    if (good == a.tq) continue;
+    if (threadIdx.x == 0) raise_device_error(DEV_ERR_ATTN_RANGE);
+    const long long n = (long long)(a.tq - good) * a.QH * D;
+    T* bad = static_cast<T*>(a.out) + ((long long)b * a.tq + good) * a.QH * D;
+    for (long long i = threadIdx.x; i < n; i += kThreads) bad[i] = from_f32<T>(0.f);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_holder) : "memory");
+  __shared__ unsigned taken_sh;
+
+  Part part;
+  if (warp == kCopy) {
+    // ------------------------------------------------------------ copies
+    if (lane == 0) {
+      unsigned n = 0;  // tiles so far
+      bool live = true;
+      while (live && walk.next(p, a, part)) {
+        const uint8_t* tiles = head_tiles(p, a.slot_of[part.b], part.h);
+        const int t1 = min(part.hi * (kBlock / kTile), (part.kend + kTile - 1) / kTile);
+        for (int t = part.lo * (kBlock / kTile); t < t1 && live; ++t, ++n) {
+          const unsigned s = n % kRing;
+          if (n >= kRing) live = mbar_wait(bar(kRawEmpty + s), (n / kRing - 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+          if (!live) break;
+          mbar_arrive_expect_tx(bar(kRawFull + s), L::kTileBytes);
+          bulk_load(base + L::raw + s * L::kTileBytes, tiles + (long long)t * L::kTileBytes, L::kTileBytes,
+                    bar(kRawFull + s));
+        }
+      }
+      // the copies in flight land before the CTA may exit
+      if (!live)
+        for (unsigned i = n < kRing ? 0 : n - kRing; i < n; ++i)
+          mbar_wait(bar(kRawFull + i % kRing), (i / kRing) & 1, DEV_ERR_ATTN_TIMEOUT);
+    }
+    __syncwarp();
+  } else if (warp == kMma) {
+    // ------------------------------------------------------------ UMMA issuer
+    if (lane == 0) {
+      const int fmt = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+      const uint32_t id_s = umma_idesc(fmt, 0, 0, kBlock);  // Q (K-major) x K (K-major)
+      const uint32_t id_o = umma_idesc(fmt, 0, 1, D);       // P (K-major) x V (MN-major along the head dim)
+      const uint64_t dq = umma_desc_sw128(base + L::q, 16u, 1024u), dp = umma_desc_sw128(base + L::p, 16u, 1024u);
+      bool live = true;
+      unsigned blk = 0, parts = 0, s_issued = 0, o_issued = 0;
+      auto scores = [&](unsigned n) {
+        live = live && mbar_wait(bar(kKFull + (n & 1)), (n >> 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+        if (!live) return;
+        tc_fence_after();
+        const uint64_t dk = umma_desc_sw128(base + L::k + (n & 1) * L::kOperand, 16u, 1024u);
+#pragma unroll
+        for (int sl = 0; sl < L::kSlabs; ++sl)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t off = (uint32_t)(sl * kRows * 128 + k * 32) >> 4;
+            umma_f16(tmem + (n & 1) * kBlock, dq + off, dk + off, id_s, (sl | k) != 0);
+          }
+        umma_commit(bar(kSFull + (n & 1)));
+        umma_commit(bar(kKEmpty + (n & 1)));
+        s_issued = n + 1;
+      };
+      while (live && walk.next(p, a, part)) {
+        const int nb = part.hi - part.lo;
+        if (nb == 0) continue;
+        live = mbar_wait(bar(kQFull), parts & 1, DEV_ERR_ATTN_TIMEOUT);
+        ++parts;
+        if (!live) break;
+        scores(blk);
+        for (int j = 0; j < nb && live; ++j, ++blk) {
+          if (j + 1 < nb) scores(blk + 1);
+          live = live && mbar_wait(bar(kPFull), blk & 1, DEV_ERR_ATTN_TIMEOUT) &&
+                 mbar_wait(bar(kVFull + (blk & 1)), (blk >> 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+          if (!live) break;
+          tc_fence_after();
+          const uint64_t dv = umma_desc_sw128(base + L::v + (blk & 1) * L::kOperand, (uint32_t)(kBlock * 128), 1024u);
+#pragma unroll
+          for (int k = 0; k < kBlock / 16; ++k) {
+            const uint32_t poff = (uint32_t)((k / 4) * kRows * 128 + (k % 4) * 32) >> 4;
+            const uint32_t voff = (uint32_t)(k * 16 * 128) >> 4;
+            umma_f16(tmem + 2 * kBlock, dp + poff, dv + voff, id_o, (j | k) != 0);
+          }
+          umma_commit(bar(kOFull));
+          umma_commit(bar(kVEmpty + (blk & 1)));
+          o_issued = blk + 1;
+        }
+      }
+      // every UMMA issued completes before TMEM is released
+      if (s_issued > 0) mbar_wait(bar(kSFull + ((s_issued - 1) & 1)), ((s_issued - 1) >> 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+      if (o_issued > 0) mbar_wait(bar(kOFull), (o_issued - 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+    }
+    __syncwarp();
+  } else if (warp >= kDequant) {
+    // ------------------------------------------------------------ codes to operands
+    const int dw = warp - kDequant, row = dw * 32 + lane;  // row of the block
+    const uint32_t out_row = (uint32_t)row * 128u;
+    bool live = true;
+    unsigned blk = 0, n = 0;  // blocks and tiles so far
+    while (live && walk.next(p, a, part)) {
+      for (int j = part.lo; j < part.hi && live; ++j, ++blk) {
+        const int key0 = j * kBlock, here = min(kBlock / kTile, (part.kend - key0 + kTile - 1) / kTile);
+        const bool tile = dw < here, ok = key0 + row < part.kend;
+        const unsigned s = (n + dw) % kRing;
+        if (tile) live = mbar_wait(bar(kRawFull + s), ((n + dw) / kRing) & 1, DEV_ERR_ATTN_TIMEOUT);
+        if (blk >= 2) live = live && mbar_wait(bar(kKEmpty + (blk & 1)), ((blk >> 1) - 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+        if (!__all_sync(0xffffffffu, live)) {
+          live = false;
+          break;
+        }
+        const uint8_t* const t8 = mem + L::raw + s * L::kTileBytes;
+        // A lane starts at its own chunk, so that eight lanes' 16-byte reads lie in
+        // distinct banks; C chunks of 16 bytes a row.
+        constexpr int C = G;  // 16 G bytes
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const uint32_t dst = base + (kv ? L::v : L::k) + (blk & 1) * L::kOperand + out_row;
+          if (kv) {
+            if (blk >= 2) live = mbar_wait(bar(kVEmpty + (blk & 1)), ((blk >> 1) - 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+            if (!__all_sync(0xffffffffu, live)) {
+              live = false;
+              break;
+            }
+          }
+          if (!ok) {  // no such position: its value must not count, and its weight is zero
+            if (kv)
+              for (int c = 0; c < D / 8; ++c)
+                sts4(dst + (c / 8) * (kBlock * 128) + (((c % 8) ^ (row & 7)) * 16), make_uint4(0u, 0u, 0u, 0u));
+          } else {
+            const uint8_t* const half = t8 + kv * (L::kTileBytes / 2);
+            const uint8_t* const codes = half + lane * 16 * G;
+            uint32_t sz[G];
+#pragma unroll
+            for (int g = 0; g < G; g += 2) {
+              const uint2 w = *reinterpret_cast<const uint2*>(half + kTile * 16 * G + (lane * G + g) * 4);
+              sz[g] = w.x;
+              sz[g + 1] = w.y;
+            }
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+              const int c = (i + lane / (8 / C)) % C;  // 16-byte chunk of the row
+              const uint4 w = *reinterpret_cast<const uint4*>(codes + c * 16);
+              // its eight-channel words: quarter (of the 32 channels) and group of each
+              uint32_t x[4];
+              int quarter[4], group[4];
+              if (G == 4) {
+                const int at = kv ? c ^ (((lane >> 1) & 1) * 2) : c;  // the values' order is turned by position
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                  quarter[g] = at;
+                  group[g] = g;
+                }
+                if (kv) {  // half words of channels 8 q .. and 8 q + 4 .. , four groups each
+                  x[0] = __byte_perm(w.x, w.z, 0x5410);
+                  x[1] = __byte_perm(w.x, w.z, 0x7632);
+                  x[2] = __byte_perm(w.y, w.w, 0x5410);
+                  x[3] = __byte_perm(w.y, w.w, 0x7632);
+                } else {
+                  x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
+                }
+              } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  quarter[k] = 2 * c + k / 2;
+                  group[k] = k & 1;
+                }
+                if (kv) {
+                  x[0] = __byte_perm(w.x, w.y, 0x5410);
+                  x[1] = __byte_perm(w.x, w.y, 0x7632);
+                  x[2] = __byte_perm(w.z, w.w, 0x5410);
+                  x[3] = __byte_perm(w.z, w.w, 0x7632);
+                } else {
+                  x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
+                }
+              }
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int o8 = 4 * group[k] + quarter[k];  // which eight channels of the row
+                sts4(dst + (group[k] / 2) * (kBlock * 128) + (((o8 & 7) ^ (row & 7)) * 16), operand8<T>(x[k], sz[group[k]]));
+              }
+            }
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar((kv ? kVFull : kKFull) + (blk & 1)));
+        }
+        if (!live) break;
+        if (tile && lane == 0) mbar_arrive(bar(kRawEmpty + s));
+        n += here;
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ queries, softmax, epilogue
+    const int r = threadIdx.x;  // row of the segment = TMEM lane
+    const uint32_t trow = tmem + ((uint32_t)(warp * 32) << 16);
+    const uint32_t prow = base + L::p + (uint32_t)r * 128u;
+    constexpr int kShare = kRows * (4 + D);  // floats of a part in the workspace
+    bool live = true;
+    unsigned blk = 0, met = 0;
+    // the four warps meet (bounded, unlike a hardware barrier: one may have given up)
+    auto together = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kTogether));
+      live = __all_sync(0xffffffffu, mbar_wait(bar(kTogether), met & 1, DEV_ERR_ATTN_TIMEOUT));
+      ++met;
+      return live;
+    };
+    while (live && walk.next(p, a, part)) {
+      const int nb = part.hi - part.lo;
+      const int row = part.row0 + r, tok = row / a.group, qh = part.h * a.group + (row - tok * a.group);
+      const bool mine = r < part.rows && part.start + tok < p.max_seq;
+      const bool used = __any_sync(0xffffffffu, mine);  // the warp has rows at all
+      const int row_keys = mine ? part.start + tok + 1 : 0;
+      unsigned w0 = 0, w1 = 0;
+      if (!part.whole) {
+        w0 = shares.holder(part.seg0, blockIdx.x);
+        w1 = shares.holder(part.seg0 + part.units - 1, blockIdx.x);
+        if (r == 0) open_tickets(a.tickets + w0, a.launch);
+      }
+      if (nb > 0) {
+        if (mine) {
+          const T* qp = static_cast<const T*>(a.q) + part.b * a.qs0 + tok * a.qs1 + qh * a.qs2;
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            uint4 w;
+            if (a.q_vec) {
+              w = reinterpret_cast<const uint4*>(qp)[c];
+            } else {
+              T e[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) e[i] = qp[c * 8 + i];
+              w = *reinterpret_cast<const uint4*>(e);
+            }
+            // the operands' order: 0 4 1 5 2 6 3 7
+            sts4(base + L::q + (c / 8) * (kRows * 128) + r * 128 + (((c % 8) ^ (r & 7)) * 16),
+                 make_uint4(__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632), __byte_perm(w.y, w.w, 0x5410),
+                            __byte_perm(w.y, w.w, 0x7632)));
+          }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kQFull));
+      }
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < nb && live; ++j, ++blk) {
+        live = mbar_wait(bar(kSFull + (blk & 1)), (blk >> 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+        if (!__all_sync(0xffffffffu, live)) {
+          live = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t ts = trow + (blk & 1) * kBlock, to = trow + 2 * kBlock;
+        const int lim = row_keys - (part.lo + j) * kBlock;  // positions of the block that the row attends
+        const bool full = __all_sync(0xffffffffu, lim >= kBlock || !mine);
+        const bool any = __any_sync(0xffffffffu, lim > 0);
+        float alpha = 1.f;
+        if (any) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < kBlock / 32; ++c) {
+            float v[32];
+            tmem_ld32(ts + c * 32, v);
+            if (full) {
+              float m4[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+              for (int e = 4; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], v[e]);
+              mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (c * 32 + e < lim) mx = fmaxf(mx, v[e]);
+            }
+          }
+          const float mn = fmaxf(m, mx * a.scale_log2);
+          alpha = m == -INFINITY ? 0.f : ex2(m - mn);
+          m = mn;
+          l *= alpha;
+        }
+        // P and the running output are free once the block before is through
+        if (j > 0) {
+          live = mbar_wait(bar(kOFull), (blk - 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+          if (!__all_sync(0xffffffffu, live)) {
+            live = false;
+            break;
+          }
+          tc_fence_after();
+          if (any && !__all_sync(0xffffffffu, alpha == 1.f || !mine)) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              float v[32];
+              tmem_ld32(to + c * 32, v);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] *= alpha;
+              tmem_st32(to + c * 32, v);
+            }
+          }
+        }
+        if (any) {
+          const float base_m = m == -INFINITY ? 0.f : m;
+          float lp[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < kBlock / 32; ++c) {
+            float v[32];
+            tmem_ld32(ts + c * 32, v);
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              float p0 = ex2(fmaf(v[e], a.scale_log2, -base_m)), p1 = ex2(fmaf(v[e + 1], a.scale_log2, -base_m));
+              if (!full) {
+                p0 = c * 32 + e < lim ? p0 : 0.f;
+                p1 = c * 32 + e + 1 < lim ? p1 : 0.f;
+              }
+              w[e / 2] = pack2<T>(p0, p1);
+              const float2 f = unpack2<T>(w[e / 2]);  // the sum of what the tensor core multiplies
+              lp[(e / 2) & 3] += f.x + f.y;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int chunk = 4 * (c % 2) + i;
+              sts4(prow + (c / 2) * (kRows * 128) + ((chunk ^ (r & 7)) * 16),
+                   make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
+            }
+          }
+          l += (lp[0] + lp[1]) + (lp[2] + lp[3]);
+        } else if (used) {  // all masked: weights of zero
+#pragma unroll
+          for (int c = 0; c < kBlock / 8; ++c)
+            sts4(prow + (c / 8) * (kRows * 128) + (((c % 8) ^ (r & 7)) * 16), make_uint4(0u, 0u, 0u, 0u));
+        }
+        fence_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kPFull));
+      }
+      if (nb > 0 && live) {
+        live = mbar_wait(bar(kOFull), (blk - 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+        live = __all_sync(0xffffffffu, live);
+        tc_fence_after();
+      }
+      if (!live) break;
+      T* const op = static_cast<T*>(a.out) + (((long long)part.b * a.tq + tok) * a.QH + qh) * D;
+      // a row's 32 columns, in the operands' order, as the output's channels
+      auto store = [&](int c, const float (&v)[32], float f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float* x = v + 8 * i;
+          const uint4 w = make_uint4(pack2<T>(x[0] * f, x[2] * f), pack2<T>(x[4] * f, x[6] * f),
+                                     pack2<T>(x[1] * f, x[3] * f), pack2<T>(x[5] * f, x[7] * f));
+          if (a.out_vec) {
+            reinterpret_cast<uint4*>(op + c * 32)[i] = w;
+          } else {
+            const T* e = reinterpret_cast<const T*>(&w);
+            for (int k = 0; k < 8; ++k) op[c * 32 + 8 * i + k] = e[k];
+          }
+        }
+      };
+      if (part.whole) {
+        if (used) {
+          const float inv = 1.0f / l;
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            float v[32];
+            tmem_ld32(trow + 2 * kBlock + c * 32, v);
+            if (mine) store(c, v, inv);
+          }
+        }
+        continue;
+      }
+      // ---- other CTAs hold parts of the segment
+      float* own = a.ws + ((long long)blockIdx.x * 2 + part.which) * kShare + r * (4 + D);
+      if (used) {
+        if (mine) __stcg(reinterpret_cast<float4*>(own), make_float4(m, l, 0.f, 0.f));
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          float v[32];
+          if (nb > 0) tmem_ld32(trow + 2 * kBlock + c * 32, v);
+          if (mine && nb > 0)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              __stcg(reinterpret_cast<float4*>(own + 4 + c * 32) + i,
+                     make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+        }
+      }
+      if (!together()) break;
+      if (r == 0) {
+        const unsigned taken = take_ticket(a.tickets + w0);
+        if (taken == w1 - w0 + 1) a.tickets[w0] = 0;  // clean for the next launch
+        taken_sh = taken;
+      }
+      if (!together()) break;
+      if (taken_sh == w1 - w0 + 1 && mine) {
+        const float* at = a.ws + r * (4 + D);
+        // the segment is the last part of the share that it starts in, the first of the others
+        auto share = [&](unsigned w) {
+          return at + ((long long)w * 2 + (w == w0 && shares.begin(w) < part.seg0 ? 1 : 0)) * kShare;
+        };
+        float mx = -INFINITY, ls = 0.f;
+        for (unsigned w = w0; w <= w1; ++w) mx = fmaxf(mx, __ldcg(share(w)));
+        for (unsigned w = w0; w <= w1; ++w) {
+          const float2 ml = __ldcg(reinterpret_cast<const float2*>(share(w)));
+          if (!(ml.x == -INFINITY && ml.y == 0.f)) ls = fmaf(ex2(ml.x - mx), ml.y, ls);
+        }
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float x[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = 0.f;
+          for (unsigned w = w0; w <= w1; ++w) {
+            const float* s = share(w);
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(s));
+            if (ml.x == -INFINITY && ml.y == 0.f) continue;  // all masked: no output left
+            const float f = ex2(ml.x - mx);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 y = __ldcg(reinterpret_cast<const float4*>(s + 4 + c * 32) + i);
+              x[4 * i] = fmaf(f, y.x, x[4 * i]);
+              x[4 * i + 1] = fmaf(f, y.y, x[4 * i + 1]);
+              x[4 * i + 2] = fmaf(f, y.z, x[4 * i + 2]);
+              x[4 * i + 3] = fmaf(f, y.w, x[4 * i + 3]);
+            }
+          }
+          store(c, x, 1.0f / ls);
+        }
+      }
+      together();  // taken_sh is read
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMma) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+template <typename T, int D>
+static int launch(const Pool& p, const Problem& a, int row_tiles, bool shared, cudaStream_t st) {
+  static std::atomic<bool> ready[64] = {};
+  const int dev = current_device();
+  if (dev < 0 || dev >= 64) return fail(FML_EUNSUPPORTED, "neb_kv4_attention: device index out of range");
+  if (!ready[dev].load()) {
+    const cudaError_t e = cudaFuncSetAttribute(attn_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)Smem<D>::total);
+    if (e != cudaSuccess) return check_cuda(e, "neb_kv4_attention smem attribute");
+    ready[dev].store(true);
+  }
+  const long long grid = shared ? num_sms(dev) : (long long)a.B * p.H * row_tiles;
+  const cudaError_t e = launch_pdl(attn_tc_kernel<T, D>, dim3((unsigned)grid), dim3(kThreads), Smem<D>::total, st, 1, p, a,
+                                   row_tiles, shared ? 1 : 0);
+  count_launch();
+  return check_cuda(e, "neb_kv4_attention launch");
+}
+
+}  // namespace tc
+
+// Whether the tensor-core kernel takes the call.
+bool tc_covers(const Pool& p, int dtype, int64_t t, int64_t group) {
+  return (dtype == FML_BF16 || dtype == FML_F16) && (p.D == 64 || p.D == 128) && t * group > 1;
+}
+static bool tc_shared(const Pool& p, int64_t segments, int64_t requests_units) {
+  return segments < 2 * num_sms(current_device()) && requests_units < (1ll << 31);
+}
+size_t tc_workspace_bytes(const Pool& p, int64_t batch, int64_t t, int64_t group) {
+  const int64_t tiles = (t * group + tc::kRows - 1) / tc::kRows, segs = batch * p.H * tiles;
+  if (!tc_shared(p, segs, segs * ((p.max_seq + tc::kBlock - 1) / tc::kBlock))) return 0;
+  const size_t sms = (size_t)num_sms(current_device());
+  return sms * 2 * tc::kRows * (4 + p.D) * sizeof(float) + sms * sizeof(unsigned long long);
+}
+int tc_attention(const Pool& p, Problem a, int dtype, cudaStream_t st) {
+  const int tiles = (int)(((int64_t)a.tq * a.group + tc::kRows - 1) / tc::kRows);
+  const int64_t segs = (int64_t)a.B * p.H * tiles;
+  if (segs >= (1ll << 31)) return fail(FML_EUNSUPPORTED, "neb_kv4_attention: too many queries");
+  const bool shared = tc_shared(p, segs, segs * ((p.max_seq + tc::kBlock - 1) / tc::kBlock));
+  a.segs = p.H * tiles;
+  const size_t sms = (size_t)num_sms(current_device());
+  a.tickets = reinterpret_cast<unsigned long long*>(reinterpret_cast<uint8_t*>(a.ws) +
+                                                    sms * 2 * tc::kRows * (4 + p.D) * sizeof(float));
+  a.launch = launch_number();
+  if (dtype == FML_BF16)
+    return p.D == 64 ? tc::launch<__nv_bfloat16, 64>(p, a, tiles, shared, st)
+                     : tc::launch<__nv_bfloat16, 128>(p, a, tiles, shared, st);
+  return p.D == 64 ? tc::launch<__half, 64>(p, a, tiles, shared, st) : tc::launch<__half, 128>(p, a, tiles, shared, st);
+}
+
+}  // namespace kv4
+}  // namespace fml
