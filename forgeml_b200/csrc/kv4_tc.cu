@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int t1 = min(part.hi * (kBlock / kTile), (part.kend + kTile - 1) / kTile);
         for (int t = part.lo * (kBlock / kTile); t < t1 && live; ++t, ++n) {
           const unsigned s = n % kRing;
-          if (n >= kRing) live = mbar_wait(bar(kRawEmpty + s), (n / kRing - 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+          if (n >= kRing) live = wait_copies(bar(kRawEmpty + s), (n / kRing - 1) & 1);
           if (!live) break;
           mbar_arrive_expect_tx(bar(kRawFull + s), L::kTileBytes);
           bulk_load(base + L::raw + s * L::kTileBytes, tiles + (long long)t * L::kTileBytes, L::kTileBytes,
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the copies in flight land before the CTA may exit
       if (!live)
         for (unsigned i = n < kRing ? 0 : n - kRing; i < n; ++i)
-          mbar_wait(bar(kRawFull + i % kRing), (i / kRing) & 1, DEV_ERR_ATTN_TIMEOUT);
+          wait_copies(bar(kRawFull + i % kRing), (i / kRing) & 1);
     }
     __syncwarp();
   } else if (warp == kMma) {
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool live = true;
       unsigned blk = 0, parts = 0, s_issued = 0, o_issued = 0;
       auto scores = [&](unsigned n) {
-        live = live && mbar_wait(bar(kKFull + (n & 1)), (n >> 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+        live = live && wait_copies(bar(kKFull + (n & 1)), (n >> 1) & 1);
         if (!live) return;
         tc_fence_after();
         const uint64_t dk = umma_desc_sw128(base + L::k + (n & 1) * L::kOperand, 16u, 1024u);
@@ -274,14 +274,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       while (live && walk.next(p, a, part)) {
         const int nb = part.hi - part.lo;
         if (nb == 0) continue;
-        live = mbar_wait(bar(kQFull), parts & 1, DEV_ERR_ATTN_TIMEOUT);
+        live = wait_copies(bar(kQFull), parts & 1);
         ++parts;
         if (!live) break;
         scores(blk);
         for (int j = 0; j < nb && live; ++j, ++blk) {
           if (j + 1 < nb) scores(blk + 1);
-          live = live && mbar_wait(bar(kPFull), blk & 1, DEV_ERR_ATTN_TIMEOUT) &&
-                 mbar_wait(bar(kVFull + (blk & 1)), (blk >> 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+          live = live && wait_copies(bar(kPFull), blk & 1) &&
+                 wait_copies(bar(kVFull + (blk & 1)), (blk >> 1) & 1);
           if (!live) break;
           tc_fence_after();
           const uint64_t dv = umma_desc_sw128(base + L::v + (blk & 1) * L::kOperand, (uint32_t)(kBlock * 128), 1024u);
@@ -297,8 +297,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // every UMMA issued completes before TMEM is released
-      if (s_issued > 0) mbar_wait(bar(kSFull + ((s_issued - 1) & 1)), ((s_issued - 1) >> 1) & 1, DEV_ERR_ATTN_TIMEOUT);
-      if (o_issued > 0) mbar_wait(bar(kOFull), (o_issued - 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+      if (s_issued > 0) wait_copies(bar(kSFull + ((s_issued - 1) & 1)), ((s_issued - 1) >> 1) & 1);
+      if (o_issued > 0) wait_copies(bar(kOFull), (o_issued - 1) & 1);
     }
     __syncwarp();
   } else if (warp >= kDequant) {
@@ -312,8 +312,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int key0 = j * kBlock, here = min(kBlock / kTile, (part.kend - key0 + kTile - 1) / kTile);
         const bool tile = dw < here, ok = key0 + row < part.kend;
         const unsigned s = (n + dw) % kRing;
-        if (tile) live = mbar_wait(bar(kRawFull + s), ((n + dw) / kRing) & 1, DEV_ERR_ATTN_TIMEOUT);
-        if (blk >= 2) live = live && mbar_wait(bar(kKEmpty + (blk & 1)), ((blk >> 1) - 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+        if (tile) live = wait_copies(bar(kRawFull + s), ((n + dw) / kRing) & 1);
+        if (blk >= 2) live = live && wait_copies(bar(kKEmpty + (blk & 1)), ((blk >> 1) - 1) & 1);
         if (!__all_sync(0xffffffffu, live)) {
           live = false;
           break;
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int kv = 0; kv < 2; ++kv) {
           const uint32_t dst = base + (kv ? L::v : L::k) + (blk & 1) * L::kOperand + out_row;
           if (kv) {
-            if (blk >= 2) live = mbar_wait(bar(kVEmpty + (blk & 1)), ((blk >> 1) - 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+            if (blk >= 2) live = wait_copies(bar(kVEmpty + (blk & 1)), ((blk >> 1) - 1) & 1);
             if (!__all_sync(0xffffffffu, live)) {
               live = false;
               break;
@@ -346,8 +346,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               sz[g] = w.x;
               sz[g + 1] = w.y;
             }
-#pragma unroll
-            for (int i = 0; i < C; ++i) {
+#pragma unroll 1
+            for (int i = 0; i < C; ++i) {  // rolled, like the softmax's: the roles' loops share the instruction cache
               const int c = (i + lane / (8 / C)) % C;  // 16-byte chunk of the row
               const uint4 w = *reinterpret_cast<const uint4*>(codes + c * 16);
               // its eight-channel words: quarter (of the 32 channels) and group of each
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto together = [&]() {
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(kTogether));
-      live = __all_sync(0xffffffffu, mbar_wait(bar(kTogether), met & 1, DEV_ERR_ATTN_TIMEOUT));
+      live = __all_sync(0xffffffffu, wait_copies(bar(kTogether), met & 1));
       ++met;
       return live;
     };
@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < nb && live; ++j, ++blk) {
-        live = mbar_wait(bar(kSFull + (blk & 1)), (blk >> 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+        live = wait_copies(bar(kSFull + (blk & 1)), (blk >> 1) & 1);
         if (!__all_sync(0xffffffffu, live)) {
           live = false;
           break;
@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float alpha = 1.f;
         if (any) {
           float mx = -INFINITY;
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < kBlock / 32; ++c) {
             float v[32];
             tmem_ld32(ts + c * 32, v);
@@ -488,14 +488,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // P and the running output are free once the block before is through
         if (j > 0) {
-          live = mbar_wait(bar(kOFull), (blk - 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+          live = wait_copies(bar(kOFull), (blk - 1) & 1);
           if (!__all_sync(0xffffffffu, live)) {
             live = false;
             break;
           }
           tc_fence_after();
           if (any && !__all_sync(0xffffffffu, alpha == 1.f || !mine)) {
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               float v[32];
               tmem_ld32(to + c * 32, v);
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (any) {
           const float base_m = m == -INFINITY ? 0.f : m;
           float lp[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < kBlock / 32; ++c) {
             float v[32];
             tmem_ld32(ts + c * 32, v);
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(bar(kPFull));
       }
       if (nb > 0 && live) {
-        live = mbar_wait(bar(kOFull), (blk - 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+        live = wait_copies(bar(kOFull), (blk - 1) & 1);
         live = __all_sync(0xffffffffu, live);
         tc_fence_after();
       }
@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (part.whole) {
         if (used) {
           const float inv = 1.0f / l;
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             float v[32];
             tmem_ld32(trow + 2 * kBlock + c * 32, v);
@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float* own = a.ws + ((long long)blockIdx.x * 2 + part.which) * kShare + r * (4 + D);
       if (used) {
         if (mine) __stcg(reinterpret_cast<float4*>(own), make_float4(m, l, 0.f, 0.f));
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float v[32];
           if (nb > 0) tmem_ld32(trow + 2 * kBlock + c * 32, v);
