@@ -6,18 +6,20 @@
 // token * group + query head within the group: UMMA M, the TMEM lanes).  Its
 // positions go by in blocks of 128, flash-attention schedule, warp-specialised:
 //
-//   warp 9     copies the cache's tiles (32 positions, one bulk copy each) into a
-//              ring;
-//   warps 4-7  turn a tile each into 16-bit operands: a lane takes a position's
-//              codes and writes z + c s, rounded once, into the swizzled key and
-//              value blocks (two of each).  A code under the exponent of 128 (fp16:
-//              1024) is a 16-bit number, two at a time; the channels of every eight
-//              stay in the order 0 4 1 5 2 6 3 7 that this leaves, in the queries
-//              too, and are put right where the output is written;
-//   warp 8     TMEM owner and single-thread UMMA issuer: S = Q K^T of block j + 1
-//              into the other of two TMEM score blocks while block j's softmax
-//              runs, O += P V into TMEM;
-//   warps 0-3  queries, softmax and epilogue, one row per thread.
+//   warps 8-15  turn the cache's codes into 16-bit operands (8-11 the keys, 12-15
+//               the values): a lane takes a position's codes, loaded a block ahead,
+//               and writes z + c s, rounded once, into the swizzled block (two of
+//               each).  A code under the exponent of 128 (fp16: 1024) is a 16-bit
+//               number, two at a time; the channels of every eight stay in the order
+//               0 4 1 5 2 6 3 7 that this leaves, in the queries too, and are put
+//               right where the output is written;
+//   warp 16     TMEM owner and single-thread UMMA issuer: S = Q K^T of block j + 1
+//               into the other of two TMEM score blocks while block j's softmax
+//               runs, O += P V into TMEM;
+//   warps 0-7   queries, softmax and epilogue: two threads a row, half of a block's
+//               positions (and of the output's channels) each.  (One thread a row and
+//               four warps for the operands left the schedulers two warps each and
+//               half idle.)
 //
 // Rounded below fp32: the operands (keys, values) and P, to the cache's dtype, as
 // attention over a 16-bit cache rounds them.
@@ -27,7 +29,7 @@
 // the last CTA to arrive (kv4_attention.cuh).
 //
 // Every wait is bounded (DEV_ERR_ATTN_TIMEOUT); a CTA that gives up lets its
-// copies land and frees its TMEM before it exits.
+// products finish and frees its TMEM before it exits.
 #include <string>
 #include <type_traits>
 
@@ -39,9 +41,8 @@ namespace tc {
 
 constexpr int kRows = 128;   // query rows of a segment
 constexpr int kBlock = 128;  // positions of a block
-constexpr int kThreads = 320;
-constexpr int kDequant = 4, kMma = 8, kCopy = 9;  // first warps of the roles
-constexpr int kRing = 6;                          // tiles
+constexpr int kThreads = 544;
+constexpr int kDequant = 8, kMma = 16;  // first warps of the roles
 constexpr uint32_t kTmemCols = 512;               // two score blocks, the output
 
 template <int D>
@@ -50,14 +51,14 @@ struct Smem {
   static constexpr uint32_t kTileBytes = 2 * kTile * G * (16 + 4);
   static constexpr uint32_t kOperand = kRows * D * 2;
   static constexpr uint32_t q = 0, k = kOperand, v = 3 * kOperand, p = 5 * kOperand;
-  static constexpr uint32_t raw = p + kRows * kBlock * 2;
-  static constexpr uint32_t bars = raw + kRing * kTileBytes;
-  static constexpr uint32_t total = bars + 256 + 1024;  // 1024: alignment of the base
+  static constexpr uint32_t bars = p + kRows * kBlock * 2;
+  static constexpr uint32_t rows = bars + 512;  // what a row's two threads tell each other: [2][2][128] fp32
+  static constexpr uint32_t total = rows + 2048 + 1024;  // 1024: alignment of the base
   static_assert(total <= 227 * 1024, "shared memory");
 };
 enum Bar : int {
-  kQFull = 0, kRawFull = 1, kRawEmpty = kRawFull + kRing, kKFull = kRawEmpty + kRing, kKEmpty = kKFull + 2,
-  kVFull = kKEmpty + 2, kVEmpty = kVFull + 2, kSFull = kVEmpty + 2, kPFull = kSFull + 2, kOFull, kTogether, kNumBars
+  kQFull = 0, kKFull = 1, kKEmpty = kKFull + 2,
+  kVFull = kKEmpty + 2, kVEmpty = kVFull + 2, kSFull = kVEmpty + 2, kPFull = kSFull + 2, kOFull, kTogether, kPair, kNumBars = kPair + 4
 };
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -151,17 +152,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   using L = Smem<D>;
   constexpr int G = L::G;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
+  static_assert(G == 2 || G == 4, "head dim 64 or 128");
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const mem = smem_raw + (base - smem_u32(smem_raw));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   auto bar = [&](int i) { return base + L::bars + 8u * (uint32_t)i; };
   const uint32_t tmem_holder = base + L::bars + 8u * kNumBars;
   if (threadIdx.x == 0) {
-    mbar_init(bar(kQFull), 4);
-    for (int i = 0; i < kRing; ++i) {
-      mbar_init(bar(kRawFull + i), 1);
-      mbar_init(bar(kRawEmpty + i), 1);
-    }
+    mbar_init(bar(kQFull), 8);
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(kKFull + i), 4);
       mbar_init(bar(kKEmpty + i), 1);
@@ -169,8 +167,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(kVEmpty + i), 1);
       mbar_init(bar(kSFull + i), 1);
     }
-    mbar_init(bar(kPFull), 4);
-    mbar_init(bar(kTogether), 4);
+    mbar_init(bar(kPFull), 8);
+    mbar_init(bar(kTogether), 8);
+    for (int i = 0; i < 4; ++i) mbar_init(bar(kPair + i), 2);
     mbar_init(bar(kOFull), 1);
     fence_mbar_init();
   }
@@ -223,30 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ unsigned taken_sh;
 
   Part part;
-  if (warp == kCopy) {
-    // ------------------------------------------------------------ copies
-    if (lane == 0) {
-      unsigned n = 0;  // tiles so far
-      bool live = true;
-      while (live && walk.next(p, a, part)) {
-        const uint8_t* tiles = head_tiles(p, a.slot_of[part.b], part.h);
-        const int t1 = min(part.hi * (kBlock / kTile), (part.kend + kTile - 1) / kTile);
-        for (int t = part.lo * (kBlock / kTile); t < t1 && live; ++t, ++n) {
-          const unsigned s = n % kRing;
-          if (n >= kRing) live = wait_copies(bar(kRawEmpty + s), (n / kRing - 1) & 1);
-          if (!live) break;
-          mbar_arrive_expect_tx(bar(kRawFull + s), L::kTileBytes);
-          bulk_load(base + L::raw + s * L::kTileBytes, tiles + (long long)t * L::kTileBytes, L::kTileBytes,
-                    bar(kRawFull + s));
-        }
-      }
-      // the copies in flight land before the CTA may exit
-      if (!live)
-        for (unsigned i = n < kRing ? 0 : n - kRing; i < n; ++i)
-          wait_copies(bar(kRawFull + i % kRing), (i / kRing) & 1);
-    }
-    __syncwarp();
-  } else if (warp == kMma) {
+  if (warp == kMma) {
     // ------------------------------------------------------------ UMMA issuer
     if (lane == 0) {
       const int fmt = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
@@ -303,111 +279,103 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp >= kDequant) {
     // ------------------------------------------------------------ codes to operands
-    const int dw = warp - kDequant, row = dw * 32 + lane;  // row of the block
+    const int kv = (warp - kDequant) >> 2, dw = (warp - kDequant) & 3, row = dw * 32 + lane;  // row of the block
     const uint32_t out_row = (uint32_t)row * 128u;
     bool live = true;
-    unsigned blk = 0, n = 0;  // blocks and tiles so far
+    unsigned blk = 0;  // blocks so far
+    // A position's row: 16 G bytes of codes, (s, z) of its groups.
+    uint4 codes[G];
+    uint2 sz[G / 2];
     while (live && walk.next(p, a, part)) {
+      const uint8_t* const rows =
+          head_tiles(p, a.slot_of[part.b], part.h) + kv * (L::kTileBytes / 2) + dw * L::kTileBytes;
+      auto load = [&](int j) {
+        if (j >= part.hi || j * kBlock + row >= part.kend) return;
+        const uint8_t* const tile = rows + (long long)j * (kBlock / kTile) * L::kTileBytes;
+#pragma unroll
+        for (int i = 0; i < G; ++i) codes[i] = __ldcg(reinterpret_cast<const uint4*>(tile + lane * 16 * G) + i);
+#pragma unroll
+        for (int i = 0; i < G / 2; ++i)
+          sz[i] = __ldcg(reinterpret_cast<const uint2*>(tile + kTile * 16 * G + lane * G * 4) + i);
+      };
+      load(part.lo);
       for (int j = part.lo; j < part.hi && live; ++j, ++blk) {
-        const int key0 = j * kBlock, here = min(kBlock / kTile, (part.kend - key0 + kTile - 1) / kTile);
-        const bool tile = dw < here, ok = key0 + row < part.kend;
-        const unsigned s = (n + dw) % kRing;
-        if (tile) live = wait_copies(bar(kRawFull + s), ((n + dw) / kRing) & 1);
-        if (blk >= 2) live = live && wait_copies(bar(kKEmpty + (blk & 1)), ((blk >> 1) - 1) & 1);
+        const bool ok = j * kBlock + row < part.kend;
+        uint4 w[G];
+        uint32_t par[G];
+#pragma unroll
+        for (int i = 0; i < G; ++i) w[i] = codes[i];
+#pragma unroll
+        for (int i = 0; i < G / 2; ++i) {
+          par[2 * i] = sz[i].x;
+          par[2 * i + 1] = sz[i].y;
+        }
+        load(j + 1);
+        if (blk >= 2) live = wait_copies(bar((kv ? kVEmpty : kKEmpty) + (blk & 1)), ((blk >> 1) - 1) & 1);
         if (!__all_sync(0xffffffffu, live)) {
           live = false;
           break;
         }
-        const uint8_t* const t8 = mem + L::raw + s * L::kTileBytes;
-        // A lane starts at its own chunk, so that eight lanes' 16-byte reads lie in
-        // distinct banks; C chunks of 16 bytes a row.
-        constexpr int C = G;  // 16 G bytes
+        const uint32_t dst = base + (kv ? L::v : L::k) + (blk & 1) * L::kOperand + out_row;
+        // eight channels, number o8 of the row
+        auto put = [&](int o8, uint32_t x, uint32_t sz8) {
+          sts4(dst + (o8 / 8) * (kBlock * 128) + (((o8 & 7) ^ (row & 7)) * 16), operand8<T>(x, sz8));
+        };
+        if (!ok) {  // no such position: its value must not count, and its weight is zero
+          if (kv)
+            for (int c = 0; c < D / 8; ++c)
+              sts4(dst + (c / 8) * (kBlock * 128) + (((c % 8) ^ (row & 7)) * 16), make_uint4(0u, 0u, 0u, 0u));
+        } else {
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const uint32_t dst = base + (kv ? L::v : L::k) + (blk & 1) * L::kOperand + out_row;
-          if (kv) {
-            if (blk >= 2) live = wait_copies(bar(kVEmpty + (blk & 1)), ((blk >> 1) - 1) & 1);
-            if (!__all_sync(0xffffffffu, live)) {
-              live = false;
-              break;
+          for (int c = 0; c < G; ++c) {  // 16-byte chunks of the row
+            uint4 x = w[c];
+            if (G == 4) {
+              int quarter = c;
+              if (kv) {  // the values' order is turned by position; half words of channels 8 q .. and 8 q + 4 ..
+                quarter = c ^ (((lane >> 1) & 1) * 2);
+                x = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632),
+                               __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+              }
+              put(quarter, x.x, par[0]);
+              put(4 + quarter, x.y, par[1]);
+              put(8 + quarter, x.z, par[G - 2]);
+              put(12 + quarter, x.w, par[G - 1]);
+            } else {
+              if (kv)
+                x = make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632),
+                               __byte_perm(x.z, x.w, 0x5410), __byte_perm(x.z, x.w, 0x7632));
+              put(2 * c, x.x, par[0]);
+              put(4 + 2 * c, x.y, par[1]);
+              put(2 * c + 1, x.z, par[0]);
+              put(4 + 2 * c + 1, x.w, par[1]);
             }
           }
-          if (!ok) {  // no such position: its value must not count, and its weight is zero
-            if (kv)
-              for (int c = 0; c < D / 8; ++c)
-                sts4(dst + (c / 8) * (kBlock * 128) + (((c % 8) ^ (row & 7)) * 16), make_uint4(0u, 0u, 0u, 0u));
-          } else {
-            const uint8_t* const half = t8 + kv * (L::kTileBytes / 2);
-            const uint8_t* const codes = half + lane * 16 * G;
-            uint32_t sz[G];
-#pragma unroll
-            for (int g = 0; g < G; g += 2) {
-              const uint2 w = *reinterpret_cast<const uint2*>(half + kTile * 16 * G + (lane * G + g) * 4);
-              sz[g] = w.x;
-              sz[g + 1] = w.y;
-            }
-#pragma unroll 1
-            for (int i = 0; i < C; ++i) {  // rolled, like the softmax's: the roles' loops share the instruction cache
-              const int c = (i + lane / (8 / C)) % C;  // 16-byte chunk of the row
-              const uint4 w = *reinterpret_cast<const uint4*>(codes + c * 16);
-              // its eight-channel words: quarter (of the 32 channels) and group of each
-              uint32_t x[4];
-              int quarter[4], group[4];
-              if (G == 4) {
-                const int at = kv ? c ^ (((lane >> 1) & 1) * 2) : c;  // the values' order is turned by position
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                  quarter[g] = at;
-                  group[g] = g;
-                }
-                if (kv) {  // half words of channels 8 q .. and 8 q + 4 .. , four groups each
-                  x[0] = __byte_perm(w.x, w.z, 0x5410);
-                  x[1] = __byte_perm(w.x, w.z, 0x7632);
-                  x[2] = __byte_perm(w.y, w.w, 0x5410);
-                  x[3] = __byte_perm(w.y, w.w, 0x7632);
-                } else {
-                  x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
-                }
-              } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  quarter[k] = 2 * c + k / 2;
-                  group[k] = k & 1;
-                }
-                if (kv) {
-                  x[0] = __byte_perm(w.x, w.y, 0x5410);
-                  x[1] = __byte_perm(w.x, w.y, 0x7632);
-                  x[2] = __byte_perm(w.z, w.w, 0x5410);
-                  x[3] = __byte_perm(w.z, w.w, 0x7632);
-                } else {
-                  x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
-                }
-              }
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int o8 = 4 * group[k] + quarter[k];  // which eight channels of the row
-                sts4(dst + (group[k] / 2) * (kBlock * 128) + (((o8 & 7) ^ (row & 7)) * 16), operand8<T>(x[k], sz[group[k]]));
-              }
-            }
-          }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar((kv ? kVFull : kKFull) + (blk & 1)));
         }
-        if (!live) break;
-        if (tile && lane == 0) mbar_arrive(bar(kRawEmpty + s));
-        n += here;
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar((kv ? kVFull : kKFull) + (blk & 1)));
       }
     }
   } else {
     // ------------------------------------------------------------ queries, softmax, epilogue
-    const int r = threadIdx.x;  // row of the segment = TMEM lane
-    const uint32_t trow = tmem + ((uint32_t)(warp * 32) << 16);
+    const int quad = warp & 3, hx = warp >> 2, r = quad * 32 + lane;  // row of the segment = TMEM lane; half
+    const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16);
+    float* const told = reinterpret_cast<float*>(mem + L::rows);
     const uint32_t prow = base + L::p + (uint32_t)r * 128u;
     constexpr int kShare = kRows * (4 + D);  // floats of a part in the workspace
     bool live = true;
-    unsigned blk = 0, met = 0;
-    // the four warps meet (bounded, unlike a hardware barrier: one may have given up)
+    unsigned blk = 0, met = 0, paired = 0;
+    // What the row's other thread has to tell (the two warps of the same rows meet).
+    auto exchange = [&](float x) {
+      const int buf = paired & 1;
+      told[(buf * 2 + hx) * kRows + r] = x;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kPair + quad));
+      live = __all_sync(0xffffffffu, live && wait_copies(bar(kPair + quad), buf));
+      ++paired;
+      return told[(buf * 2 + (hx ^ 1)) * kRows + r];
+    };
+    // the eight warps meet (bounded, unlike a hardware barrier: one may have given up)
     auto together = [&]() {
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(kTogether));
@@ -425,13 +393,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!part.whole) {
         w0 = shares.holder(part.seg0, blockIdx.x);
         w1 = shares.holder(part.seg0 + part.units - 1, blockIdx.x);
-        if (r == 0) open_tickets(a.tickets + w0, a.launch);
+        if (threadIdx.x == 0) open_tickets(a.tickets + w0, a.launch);
       }
       if (nb > 0) {
         if (mine) {
           const T* qp = static_cast<const T*>(a.q) + part.b * a.qs0 + tok * a.qs1 + qh * a.qs2;
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c) {
+          for (int c = hx * (D / 16); c < (hx + 1) * (D / 16); ++c) {
             uint4 w;
             if (a.q_vec) {
               w = reinterpret_cast<const uint4*>(qp)[c];
@@ -467,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (any) {
           float mx = -INFINITY;
 #pragma unroll 1
-          for (int c = 0; c < kBlock / 32; ++c) {
+          for (int c = 2 * hx; c < 2 * hx + 2; ++c) {
             float v[32];
             tmem_ld32(ts + c * 32, v);
             if (full) {
@@ -481,6 +449,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (c * 32 + e < lim) mx = fmaxf(mx, v[e]);
             }
           }
+          mx = fmaxf(mx, exchange(mx));
+          if (!live) break;
           const float mn = fmaxf(m, mx * a.scale_log2);
           alpha = m == -INFINITY ? 0.f : ex2(m - mn);
           m = mn;
@@ -496,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
           if (any && !__all_sync(0xffffffffu, alpha == 1.f || !mine)) {
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
+            for (int c = hx * (D / 64); c < (hx + 1) * (D / 64); ++c) {
               float v[32];
               tmem_ld32(to + c * 32, v);
 #pragma unroll
@@ -509,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float base_m = m == -INFINITY ? 0.f : m;
           float lp[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-          for (int c = 0; c < kBlock / 32; ++c) {
+          for (int c = 2 * hx; c < 2 * hx + 2; ++c) {
             float v[32];
             tmem_ld32(ts + c * 32, v);
             uint32_t w[16];
@@ -534,8 +504,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           l += (lp[0] + lp[1]) + (lp[2] + lp[3]);
         } else if (used) {  // all masked: weights of zero
 #pragma unroll
-          for (int c = 0; c < kBlock / 8; ++c)
-            sts4(prow + (c / 8) * (kRows * 128) + (((c % 8) ^ (r & 7)) * 16), make_uint4(0u, 0u, 0u, 0u));
+          for (int c = 0; c < 8; ++c)
+            sts4(prow + hx * (kRows * 128) + ((c ^ (r & 7)) * 16), make_uint4(0u, 0u, 0u, 0u));
         }
         fence_async_smem();
         tc_fence_before();
@@ -547,6 +517,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         live = __all_sync(0xffffffffu, live);
         tc_fence_after();
       }
+      if (!live) break;
+      l += exchange(l);
       if (!live) break;
       T* const op = static_cast<T*>(a.out) + (((long long)part.b * a.tq + tok) * a.QH + qh) * D;
       // a row's 32 columns, in the operands' order, as the output's channels
@@ -568,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (used) {
           const float inv = 1.0f / l;
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
+          for (int c = hx * (D / 64); c < (hx + 1) * (D / 64); ++c) {
             float v[32];
             tmem_ld32(trow + 2 * kBlock + c * 32, v);
             if (mine) store(c, v, inv);
@@ -579,9 +551,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---- other CTAs hold parts of the segment
       float* own = a.ws + ((long long)blockIdx.x * 2 + part.which) * kShare + r * (4 + D);
       if (used) {
-        if (mine) __stcg(reinterpret_cast<float4*>(own), make_float4(m, l, 0.f, 0.f));
+        if (mine && hx == 0) __stcg(reinterpret_cast<float4*>(own), make_float4(m, l, 0.f, 0.f));
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = hx * (D / 64); c < (hx + 1) * (D / 64); ++c) {
           float v[32];
           if (nb > 0) tmem_ld32(trow + 2 * kBlock + c * 32, v);
           if (mine && nb > 0)
@@ -592,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!together()) break;
-      if (r == 0) {
+      if (threadIdx.x == 0) {
         const unsigned taken = take_ticket(a.tickets + w0);
         if (taken == w1 - w0 + 1) a.tickets[w0] = 0;  // clean for the next launch
         taken_sh = taken;
@@ -611,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!(ml.x == -INFINITY && ml.y == 0.f)) ls = fmaf(ex2(ml.x - mx), ml.y, ls);
         }
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = hx * (D / 64); c < (hx + 1) * (D / 64); ++c) {
           float x[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[e] = 0.f;
