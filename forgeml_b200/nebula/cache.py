@@ -33,6 +33,7 @@ from __future__ import annotations
 
 import ctypes
 import heapq
+import math
 
 import torch
 
@@ -114,6 +115,20 @@ class KV4Pool:
                                 device=device, dtype=torch.uint8)
         self._struct = _native.neb_kv4_pool(self.data.data_ptr(), slots, heads, max_seq_len, head_dim, code)
         self.handle = ctypes.byref(self._struct)
+        self.scale = 1.0 / math.sqrt(head_dim)
+        self._workspace: dict[tuple[int, int, int], int] = {}
+
+    def workspace_bytes(self, batch: int, t: int, q_heads: int) -> int:
+        """Device memory that ``ops.kv4_attention`` needs for a call of this shape."""
+        key = (batch, t, q_heads)
+        need = self._workspace.get(key)
+        if need is None:
+            with torch.cuda.device(self.device):
+                need = int(_native.load().neb_kv4_attention_workspace_size(self.handle, batch, t, q_heads))
+            if len(self._workspace) >= 4096:
+                self._workspace.clear()
+            self._workspace[key] = need
+        return need
 
     @property
     def nbytes(self) -> int:

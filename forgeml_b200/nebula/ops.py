@@ -8,7 +8,7 @@ arguments (ValueError) and select the pool's device.
 
 from __future__ import annotations
 
-import contextlib
+import functools
 import math
 
 import torch
@@ -46,42 +46,66 @@ def attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, slot_
     return out
 
 
-def _on_device(device: torch.device):
-    return torch.cuda.device(device) if torch.cuda.current_device() != device.index else contextlib.nullcontext()
+# The kv4_* wrappers run once per layer and step, outside captured graphs too, so
+# their checks are plain attribute comparisons and their strides' arrays are kept
+# by value.
+_I32 = torch.int32
+_get_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
-def _kv4_tables(pool, slot_of: torch.Tensor, start_pos: torch.Tensor | None, batch: int | None = None) -> int:
-    """Check a batch's slot and position tables; returns the batch size."""
-    for name, t in (("slot_of", slot_of), ("start_pos", start_pos)):
-        if t is None and name == "start_pos":
-            continue
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous 1-D int32 tensor")
-        if t.device != pool.device:
-            raise ValueError(f"{name} must be on the pool's device")
-        if batch is None:
-            batch = t.shape[0]
-        if t.shape[0] != batch:
-            raise ValueError(f"{name} must hold one entry per request")
+def _raw_stream(index: int) -> int:
+    return _get_stream(index) if _get_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+@functools.lru_cache(maxsize=1024)
+def _kv4_strides(s0: int, s1: int, s2: int):
+    return _native.strides4((s0, s1, s2, 1))
+
+
+def _kv4_call(pool, name: str, *args) -> None:
+    """One C call on the pool's device and its current stream."""
+    index = pool.device.index
+    if torch.cuda.current_device() == index:
+        _native.call(name, *args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            _native.call(name, *args, _raw_stream(index))
+
+
+def _kv4_table(pool, name: str, t: torch.Tensor) -> int:
+    """Check a batch's slot or position table; returns its length."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not _I32 or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous 1-D int32 tensor")
+    if t.device != pool.device:
+        raise ValueError(f"{name} must be on the pool's device")
+    return t.shape[0]
+
+
+def _kv4_tables(pool, slot_of: torch.Tensor, start_pos: torch.Tensor | None) -> int:
+    """Check a batch's tables; returns the batch size."""
+    batch = _kv4_table(pool, "slot_of", slot_of)
+    if start_pos is not None and _kv4_table(pool, "start_pos", start_pos) != batch:
+        raise ValueError("start_pos must hold one entry per request")
     if batch == 0:
         raise ValueError("the batch must not be empty")
     return batch
 
 
-def _kv4_rows(pool, name: str, x: torch.Tensor) -> torch.Tensor:
+def _kv4_rows(pool, name: str, x: torch.Tensor, batch: int):
+    """Check rows [B, T, heads, head_dim]; returns T, heads and the strides' array."""
     if not isinstance(x, torch.Tensor) or x.dim() != 4:
         raise ValueError(f"{name} must be a tensor [B, T, heads, head_dim]")
-    if x.device != pool.device or x.dtype != pool.dtype:
+    if x.dtype is not pool.dtype or x.device != pool.device:
         raise ValueError(f"{name} must match the pool's device and dtype")
-    if x.shape[1] == 0 or x.shape[3] != pool.head_dim:
+    b, t, heads, d = x.shape
+    if b != batch or t == 0 or d != pool.head_dim:
         raise ValueError(f"bad {name} shape {tuple(x.shape)}")
-    if x.stride(3) != 1 and pool.head_dim > 1:
+    s0, s1, s2, s3 = x.stride()
+    if s3 != 1 and d > 1:
         raise ValueError(f"{name} needs unit stride in the head dimension")
-    return x
-
-
-def _kv4_strides(x: torch.Tensor):
-    return _native.strides4((x.stride(0), x.stride(1), x.stride(2), 1))
+    if t > pool.max_seq_len:
+        raise ValueError("more rows than the pool's max_seq_len")
+    return t, heads, _kv4_strides(s0, s1, s2)
 
 
 def kv4_append(k: torch.Tensor, v: torch.Tensor, pool, slot_of: torch.Tensor, start_pos: torch.Tensor) -> None:
@@ -93,16 +117,14 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, pool, slot_of: torch.Tensor, st
     the device error word's bit 4 is raised, as for a slot or position outside
     the pool, whose rows are not written."""
     b = _kv4_tables(pool, slot_of, start_pos)
-    for name, x in (("k", k), ("v", v)):
-        _kv4_rows(pool, name, x)
-        if x.shape[0] != b or x.shape[1] != k.shape[1] or x.shape[2] != pool.heads:
-            raise ValueError(f"bad {name} shape {tuple(x.shape)}")
-    t = k.shape[1]
-    if t > pool.max_seq_len:
-        raise ValueError("more rows than the pool's max_seq_len")
-    with _on_device(pool.device):
-        _native.call("neb_kv4_append", k.data_ptr(), _kv4_strides(k), v.data_ptr(), _kv4_strides(v), pool.handle,
-                     slot_of.data_ptr(), start_pos.data_ptr(), b, t, _stream(k))
+    t, heads, ks = _kv4_rows(pool, "k", k, b)
+    vt, v_heads, vs = _kv4_rows(pool, "v", v, b)
+    if heads != pool.heads:
+        raise ValueError(f"bad k shape {tuple(k.shape)}")
+    if v_heads != heads or vt != t:
+        raise ValueError(f"bad v shape {tuple(v.shape)}")
+    _kv4_call(pool, "neb_kv4_append", k.data_ptr(), ks, v.data_ptr(), vs, pool.handle, slot_of.data_ptr(),
+              start_pos.data_ptr(), b, t)
 
 
 def kv4_read(pool, slot_of: torch.Tensor, count: int, *, start_pos: torch.Tensor | None = None,
@@ -116,16 +138,16 @@ def kv4_read(pool, slot_of: torch.Tensor, count: int, *, start_pos: torch.Tensor
         raise ValueError("count must be an integer in 1..max_seq_len")
     shape = (b, pool.heads, count, pool.head_dim)
     if out is None:
-        out = tuple(torch.empty(shape, dtype=pool.dtype, device=pool.device) for _ in range(2))
-    ko, vo = out
-    for x in (ko, vo):
-        if not isinstance(x, torch.Tensor) or tuple(x.shape) != shape or x.dtype != pool.dtype \
-                or x.device != pool.device or not x.is_contiguous():
-            raise ValueError(f"out must be two contiguous {shape} tensors of the pool's dtype and device")
-    with _on_device(pool.device):
-        _native.call("neb_kv4_read", pool.handle, slot_of.data_ptr(),
-                     start_pos.data_ptr() if start_pos is not None else None, count, ko.data_ptr(), vo.data_ptr(), b,
-                     _stream(ko))
+        ko = torch.empty(shape, dtype=pool.dtype, device=pool.device)
+        vo = torch.empty_like(ko)
+    else:
+        ko, vo = out
+        for x in (ko, vo):
+            if not isinstance(x, torch.Tensor) or tuple(x.shape) != shape or x.dtype is not pool.dtype \
+                    or x.device != pool.device or not x.is_contiguous():
+                raise ValueError(f"out must be two contiguous {shape} tensors of the pool's dtype and device")
+    _kv4_call(pool, "neb_kv4_read", pool.handle, slot_of.data_ptr(),
+              start_pos.data_ptr() if start_pos is not None else None, count, ko.data_ptr(), vo.data_ptr(), b)
     return ko, vo
 
 
@@ -138,23 +160,18 @@ def kv4_attention(q: torch.Tensor, pool, slot_of: torch.Tensor, start_pos: torch
     A slot or position outside the pool gives zeros and raises the device
     error word's bit 4."""
     b = _kv4_tables(pool, slot_of, start_pos)
-    _kv4_rows(pool, "q", q)
-    _, t, qh, d = q.shape
-    if q.shape[0] != b or qh == 0 or qh % pool.heads:
+    t, qh, qs = _kv4_rows(pool, "q", q, b)
+    if qh == 0 or qh % pool.heads:
         raise ValueError(f"bad q shape {tuple(q.shape)}")
-    if t > pool.max_seq_len:
-        raise ValueError("more rows than the pool's max_seq_len")
+    shape = (b, t, qh * pool.head_dim)
     if out is None:
-        out = torch.empty((b, t, qh * d), dtype=q.dtype, device=q.device)
-    elif tuple(out.shape) != (b, t, qh * d) or out.dtype != q.dtype or out.device != q.device \
-            or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous {(b, t, qh * d)} tensor of q's dtype and device")
-    with _on_device(pool.device):
-        need = int(_native.load().neb_kv4_attention_workspace_size(pool.handle, b, t, qh))
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        _native.call("neb_kv4_attention", q.data_ptr(), _kv4_strides(q), pool.handle, slot_of.data_ptr(),
-                     start_pos.data_ptr(), out.data_ptr(), b, t, qh, 1.0 / math.sqrt(d),
-                     ws.data_ptr() if need else None, need, _stream(q))
+        out = torch.empty(shape, dtype=pool.dtype, device=pool.device)
+    elif tuple(out.shape) != shape or out.dtype is not q.dtype or out.device != q.device or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {shape} tensor of q's dtype and device")
+    need = pool.workspace_bytes(b, t, qh)
+    ws = torch.empty(need, dtype=torch.uint8, device=pool.device) if need else None
+    _kv4_call(pool, "neb_kv4_attention", q.data_ptr(), qs, pool.handle, slot_of.data_ptr(), start_pos.data_ptr(),
+              out.data_ptr(), b, t, qh, pool.scale, ws.data_ptr() if need else None, need)
     return out
 
 
