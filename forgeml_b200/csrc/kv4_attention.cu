@@ -843,6 +843,8 @@ extern "C" int neb_kv4_attention(const void* q, const int64_t q_strides[4], cons
   if (q_heads % p.H != 0) return fail(FML_EINVAL, "neb_kv4_attention: q_heads must be a multiple of the pool's heads");
   if (q_strides[3] != 1) return fail(FML_EUNSUPPORTED, "neb_kv4_attention: q innermost stride must be 1");
   if (t > p.max_seq) return fail(FML_EINVAL, "neb_kv4_attention: t exceeds max_seq");
+  if (!(scale > 0.f && scale <= 3.402823466e38f))
+    return fail(FML_EINVAL, "neb_kv4_attention: scale must be positive and finite");
   if (batch > (1 << 24) || q_heads > (1 << 20) || batch * t > (1ll << 31) / q_heads / 8)
     return fail(FML_EUNSUPPORTED, "neb_kv4_attention: too many queries");
   const bool tc = kv4::tc_covers(p, pool->dtype, t, q_heads / p.H);

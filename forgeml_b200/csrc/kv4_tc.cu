@@ -6,23 +6,20 @@
 // token * group + query head within the group: UMMA M, the TMEM lanes).  Its
 // positions go by in blocks of 128, flash-attention schedule, warp-specialised:
 //
-//   warps 8-15  turn the cache's codes into 16-bit operands (8-11 the keys, 12-15
-//               the values): a lane takes a position's codes, loaded a block ahead,
-//               and writes z + c s, rounded once, into the swizzled block (two of
-//               each).  A code under the exponent of 128 (fp16: 1024) is a 16-bit
-//               number, two at a time; the channels of every eight stay in the order
-//               0 4 1 5 2 6 3 7 that this leaves, in the queries too, and are put
-//               right where the output is written;
-//   warp 16     TMEM owner and single-thread UMMA issuer: S = Q K^T of block j + 1
+//   warps 8-11  turn the cache's codes into fp16 operands: a lane takes a position's
+//               key and value, loaded a block ahead, and writes z + c s, rounded once,
+//               into the swizzled blocks (two of each).  A code under the exponent of
+//               1024 is a 16-bit number, two at a time; the channels of every eight
+//               stay in the order 0 4 1 5 2 6 3 7 that this leaves, in the queries too,
+//               and are put right where the output is written;
+//   warp 12     TMEM owner and single-thread UMMA issuer: S = Q K^T of block j + 1
 //               into the other of two TMEM score blocks while block j's softmax
 //               runs, O += P V into TMEM;
 //   warps 0-7   queries, softmax and epilogue: two threads a row, half of a block's
-//               positions (and of the output's channels) each.  (One thread a row and
-//               four warps for the operands left the schedulers two warps each and
-//               half idle.)
+//               positions (and of the output's channels) each, the scores read from
+//               TMEM once.
 //
-// Rounded below fp32: the operands (keys, values) and P, to the cache's dtype, as
-// attention over a 16-bit cache rounds them.
+// Rounded below fp32: the operands (keys, values) and P, to fp16.
 //
 // Work: either one segment per CTA (prompts: enough segments), or, for few
 // segments, equal shares of all blocks per CTA with the split segments joined by
@@ -41,8 +38,8 @@ namespace tc {
 
 constexpr int kRows = 128;   // query rows of a segment
 constexpr int kBlock = 128;  // positions of a block
-constexpr int kThreads = 544;
-constexpr int kDequant = 8, kMma = 16;  // first warps of the roles
+constexpr int kThreads = 416;
+constexpr int kDequant = 8, kMma = 12;  // first warps of the roles
 constexpr uint32_t kTmemCols = 512;               // two score blocks, the output
 
 template <int D>
@@ -53,7 +50,8 @@ struct Smem {
   static constexpr uint32_t q = 0, k = kOperand, v = 3 * kOperand, p = 5 * kOperand;
   static constexpr uint32_t bars = p + kRows * kBlock * 2;
   static constexpr uint32_t rows = bars + 512;  // what a row's two threads tell each other: [2][2][128] fp32
-  static constexpr uint32_t total = rows + 2048 + 1024;  // 1024: alignment of the base
+  static constexpr uint32_t factors = rows + 2048;  // powers of two of the tiles' keys and values: [4 blocks][2][4]
+  static constexpr uint32_t total = factors + 128 + 1024;  // 1024: alignment of the base
   static_assert(total <= 227 * 1024, "shared memory");
 };
 enum Bar : int {
@@ -75,32 +73,70 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t w) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-  else
-    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+// 64 consecutive fp32 columns of the warp's 32 TMEM lanes; complete on return.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
+      "}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+        "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]),
+        "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]),
+        "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]),
+        "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]),
+        "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
+      : "r"(taddr)
+      : "memory");
 }
 
-// A word of eight codes as eight 16-bit numbers z + c s, in the order 0 4 1 5 2 6 3 7.
-// (fp16 stays within its finite range where a rounded-up step would leave it.)
-template <typename T>
+// The tensor cores multiply fp16 numbers whatever the cache's type: bf16 numbers,
+// rounded to 8 bits once more, would double the output's error.  bf16's range is
+// kept by powers of two: of a query row, of a tile's keys and of a tile's values,
+// each chosen so that the largest number lies near 2^12 (numbers 2^-26 of that are
+// still whole); they are taken off the scores, and put on the weights.
+//
+// 2^12 over the power of two at or below x (positive, not NaN); 2^127 at most.
+__device__ __forceinline__ float power_to_12(float x) {
+  const int e = __float_as_int(x) >> 23;
+  return __int_as_float(max(1, min(254, 266 - e)) << 23);
+}
+
+// A word of eight codes as eight fp16 numbers z + c s (s, z in `sz`), in the order
+// 0 4 1 5 2 6 3 7, within the finite range that a rounded-up step could leave.
 __device__ __forceinline__ uint4 operand8(uint32_t w, uint32_t sz) {
-  using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
-  constexpr bool kHalf = std::is_same<T, __half>::value;
-  const uint32_t exponent = kHalf ? 0x64006400u : 0x43004300u, top = 0x7bff7bffu;
+  const uint32_t exponent = 0x64006400u, top = 0x7bff7bffu;
   const uint32_t ss = __byte_perm(sz, sz, 0x1010), zz = __byte_perm(sz, sz, 0x3232);
   uint32_t e[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t c = ((w >> (4 * i)) & 0x000f000fu) | exponent;
-    T2 x = __hfma2(__hsub2(*reinterpret_cast<const T2*>(&c), *reinterpret_cast<const T2*>(&exponent)),
-                   *reinterpret_cast<const T2*>(&ss), *reinterpret_cast<const T2*>(&zz));
-    if constexpr (kHalf) x = __hmin2_nan(x, *reinterpret_cast<const T2*>(&top));
+    const __half2 x =
+        __hmin2_nan(__hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), *reinterpret_cast<const __half2*>(&exponent)),
+                            *reinterpret_cast<const __half2*>(&ss), *reinterpret_cast<const __half2*>(&zz)),
+                    *reinterpret_cast<const __half2*>(&top));
     e[i] = *reinterpret_cast<const uint32_t*>(&x);
   }
   return make_uint4(e[0], e[1], e[2], e[3]);
+}
+// (s, z) of the cache's type times a power of two, in fp16; and the largest
+// number that a group can stand for.
+template <typename T>
+__device__ __forceinline__ uint32_t scaled_params(uint32_t sz, float f) {
+  if constexpr (std::is_same<T, __half>::value) {
+    return sz;
+  } else {
+    return pack2<__half>(__uint_as_float(sz << 16) * f, __uint_as_float(sz & 0xffff0000u) * f);
+  }
+}
+__device__ __forceinline__ float largest_of(uint32_t sz) {  // bf16
+  const float s = __uint_as_float(sz << 16), z = __uint_as_float(sz & 0xffff0000u);
+  return fmaxf(fabsf(z), fabsf(fmaf(15.f, s, z)));
 }
 
 // A part of a segment: its blocks [lo, hi) (those that its rows attend at all).
@@ -225,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kMma) {
     // ------------------------------------------------------------ UMMA issuer
     if (lane == 0) {
-      const int fmt = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+      const int fmt = 0;  // fp16
       const uint32_t id_s = umma_idesc(fmt, 0, 0, kBlock);  // Q (K-major) x K (K-major)
       const uint32_t id_o = umma_idesc(fmt, 0, 1, D);       // P (K-major) x V (MN-major along the head dim)
       const uint64_t dq = umma_desc_sw128(base + L::q, 16u, 1024u), dp = umma_desc_sw128(base + L::p, 16u, 1024u);
@@ -279,81 +315,96 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp >= kDequant) {
     // ------------------------------------------------------------ codes to operands
-    const int kv = (warp - kDequant) >> 2, dw = (warp - kDequant) & 3, row = dw * 32 + lane;  // row of the block
+    const int dw = warp - kDequant, row = dw * 32 + lane;  // tile, row of the block
     const uint32_t out_row = (uint32_t)row * 128u;
+    float* const factors = reinterpret_cast<float*>(mem + L::factors);
     bool live = true;
     unsigned blk = 0;  // blocks so far
-    // A position's row: 16 G bytes of codes, (s, z) of its groups.
-    uint4 codes[G];
-    uint2 sz[G / 2];
+    // A position's key and value: 16 G bytes of codes, (s, z) of its groups.
+    uint4 codes[2][G];
+    uint32_t sz[2][G];
     while (live && walk.next(p, a, part)) {
-      const uint8_t* const rows =
-          head_tiles(p, a.slot_of[part.b], part.h) + kv * (L::kTileBytes / 2) + dw * L::kTileBytes;
-      auto load = [&](int j) {
+      const uint8_t* const rows = head_tiles(p, a.slot_of[part.b], part.h) + dw * L::kTileBytes;
+      auto load = [&](int kv, int j) {
         if (j >= part.hi || j * kBlock + row >= part.kend) return;
-        const uint8_t* const tile = rows + (long long)j * (kBlock / kTile) * L::kTileBytes;
+        const uint8_t* const half = rows + (long long)j * (kBlock / kTile) * L::kTileBytes + kv * (L::kTileBytes / 2);
 #pragma unroll
-        for (int i = 0; i < G; ++i) codes[i] = __ldcg(reinterpret_cast<const uint4*>(tile + lane * 16 * G) + i);
+        for (int i = 0; i < G; ++i) codes[kv][i] = __ldcg(reinterpret_cast<const uint4*>(half + lane * 16 * G) + i);
 #pragma unroll
-        for (int i = 0; i < G / 2; ++i)
-          sz[i] = __ldcg(reinterpret_cast<const uint2*>(tile + kTile * 16 * G + lane * G * 4) + i);
+        for (int i = 0; i < G; i += 2) {
+          const uint2 x = __ldcg(reinterpret_cast<const uint2*>(half + kTile * 16 * G + lane * G * 4) + i / 2);
+          sz[kv][i] = x.x;
+          sz[kv][i + 1] = x.y;
+        }
       };
-      load(part.lo);
+      load(0, part.lo);
+      load(1, part.lo);
       for (int j = part.lo; j < part.hi && live; ++j, ++blk) {
         const bool ok = j * kBlock + row < part.kend;
-        uint4 w[G];
-        uint32_t par[G];
+        float mine = 1.f;  // lane 0: the keys' power of two, lane 1: the values'
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
-        for (int i = 0; i < G; ++i) w[i] = codes[i];
+          for (int kv = 0; kv < 2; ++kv) {
+            float big = 0.f;
 #pragma unroll
-        for (int i = 0; i < G / 2; ++i) {
-          par[2 * i] = sz[i].x;
-          par[2 * i + 1] = sz[i].y;
-        }
-        load(j + 1);
-        if (blk >= 2) live = wait_copies(bar((kv ? kVEmpty : kKEmpty) + (blk & 1)), ((blk >> 1) - 1) & 1);
-        if (!__all_sync(0xffffffffu, live)) {
-          live = false;
-          break;
-        }
-        const uint32_t dst = base + (kv ? L::v : L::k) + (blk & 1) * L::kOperand + out_row;
-        // eight channels, number o8 of the row
-        auto put = [&](int o8, uint32_t x, uint32_t sz8) {
-          sts4(dst + (o8 / 8) * (kBlock * 128) + (((o8 & 7) ^ (row & 7)) * 16), operand8<T>(x, sz8));
-        };
-        if (!ok) {  // no such position: its value must not count, and its weight is zero
-          if (kv)
-            for (int c = 0; c < D / 8; ++c)
-              sts4(dst + (c / 8) * (kBlock * 128) + (((c % 8) ^ (row & 7)) * 16), make_uint4(0u, 0u, 0u, 0u));
-        } else {
+            for (int i = 0; i < G; ++i) big = fmaxf(big, ok ? largest_of(sz[kv][i]) : 0.f);
+            const float f = power_to_12(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big))));
+            if (lane == kv) mine = f;
 #pragma unroll
-          for (int c = 0; c < G; ++c) {  // 16-byte chunks of the row
-            uint4 x = w[c];
-            if (G == 4) {
-              int quarter = c;
-              if (kv) {  // the values' order is turned by position; half words of channels 8 q .. and 8 q + 4 ..
-                quarter = c ^ (((lane >> 1) & 1) * 2);
-                x = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632),
-                               __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
-              }
-              put(quarter, x.x, par[0]);
-              put(4 + quarter, x.y, par[1]);
-              put(8 + quarter, x.z, par[G - 2]);
-              put(12 + quarter, x.w, par[G - 1]);
-            } else {
-              if (kv)
-                x = make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632),
-                               __byte_perm(x.z, x.w, 0x5410), __byte_perm(x.z, x.w, 0x7632));
-              put(2 * c, x.x, par[0]);
-              put(4 + 2 * c, x.y, par[1]);
-              put(2 * c + 1, x.z, par[0]);
-              put(4 + 2 * c + 1, x.w, par[1]);
-            }
+            for (int i = 0; i < G; ++i) sz[kv][i] = scaled_params<T>(sz[kv][i], f);
           }
         }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar((kv ? kVFull : kKFull) + (blk & 1)));
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          if (blk >= 2) live = wait_copies(bar((kv ? kVEmpty : kKEmpty) + (blk & 1)), ((blk >> 1) - 1) & 1);
+          if (!__all_sync(0xffffffffu, live)) {
+            live = false;
+            break;
+          }
+          // The powers of two, for this block's softmax.  Four blocks' lie side by side: the
+          // keys' place is free once S of the block two before is done, which was issued
+          // after the softmax of the block four before.
+          if (kv == 0 && lane < 2) factors[(blk & 3) * 8 + 4 * lane + dw] = mine;
+          const uint32_t dst = base + (kv ? L::v : L::k) + (blk & 1) * L::kOperand + out_row;
+          // eight channels, number o8 of the row
+          auto put = [&](int o8, uint32_t x, uint32_t sz8) {
+            sts4(dst + (o8 / 8) * (kBlock * 128) + (((o8 & 7) ^ (row & 7)) * 16), operand8(x, sz8));
+          };
+          if (!ok) {  // no such position: its value must not count, and its weight is zero
+            if (kv)
+              for (int c = 0; c < D / 8; ++c)
+                sts4(dst + (c / 8) * (kBlock * 128) + (((c % 8) ^ (row & 7)) * 16), make_uint4(0u, 0u, 0u, 0u));
+          } else {
+#pragma unroll
+            for (int c = 0; c < G; ++c) {  // 16-byte chunks of the row
+              uint4 x = codes[kv][c];
+              if (G == 4) {
+                int quarter = c;
+                if (kv) {  // the values' order is turned by position; half words of channels 8 q .. and 8 q + 4 ..
+                  quarter = c ^ (((lane >> 1) & 1) * 2);
+                  x = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632),
+                                 __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+                }
+                put(quarter, x.x, sz[kv][0]);
+                put(4 + quarter, x.y, sz[kv][1]);
+                put(8 + quarter, x.z, sz[kv][G - 2]);
+                put(12 + quarter, x.w, sz[kv][G - 1]);
+              } else {
+                if (kv)
+                  x = make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632),
+                                 __byte_perm(x.z, x.w, 0x5410), __byte_perm(x.z, x.w, 0x7632));
+                put(2 * c, x.x, sz[kv][0]);
+                put(4 + 2 * c, x.y, sz[kv][1]);
+                put(2 * c + 1, x.z, sz[kv][0]);
+                put(4 + 2 * c + 1, x.w, sz[kv][1]);
+              }
+            }
+          }
+          load(kv, j + 1);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar((kv ? kVFull : kKFull) + (blk & 1)));
+        }
       }
     }
   } else {
@@ -395,30 +446,63 @@ __global__ void __launch_bounds__(kThreads, 1)
         w1 = shares.holder(part.seg0 + part.units - 1, blockIdx.x);
         if (threadIdx.x == 0) open_tickets(a.tickets + w0, a.launch);
       }
+      float q_scale = a.scale_log2;  // of the scores, the row's power of two taken off
       if (nb > 0) {
+        uint4 w[D / 16];  // half of the row's channels
+        float big = 0.f;
         if (mine) {
-          const T* qp = static_cast<const T*>(a.q) + part.b * a.qs0 + tok * a.qs1 + qh * a.qs2;
+          const T* qp = static_cast<const T*>(a.q) + part.b * a.qs0 + tok * a.qs1 + qh * a.qs2 + hx * (D / 2);
 #pragma unroll
-          for (int c = hx * (D / 16); c < (hx + 1) * (D / 16); ++c) {
-            uint4 w;
+          for (int c = 0; c < D / 16; ++c) {
             if (a.q_vec) {
-              w = reinterpret_cast<const uint4*>(qp)[c];
+              w[c] = reinterpret_cast<const uint4*>(qp)[c];
             } else {
               T e[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) e[i] = qp[c * 8 + i];
-              w = *reinterpret_cast<const uint4*>(e);
+              w[c] = *reinterpret_cast<const uint4*>(e);
             }
+          }
+        }
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          if (mine) {
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+              const uint32_t x[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                big = fmaxf(big, fmaxf(fabsf(__uint_as_float(x[i] << 16)), fabsf(__uint_as_float(x[i] & 0xffff0000u))));
+            }
+          }
+          big = fmaxf(big, exchange(big));
+          if (!live) break;
+          const float f = power_to_12(big);
+          q_scale = __fdividef(a.scale_log2, f);
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t x[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              x[i] = pack2<__half>(__uint_as_float(x[i] << 16) * f, __uint_as_float(x[i] & 0xffff0000u) * f);
+            w[c] = make_uint4(x[0], x[1], x[2], x[3]);
+          }
+        }
+        if (mine) {
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            const int o8 = hx * (D / 16) + c;
             // the operands' order: 0 4 1 5 2 6 3 7
-            sts4(base + L::q + (c / 8) * (kRows * 128) + r * 128 + (((c % 8) ^ (r & 7)) * 16),
-                 make_uint4(__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632), __byte_perm(w.y, w.w, 0x5410),
-                            __byte_perm(w.y, w.w, 0x7632)));
+            sts4(base + L::q + (o8 / 8) * (kRows * 128) + r * 128 + (((o8 % 8) ^ (r & 7)) * 16),
+                 make_uint4(__byte_perm(w[c].x, w[c].z, 0x5410), __byte_perm(w[c].x, w[c].z, 0x7632),
+                            __byte_perm(w[c].y, w[c].w, 0x5410), __byte_perm(w[c].y, w[c].w, 0x7632)));
           }
         }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kQFull));
       }
+      // the values' power of two that the output is in: the least of the tiles' so far
+      float unit = __int_as_float(254 << 23);
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < nb && live; ++j, ++blk) {
         live = wait_copies(bar(kSFull + (blk & 1)), (blk >> 1) & 1);
@@ -431,30 +515,41 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int lim = row_keys - (part.lo + j) * kBlock;  // positions of the block that the row attends
         const bool full = __all_sync(0xffffffffu, lim >= kBlock || !mine);
         const bool any = __any_sync(0xffffffffu, lim > 0);
-        float alpha = 1.f;
+        const float* const f = reinterpret_cast<const float*>(mem + L::factors) + (blk & 3) * 8;
+        float alpha = 1.f, v[64], k_scale[2], v_scale[2];
         if (any) {
+          tmem_ld64(ts + 64 * hx, v);
           float mx = -INFINITY;
-#pragma unroll 1
-          for (int c = 2 * hx; c < 2 * hx + 2; ++c) {
-            float v[32];
-            tmem_ld32(ts + c * 32, v);
-            if (full) {
-              float m4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-              for (int e = 4; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], v[e]);
-              mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+          for (int c = 0; c < 2; ++c) {
+            // scores in log2 units: both powers of two off
+            k_scale[c] = std::is_same<T, __half>::value ? q_scale : fmaxf(__fdividef(q_scale, f[2 * hx + c]), 1.2e-38f);
+            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (full) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], v[32 * c + e]);
             } else {
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (c * 32 + e < lim) mx = fmaxf(mx, v[e]);
+              for (int e = 0; e < 32; ++e) {
+                if (64 * hx + 32 * c + e >= lim) v[32 * c + e] = -INFINITY;
+                m4[e & 3] = fmaxf(m4[e & 3], v[32 * c + e]);
+              }
             }
+            mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * k_scale[c]);
           }
           mx = fmaxf(mx, exchange(mx));
           if (!live) break;
-          const float mn = fmaxf(m, mx * a.scale_log2);
+          const float mn = fmaxf(m, mx);
           alpha = m == -INFINITY ? 0.f : ex2(m - mn);
           m = mn;
           l *= alpha;
+        }
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          const float least = fminf(unit, fminf(fminf(f[4], f[5]), fminf(f[6], f[7])));
+          alpha *= __fdividef(least, unit);
+          unit = least;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) v_scale[c] = __fdividef(unit, f[4 + 2 * hx + c]);
         }
         // P and the running output are free once the block before is through
         if (j > 0) {
@@ -464,41 +559,39 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           tc_fence_after();
-          if (any && !__all_sync(0xffffffffu, alpha == 1.f || !mine)) {
+          if (used && !__all_sync(0xffffffffu, alpha == 1.f || !mine)) {
 #pragma unroll 1
             for (int c = hx * (D / 64); c < (hx + 1) * (D / 64); ++c) {
-              float v[32];
-              tmem_ld32(to + c * 32, v);
+              float o[32];
+              tmem_ld32(to + c * 32, o);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] *= alpha;
-              tmem_st32(to + c * 32, v);
+              for (int e = 0; e < 32; ++e) o[e] *= alpha;
+              tmem_st32(to + c * 32, o);
             }
           }
         }
         if (any) {
-          const float base_m = m == -INFINITY ? 0.f : m;
+          const float off = m == -INFINITY ? 0.f : m;
           float lp[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-          for (int c = 2 * hx; c < 2 * hx + 2; ++c) {
-            float v[32];
-            tmem_ld32(ts + c * 32, v);
-            uint32_t w[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              float p0 = ex2(fmaf(v[e], a.scale_log2, -base_m)), p1 = ex2(fmaf(v[e + 1], a.scale_log2, -base_m));
-              if (!full) {
-                p0 = c * 32 + e < lim ? p0 : 0.f;
-                p1 = c * 32 + e + 1 < lim ? p1 : 0.f;
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // 16 bytes of P
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int x = 32 * c + 8 * i + 2 * e;
+                const float p0 = ex2(fmaf(v[x], k_scale[c], -off)), p1 = ex2(fmaf(v[x + 1], k_scale[c], -off));
+                if constexpr (std::is_same<T, __half>::value) {
+                  w[e] = pack2<__half>(p0, p1);
+                  const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                  lp[e] += g.x + g.y;  // the sum of what the tensor core multiplies
+                } else {
+                  w[e] = pack2<__half>(p0 * v_scale[c], p1 * v_scale[c]);
+                  lp[e] += p0 + p1;
+                }
               }
-              w[e / 2] = pack2<T>(p0, p1);
-              const float2 f = unpack2<T>(w[e / 2]);  // the sum of what the tensor core multiplies
-              lp[(e / 2) & 3] += f.x + f.y;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int chunk = 4 * (c % 2) + i;
-              sts4(prow + (c / 2) * (kRows * 128) + ((chunk ^ (r & 7)) * 16),
-                   make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
+              sts4(prow + hx * (kRows * 128) + (((4 * c + i) ^ (r & 7)) * 16), make_uint4(w[0], w[1], w[2], w[3]));
             }
           }
           l += (lp[0] + lp[1]) + (lp[2] + lp[3]);
@@ -520,6 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!live) break;
       l += exchange(l);
       if (!live) break;
+      const float off_unit = std::is_same<T, __half>::value ? 1.f : __fdividef(1.0f, unit);
       T* const op = static_cast<T*>(a.out) + (((long long)part.b * a.tq + tok) * a.QH + qh) * D;
       // a row's 32 columns, in the operands' order, as the output's channels
       auto store = [&](int c, const float (&v)[32], float f) {
@@ -538,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       if (part.whole) {
         if (used) {
-          const float inv = 1.0f / l;
+          const float inv = __fdividef(1.0f, l) * off_unit;
 #pragma unroll 1
           for (int c = hx * (D / 64); c < (hx + 1) * (D / 64); ++c) {
             float v[32];
@@ -560,7 +654,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
               __stcg(reinterpret_cast<float4*>(own + 4 + c * 32) + i,
-                     make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+                     make_float4(v[4 * i] * off_unit, v[4 * i + 1] * off_unit, v[4 * i + 2] * off_unit,
+                                 v[4 * i + 3] * off_unit));
         }
       }
       if (!together()) break;
