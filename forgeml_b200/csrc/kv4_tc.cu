@@ -40,15 +40,18 @@ constexpr int kRows = 128;   // query rows of a segment
 constexpr int kBlock = 128;  // positions of a block
 constexpr int kThreads = 416;
 constexpr int kDequant = 8, kMma = 12;  // first warps of the roles
-constexpr uint32_t kTmemCols = 512;               // two score blocks, the output
+// TMEM columns: two score blocks, the output, P and the queries (fp16 pairs).  P and
+// the queries as operands from TMEM halve what the products read of shared memory,
+// whose bandwidth the operands' writes and reads are bound by.
+constexpr uint32_t kTmemCols = 512, kTmemO = 2 * kBlock, kTmemP = 384, kTmemQ = 448;
 
 template <int D>
 struct Smem {
   static constexpr int G = D / 32, kSlabs = D / 64;  // 128-byte slabs along the head dim
   static constexpr uint32_t kTileBytes = 2 * kTile * G * (16 + 4);
   static constexpr uint32_t kOperand = kRows * D * 2;
-  static constexpr uint32_t q = 0, k = kOperand, v = 3 * kOperand, p = 5 * kOperand;
-  static constexpr uint32_t bars = p + kRows * kBlock * 2;
+  static constexpr uint32_t k = 0, v = 2 * kOperand;
+  static constexpr uint32_t bars = 4 * kOperand;
   static constexpr uint32_t rows = bars + 512;  // what a row's two threads tell each other: [2][2][128] fp32
   static constexpr uint32_t factors = rows + 2048;  // powers of two of the tiles' keys and values: [4 blocks][2][4]
   static constexpr uint32_t total = factors + 128 + 1024;  // 1024: alignment of the base
@@ -92,6 +95,28 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
         "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]),
         "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
       : "r"(taddr)
+      : "memory");
+}
+
+// 16 columns of 32 bits (32 fp16 numbers of a row); tmem_st_wait() completes them.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&w)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]), "r"(w[9]),
+      "r"(w[10]), "r"(w[11]), "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D[tmem] (+)= A[tmem] * B[smem desc]^T: A's row is its TMEM lane, two fp16 numbers a
+// column.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
@@ -264,7 +289,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int fmt = 0;  // fp16
       const uint32_t id_s = umma_idesc(fmt, 0, 0, kBlock);  // Q (K-major) x K (K-major)
       const uint32_t id_o = umma_idesc(fmt, 0, 1, D);       // P (K-major) x V (MN-major along the head dim)
-      const uint64_t dq = umma_desc_sw128(base + L::q, 16u, 1024u), dp = umma_desc_sw128(base + L::p, 16u, 1024u);
       bool live = true;
       unsigned blk = 0, parts = 0, s_issued = 0, o_issued = 0;
       auto scores = [&](unsigned n) {
@@ -276,8 +300,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int sl = 0; sl < L::kSlabs; ++sl)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t off = (uint32_t)(sl * kRows * 128 + k * 32) >> 4;
-            umma_f16(tmem + (n & 1) * kBlock, dq + off, dk + off, id_s, (sl | k) != 0);
+            const uint32_t off = (uint32_t)(sl * kBlock * 128 + k * 32) >> 4;
+            umma_f16_ts(tmem + (n & 1) * kBlock, tmem + kTmemQ + (4 * sl + k) * 8, dk + off, id_s, (sl | k) != 0);
           }
         umma_commit(bar(kSFull + (n & 1)));
         umma_commit(bar(kKEmpty + (n & 1)));
@@ -299,9 +323,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint64_t dv = umma_desc_sw128(base + L::v + (blk & 1) * L::kOperand, (uint32_t)(kBlock * 128), 1024u);
 #pragma unroll
           for (int k = 0; k < kBlock / 16; ++k) {
-            const uint32_t poff = (uint32_t)((k / 4) * kRows * 128 + (k % 4) * 32) >> 4;
             const uint32_t voff = (uint32_t)(k * 16 * 128) >> 4;
-            umma_f16(tmem + 2 * kBlock, dp + poff, dv + voff, id_o, (j | k) != 0);
+            umma_f16_ts(tmem + kTmemO, tmem + kTmemP + k * 8, dv + voff, id_o, (j | k) != 0);
           }
           umma_commit(bar(kOFull));
           umma_commit(bar(kVEmpty + (blk & 1)));
@@ -412,7 +435,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quad = warp & 3, hx = warp >> 2, r = quad * 32 + lane;  // row of the segment = TMEM lane; half
     const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16);
     float* const told = reinterpret_cast<float*>(mem + L::rows);
-    const uint32_t prow = base + L::p + (uint32_t)r * 128u;
     constexpr int kShare = kRows * (4 + D);  // floats of a part in the workspace
     bool live = true;
     unsigned blk = 0, met = 0, paired = 0;
@@ -448,7 +470,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       float q_scale = a.scale_log2;  // of the scores, the row's power of two taken off
       if (nb > 0) {
-        uint4 w[D / 16];  // half of the row's channels
+        uint4 w[D / 16];  // half of the row's channels; zeros where there is no row
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) w[c] = make_uint4(0u, 0u, 0u, 0u);
         float big = 0.f;
         if (mine) {
           const T* qp = static_cast<const T*>(a.q) + part.b * a.qs0 + tok * a.qs1 + qh * a.qs2 + hx * (D / 2);
@@ -487,17 +511,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             w[c] = make_uint4(x[0], x[1], x[2], x[3]);
           }
         }
-        if (mine) {
+        // the operands' order: 0 4 1 5 2 6 3 7
 #pragma unroll
-          for (int c = 0; c < D / 16; ++c) {
-            const int o8 = hx * (D / 16) + c;
-            // the operands' order: 0 4 1 5 2 6 3 7
-            sts4(base + L::q + (o8 / 8) * (kRows * 128) + r * 128 + (((o8 % 8) ^ (r & 7)) * 16),
-                 make_uint4(__byte_perm(w[c].x, w[c].z, 0x5410), __byte_perm(w[c].x, w[c].z, 0x7632),
-                            __byte_perm(w[c].y, w[c].w, 0x5410), __byte_perm(w[c].y, w[c].w, 0x7632)));
+        for (int c = 0; c < D / 16; c += 4) {
+          uint32_t x[16];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[4 * i] = __byte_perm(w[c + i].x, w[c + i].z, 0x5410);
+            x[4 * i + 1] = __byte_perm(w[c + i].x, w[c + i].z, 0x7632);
+            x[4 * i + 2] = __byte_perm(w[c + i].y, w[c + i].w, 0x5410);
+            x[4 * i + 3] = __byte_perm(w[c + i].y, w[c + i].w, 0x7632);
           }
+          tmem_st16(trow + kTmemQ + hx * (D / 4) + 4 * c, x);
         }
-        fence_async_smem();
+        tmem_st_wait();
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kQFull));
       }
@@ -511,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         tc_fence_after();
-        const uint32_t ts = trow + (blk & 1) * kBlock, to = trow + 2 * kBlock;
+        const uint32_t ts = trow + (blk & 1) * kBlock, to = trow + kTmemO;
         const int lim = row_keys - (part.lo + j) * kBlock;  // positions of the block that the row attends
         const bool full = __all_sync(0xffffffffu, lim >= kBlock || !mine);
         const bool any = __any_sync(0xffffffffu, lim > 0);
@@ -575,32 +603,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           float lp[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
+            uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {  // 16 bytes of P
-              uint32_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int x = 32 * c + 8 * i + 2 * e;
-                const float p0 = ex2(fmaf(v[x], k_scale[c], -off)), p1 = ex2(fmaf(v[x + 1], k_scale[c], -off));
-                if constexpr (std::is_same<T, __half>::value) {
-                  w[e] = pack2<__half>(p0, p1);
-                  const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-                  lp[e] += g.x + g.y;  // the sum of what the tensor core multiplies
-                } else {
-                  w[e] = pack2<__half>(p0 * v_scale[c], p1 * v_scale[c]);
-                  lp[e] += p0 + p1;
-                }
+            for (int e = 0; e < 16; ++e) {
+              const int x = 32 * c + 2 * e;
+              const float p0 = ex2(fmaf(v[x], k_scale[c], -off)), p1 = ex2(fmaf(v[x + 1], k_scale[c], -off));
+              if constexpr (std::is_same<T, __half>::value) {
+                w[e] = pack2<__half>(p0, p1);
+                const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                lp[e & 3] += g.x + g.y;  // the sum of what the tensor core multiplies
+              } else {
+                w[e] = pack2<__half>(p0 * v_scale[c], p1 * v_scale[c]);
+                lp[e & 3] += p0 + p1;
               }
-              sts4(prow + hx * (kRows * 128) + (((4 * c + i) ^ (r & 7)) * 16), make_uint4(w[0], w[1], w[2], w[3]));
             }
+            tmem_st16(trow + kTmemP + 32 * hx + 16 * c, w);
           }
+          tmem_st_wait();
           l += (lp[0] + lp[1]) + (lp[2] + lp[3]);
         } else if (used) {  // all masked: weights of zero
-#pragma unroll
-          for (int c = 0; c < 8; ++c)
-            sts4(prow + hx * (kRows * 128) + ((c ^ (r & 7)) * 16), make_uint4(0u, 0u, 0u, 0u));
+          const uint32_t w[16] = {};
+          tmem_st16(trow + kTmemP + 32 * hx, w);
+          tmem_st16(trow + kTmemP + 32 * hx + 16, w);
+          tmem_st_wait();
         }
-        fence_async_smem();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kPFull));
@@ -636,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (int c = hx * (D / 64); c < (hx + 1) * (D / 64); ++c) {
             float v[32];
-            tmem_ld32(trow + 2 * kBlock + c * 32, v);
+            tmem_ld32(trow + kTmemO + c * 32, v);
             if (mine) store(c, v, inv);
           }
         }
@@ -649,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int c = hx * (D / 64); c < (hx + 1) * (D / 64); ++c) {
           float v[32];
-          if (nb > 0) tmem_ld32(trow + 2 * kBlock + c * 32, v);
+          if (nb > 0) tmem_ld32(trow + kTmemO + c * 32, v);
           if (mine && nb > 0)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
