@@ -108,6 +108,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&w)[16
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 // D[tmem] (+)= A[tmem] * B[smem desc]^T: A's row is its TMEM lane, two fp16 numbers a
 // column.
 __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
@@ -285,56 +290,60 @@ __global__ void __launch_bounds__(kThreads, 1)
   Part part;
   if (warp == kMma) {
     // ------------------------------------------------------------ UMMA issuer
-    if (lane == 0) {
-      const int fmt = 0;  // fp16
-      const uint32_t id_s = umma_idesc(fmt, 0, 0, kBlock);  // Q (K-major) x K (K-major)
-      const uint32_t id_o = umma_idesc(fmt, 0, 1, D);       // P (K-major) x V (MN-major along the head dim)
-      bool live = true;
-      unsigned blk = 0, parts = 0, s_issued = 0, o_issued = 0;
-      auto scores = [&](unsigned n) {
-        live = live && wait_copies(bar(kKFull + (n & 1)), (n >> 1) & 1);
-        if (!live) return;
-        tc_fence_after();
-        const uint64_t dk = umma_desc_sw128(base + L::k + (n & 1) * L::kOperand, 16u, 1024u);
+    // The whole warp walks along (its values are then the same in every lane, which
+    // the products' operands must be); one lane issues.  It polls: its answer to P is
+    // on the blocks' critical path.
+    const uint32_t id_s = umma_idesc(0, 0, 0, kBlock);  // fp16: Q (TMEM) x K (K-major)
+    const uint32_t id_o = umma_idesc(0, 0, 1, D);       // P (TMEM) x V (MN-major along the head dim)
+    const bool leader = elect_one();
+    const uint64_t dk0 = umma_desc_sw128(base + L::k, 16u, 1024u);
+    const uint64_t dv0 = umma_desc_sw128(base + L::v, (uint32_t)(kBlock * 128), 1024u);
+    bool live = true;
+    unsigned blk = 0, parts = 0, s_issued = 0, o_issued = 0;
+    auto await = [&](int b, uint32_t parity) {
+      live = __all_sync(0xffffffffu, live && mbar_wait(bar(b), parity, DEV_ERR_ATTN_TIMEOUT));
+      return live;
+    };
+    auto scores = [&](unsigned n) {
+      if (!await(kKFull + (n & 1), (n >> 1) & 1)) return;
+      tc_fence_after();
+      if (leader) {
+        const uint64_t dk = dk0 + (n & 1) * (L::kOperand >> 4);
+        const uint32_t to = tmem + (n & 1) * kBlock;
 #pragma unroll
-        for (int sl = 0; sl < L::kSlabs; ++sl)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t off = (uint32_t)(sl * kBlock * 128 + k * 32) >> 4;
-            umma_f16_ts(tmem + (n & 1) * kBlock, tmem + kTmemQ + (4 * sl + k) * 8, dk + off, id_s, (sl | k) != 0);
-          }
+        for (int k = 0; k < D / 16; ++k)
+          umma_f16_ts(to, tmem + kTmemQ + k * 8, dk + (uint32_t)(((k / 4) * kBlock * 128 + (k % 4) * 32) >> 4), id_s, k != 0);
         umma_commit(bar(kSFull + (n & 1)));
         umma_commit(bar(kKEmpty + (n & 1)));
-        s_issued = n + 1;
-      };
-      while (live && walk.next(p, a, part)) {
-        const int nb = part.hi - part.lo;
-        if (nb == 0) continue;
-        live = wait_copies(bar(kQFull), parts & 1);
-        ++parts;
-        if (!live) break;
-        scores(blk);
-        for (int j = 0; j < nb && live; ++j, ++blk) {
-          if (j + 1 < nb) scores(blk + 1);
-          live = live && wait_copies(bar(kPFull), blk & 1) &&
-                 wait_copies(bar(kVFull + (blk & 1)), (blk >> 1) & 1);
-          if (!live) break;
-          tc_fence_after();
-          const uint64_t dv = umma_desc_sw128(base + L::v + (blk & 1) * L::kOperand, (uint32_t)(kBlock * 128), 1024u);
+      }
+      __syncwarp();
+      s_issued = n + 1;
+    };
+    while (live && walk.next(p, a, part)) {
+      const int nb = part.hi - part.lo;
+      if (nb == 0) continue;
+      if (!await(kQFull, parts & 1)) break;
+      ++parts;
+      scores(blk);
+      for (int j = 0; j < nb && live; ++j, ++blk) {
+        if (j + 1 < nb) scores(blk + 1);
+        if (!await(kVFull + (blk & 1), (blk >> 1) & 1) || !await(kPFull, blk & 1)) break;
+        tc_fence_after();
+        if (leader) {
+          const uint64_t dv = dv0 + (blk & 1) * (L::kOperand >> 4);
 #pragma unroll
-          for (int k = 0; k < kBlock / 16; ++k) {
-            const uint32_t voff = (uint32_t)(k * 16 * 128) >> 4;
-            umma_f16_ts(tmem + kTmemO, tmem + kTmemP + k * 8, dv + voff, id_o, (j | k) != 0);
-          }
+          for (int k = 0; k < kBlock / 16; ++k)
+            umma_f16_ts(tmem + kTmemO, tmem + kTmemP + k * 8, dv + (uint32_t)((k * 16 * 128) >> 4), id_o, (j | k) != 0);
           umma_commit(bar(kOFull));
           umma_commit(bar(kVEmpty + (blk & 1)));
-          o_issued = blk + 1;
         }
+        __syncwarp();
+        o_issued = blk + 1;
       }
-      // every UMMA issued completes before TMEM is released
-      if (s_issued > 0) wait_copies(bar(kSFull + ((s_issued - 1) & 1)), ((s_issued - 1) >> 1) & 1);
-      if (o_issued > 0) wait_copies(bar(kOFull), (o_issued - 1) & 1);
     }
+    // every UMMA issued completes before TMEM is released
+    if (s_issued > 0) mbar_wait(bar(kSFull + ((s_issued - 1) & 1)), ((s_issued - 1) >> 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+    if (o_issued > 0) mbar_wait(bar(kOFull), (o_issued - 1) & 1, DEV_ERR_ATTN_TIMEOUT);
     __syncwarp();
   } else if (warp >= kDequant) {
     // ------------------------------------------------------------ codes to operands
