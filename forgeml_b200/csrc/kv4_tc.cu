@@ -765,9 +765,15 @@ static int launch(const Pool& p, const Problem& a, int row_tiles, bool shared, c
 
 }  // namespace tc
 
-// Whether the tensor-core kernel takes the call.
+// Whether the tensor-core kernel takes the call: more than 8 query rows of a
+// key/value head.  Up to there the row kernel, which goes over the cache once per
+// row (from L2 after the first), is the faster one or near it.  Measured, row kernel
+// against this one, at 2 / 4 / 8 / 16 rows, head dim 128, bf16:
+//   16 requests x 8 heads x 6000 positions   47 / 77 / 139 / 262 against 117 .. 120 us
+//    2 requests x 8 heads x 6000             16 / 20 /  31 /  44 against  47 ..  51 us
+//    4 requests x 8 heads x 300               8 /  8 /  10 /  12 against  23 ..  24 us
 bool tc_covers(const Pool& p, int dtype, int64_t t, int64_t group) {
-  return (dtype == FML_BF16 || dtype == FML_F16) && (p.D == 64 || p.D == 128) && t * group > 1;
+  return (dtype == FML_BF16 || dtype == FML_F16) && (p.D == 64 || p.D == 128) && t * group > 8;
 }
 static bool tc_shared(const Pool& p, int64_t segments, int64_t requests_units) {
   return segments < 2 * num_sms(current_device()) && requests_units < (1ll << 31);
