@@ -19,7 +19,10 @@
 // the 16-bit types and all but the smallest channels of fp32 are exact), the
 // weights p s to 16 bits below their running bound (two digits; three, 23
 // bits, for fp16 and fp32, whose outputs keep more bits than bf16's).  Scores,
-// maxima, sums and outputs are fp32.
+// maxima, sums and outputs are fp32.  An fp32 cache's scores, whose errors the
+// exponentials pass on whole, are put together from the integers in 64 bits, and
+// its values' codes count from 8: p (z + 8 s) + p s (c - 8) keeps the bits that
+// p z + p s c, two sums of a group's whole range that all but cancel, loses.
 #include <algorithm>
 #include <atomic>
 #include <string>
@@ -268,6 +271,8 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
   using U = Unit<T, G>;
   constexpr int PP = Parts<T>::p, SETS = U::SETS, kWarps = U::warps, kStages = U::stages;
   constexpr float kPMax = PP == 3 ? 8388600.f : 65530.f;
+  constexpr bool kWide = std::is_same<T, float>::value;
+  using Score = typename std::conditional<kWide, double, float>::type;
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -379,9 +384,10 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
   const int my_pos = 16 * (li >> 2) + 4 * (li & 3) + ((li & 1) ? lt ^ 1 : lt);
 
   uint32_t qa[G][4];  // A: this lane's bytes, zero outside its row's group
-  float qsum[G], unit_q = 0.f;
+  Score qsum[G], unit_q = 0;
   int accm[G][4], accr[G][4];                                // sums of P lo and of P (lo + 16 hi)
   int accm3[PP == 3 ? G : 1][4], accr3[PP == 3 ? G : 1][4];  // third digits
+  int ones[kWide ? SETS : 1][4], ones3[kWide ? SETS : 1][4];  // sums of P: the codes count from 8 then
   float zacc[G], to_int[G], m = -INFINITY, l = 0.f;
   float* const o = reinterpret_cast<float*>(mem + U::out) + lane;  // channel 32 gi + 4 g + i: o[(4 gi + i) * 32]
   int stage = 0, since = 0;
@@ -406,12 +412,14 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
       for (int h = 0; h < 2; ++h) {
         const int e = 2 * h + (gi & 1);
         float* const x = o + (4 * gi + 2 * h) * 32;
-        float x0 = fmaf((float)accm[gi][e], d1, x[0] * scale);
-        float x1 = fmaf((float)(accr[gi][e] - accm[gi][e]), d1 * 0.0625f, x[32] * scale);
+        const int w = kWide ? ones[gi / 4][e] : 0;
+        float x0 = fmaf((float)(accm[gi][e] - 8 * w), d1, x[0] * scale);
+        float x1 = fmaf((float)(accr[gi][e] - accm[gi][e] - 128 * w), d1 * 0.0625f, x[32] * scale);
         if constexpr (PP == 3) {
           if (t < 2) {
-            x0 = fmaf((float)accm3[gi][e], u, x0);
-            x1 = fmaf((float)(accr3[gi][e] - accm3[gi][e]), u * 0.0625f, x1);
+            const int w3 = kWide ? ones3[gi / 4][e] : 0;
+            x0 = fmaf((float)(accm3[gi][e] - 8 * w3), u, x0);
+            x1 = fmaf((float)(accr3[gi][e] - accm3[gi][e] - 128 * w3), u * 0.0625f, x1);
           }
         }
         x[0] = x0;
@@ -422,6 +430,12 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
         accm[gi][e] = accr[gi][e] = 0;
         if constexpr (PP == 3) accm3[gi][e] = accr3[gi][e] = 0;
       }
+    }
+    if constexpr (kWide) {
+#pragma unroll
+      for (int s = 0; s < SETS; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ones[s][e] = ones3[s][e] = 0;
     }
   };
 
@@ -467,16 +481,18 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
     const bool sound = big <= 3.402823466e38f;
     const float to_q = big > 0.f && sound ? fminf(__fdividef(kQMax, big), 1e37f) : 0.f;
     // scores = (integer sums / 16) * unit_q + minima's share, in log2 units
-    unit_q = sound ? (to_q > 0.f ? __fdividef(0.0625f, to_q) * a.scale_log2 : 0.f) : NAN;
+    if constexpr (kWide) unit_q = sound ? (to_q > 0.f ? 0.0625 / to_q * a.scale_log2_wide : 0.0) : (double)NAN;
+    else unit_q = sound ? (to_q > 0.f ? __fdividef(0.0625f, to_q) * a.scale_log2 : 0.f) : NAN;
     const int hi = g < 4 ? 3 : 1;
 #pragma unroll
     for (int s = 0; s < SETS; ++s) {
-      float sum = 0.f;
+      Score sum = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum += x[s][i];
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      sum *= a.scale_log2;
+      if constexpr (kWide) sum *= a.scale_log2_wide;
+      else sum *= a.scale_log2;
       uint32_t r[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -507,6 +523,12 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
       }
       zacc[gi] = 0.f;
       to_int[gi] = kToInt0;
+    }
+    if constexpr (kWide) {
+#pragma unroll
+      for (int s = 0; s < SETS; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ones[s][e] = ones3[s][e] = 0;
     }
     m = -INFINITY;
     l = 0.f;
@@ -539,30 +561,36 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
       for (int s = 0; s < SETS; ++s)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float4 f;
-          f.x = (float)(c[s][2 * i][0] * 256 + c[s][2 * i][2]);
-          f.y = (float)(c[s][2 * i][1] * 256 + c[s][2 * i][3]);
-          f.z = (float)(c[s][2 * i + 1][0] * 256 + c[s][2 * i + 1][2]);
-          f.w = (float)(c[s][2 * i + 1][1] * 256 + c[s][2 * i + 1][3]);
-          *reinterpret_cast<float4*>(dots + s * 8 * 36 + g * 36 + t * 8 + 4 * i) = f;
+          const int4 f = make_int4(c[s][2 * i][0] * 256 + c[s][2 * i][2], c[s][2 * i][1] * 256 + c[s][2 * i][3],
+                                   c[s][2 * i + 1][0] * 256 + c[s][2 * i + 1][2],
+                                   c[s][2 * i + 1][1] * 256 + c[s][2 * i + 1][3]);
+          float* const at = dots + s * 8 * 36 + g * 36 + t * 8 + 4 * i;
+          if constexpr (kWide) *reinterpret_cast<int4*>(at) = f;
+          else *reinterpret_cast<float4*>(at) = make_float4((float)f.x, (float)f.y, (float)f.z, (float)f.w);
         }
       __syncwarp();
       const bool part = nk < kUnit, valid = my_pos < nk;
       float step[G], low[G];
       lds_params<T, G>(st + U::kp + my_pos * U::PR, part, valid, step, low);
-      float x = 0.f, y = 0.f;
+      Score x = 0, y = 0;
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) {
         const float* d = dots + (gi / 4) * 8 * 36 + (gi & 3) * 36 + lane;
-        x = fmaf(step[gi], fmaf(d[0], 65536.f, d[4 * 36]), x);
-        y = fmaf(low[gi], qsum[gi], y);
+        if constexpr (kWide) {
+          const int* e = reinterpret_cast<const int*>(d);
+          x = fma((double)step[gi], fma((double)e[0], 65536.0, (double)e[4 * 36]), x);
+          y = fma((double)low[gi], qsum[gi], y);
+        } else {
+          x = fmaf(step[gi], fmaf(d[0], 65536.f, d[4 * 36]), x);
+          y = fmaf(low[gi], qsum[gi], y);
+        }
       }
-      const float sc = valid ? fmaf(x, unit_q, y) : -INFINITY;
-      const float mx = warp_max(sc);
+      const Score sc = valid ? x * unit_q + y : (Score)-INFINITY;
+      const float mx = warp_max((float)sc);
       lds_params<T, G>(st + U::vp + my_pos * U::PR, part, valid, step, low);
       // ---- weights, as integers up to kPMax
       const float mn = fmaxf(m, mx);
-      const float pr = valid ? ex2(sc - mn) : 0.f;
+      const float pr = valid ? ex2((float)(sc - mn)) : 0.f;
       float n[G];
       bool over = false;
 #pragma unroll
@@ -594,7 +622,7 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
       ++since;
       l += pr;
 #pragma unroll
-      for (int gi = 0; gi < G; ++gi) zacc[gi] = fmaf(pr, low[gi], zacc[gi]);
+      for (int gi = 0; gi < G; ++gi) zacc[gi] = fmaf(pr, kWide ? fmaf(8.f, step[gi], low[gi]) : low[gi], zacc[gi]);
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) {
         const uint32_t w = __float_as_uint(n[gi]);
@@ -615,6 +643,11 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
         const uint8_t* d = digits + s * (PP == 3 ? 16 : 8) * 32 + t * 8;
         pb[s] = *reinterpret_cast<const uint2*>(d + g * 32);
         if constexpr (PP == 3) pb3[s] = *reinterpret_cast<const uint2*>(d + (8 + (g & 3)) * 32);
+        if constexpr (kWide) {
+          constexpr uint32_t k1 = 0x01010101u;
+          mma_u8u8(ones[s], k1, k1, k1, k1, pb[s].x, pb[s].y);
+          mma_u8u8(ones3[s], k1, k1, k1, k1, pb3[s].x, pb3[s].y);
+        }
       }
 
       // ---- output: per word (two groups) the bytes of four rows change places
@@ -862,6 +895,7 @@ extern "C" int neb_kv4_attention(const void* q, const int64_t q_strides[4], cons
   a.qs1 = q_strides[1];
   a.qs2 = q_strides[2];
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2_wide = (double)scale * 1.4426950408889634;
   const size_t es = dtype_size(pool->dtype);
   a.q_vec = p.D % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_strides[0] * es % 16 == 0 &&
             q_strides[1] * es % 16 == 0 && q_strides[2] * es % 16 == 0;

@@ -19,6 +19,7 @@ struct Problem {
   long long qs0, qs1, qs2;
   bool q_vec, out_vec;  // 16-byte loads of q, 8-byte stores of the output
   float scale_log2;  // softmax scale * log2(e)
+  double scale_log2_wide;
   const void* q;
   void* out;
   // Workspace: the CTAs' shares of the segments that they hold in part, then a
