@@ -54,7 +54,8 @@ struct Smem {
   static constexpr uint32_t bars = 4 * kOperand;
   static constexpr uint32_t rows = bars + 512;  // what a row's two threads tell each other: [2][2][128] fp32
   static constexpr uint32_t factors = rows + 2048;  // powers of two of the tiles' keys and values: [4 blocks][2][4]
-  static constexpr uint32_t total = factors + 128 + 1024;  // 1024: alignment of the base
+  static constexpr uint32_t nans = factors + 128;   // first position whose value is NaN: [4 parts][4 tiles][4 groups]
+  static constexpr uint32_t total = nans + 256 + 1024;  // 1024: alignment of the base
   static_assert(total <= 227 * 1024, "shared memory");
 };
 enum Bar : int {
@@ -131,10 +132,11 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
 // each chosen so that the largest number lies near 2^12 (numbers 2^-26 of that are
 // still whole); they are taken off the scores, and put on the weights.
 //
-// 2^12 over the power of two at or below x (positive, not NaN); 2^127 at most.
+// 2^12 over the power of two at or below x (positive, not NaN); 2^126 at most (a
+// fast division by more gives 0).
 __device__ __forceinline__ float power_to_12(float x) {
   const int e = __float_as_int(x) >> 23;
-  return __int_as_float(max(1, min(254, 266 - e)) << 23);
+  return __int_as_float(max(1, min(253, 266 - e)) << 23);
 }
 
 // A word of eight codes as eight fp16 numbers z + c s (s, z in `sz`), in the order
@@ -167,6 +169,14 @@ __device__ __forceinline__ uint32_t scaled_params(uint32_t sz, float f) {
 __device__ __forceinline__ float largest_of(uint32_t sz) {  // bf16
   const float s = __uint_as_float(sz << 16), z = __uint_as_float(sz & 0xffff0000u);
   return fmaxf(fabsf(z), fabsf(fmaf(15.f, s, z)));
+}
+
+// Whether a group's numbers are NaN, as its parameters are: an exponent of ones, plus
+// one, carries into the sign's place.
+template <typename T>
+__device__ __forceinline__ uint32_t reads_nan(uint32_t sz) {
+  constexpr bool half = std::is_same<T, __half>::value;
+  return ((sz & (half ? 0x7c007c00u : 0x7f807f80u)) + (half ? 0x04000400u : 0x00800080u)) & 0x80008000u;
 }
 
 // A part of a segment: its blocks [lo, hi) (those that its rows attend at all).
@@ -350,8 +360,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int dw = warp - kDequant, row = dw * 32 + lane;  // tile, row of the block
     const uint32_t out_row = (uint32_t)row * 128u;
     float* const factors = reinterpret_cast<float*>(mem + L::factors);
+    int* const nans = reinterpret_cast<int*>(mem + L::nans);
     bool live = true;
-    unsigned blk = 0;  // blocks so far
+    unsigned blk = 0, parts = 0;  // blocks so far, parts with blocks
     // A position's key and value: 16 G bytes of codes, (s, z) of its groups.
     uint4 codes[2][G];
     uint32_t sz[2][G];
@@ -371,8 +382,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       load(0, part.lo);
       load(1, part.lo);
+      int nan = 0x7fffffff;  // lane i: the part's first position where group i's value is NaN
       for (int j = part.lo; j < part.hi && live; ++j, ++blk) {
         const bool ok = j * kBlock + row < part.kend;
+        // A weight of zero does not undo a value of NaN: it counts as 0 here, and the rows
+        // that attend it are told.
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < G; ++i) bad |= reads_nan<T>(sz[1][i]);
+        if (__any_sync(0xffffffffu, ok && bad != 0)) {
+#pragma unroll
+          for (int i = 0; i < G; ++i) {
+            const bool mine = ok && reads_nan<T>(sz[1][i]) != 0;
+            const uint32_t who = __ballot_sync(0xffffffffu, mine);
+            if (mine) sz[1][i] = 0;
+            if (who != 0 && lane == i) nan = min(nan, j * kBlock + dw * 32 + __ffs((int)who) - 1);
+          }
+        }
         float mine = 1.f;  // lane 0: the keys' power of two, lane 1: the values'
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
@@ -397,6 +423,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           // keys' place is free once S of the block two before is done, which was issued
           // after the softmax of the block four before.
           if (kv == 0 && lane < 2) factors[(blk & 3) * 8 + 4 * lane + dw] = mine;
+          // likewise four parts': S of a part's first block is issued after the softmax's
+          // warps have read all of the part before
+          if (kv == 0 && lane < G) nans[(parts & 3) * 16 + 4 * dw + lane] = nan;
           const uint32_t dst = base + (kv ? L::v : L::k) + (blk & 1) * L::kOperand + out_row;
           // eight channels, number o8 of the row
           auto put = [&](int o8, uint32_t x, uint32_t sz8) {
@@ -438,6 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive(bar((kv ? kVFull : kKFull) + (blk & 1)));
         }
       }
+      if (part.lo < part.hi) ++parts;
     }
   } else {
     // ------------------------------------------------------------ queries, softmax, epilogue
@@ -446,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* const told = reinterpret_cast<float*>(mem + L::rows);
     constexpr int kShare = kRows * (4 + D);  // floats of a part in the workspace
     bool live = true;
-    unsigned blk = 0, met = 0, paired = 0;
+    unsigned blk = 0, parts = 0, met = 0, paired = 0;
     // What the row's other thread has to tell (the two warps of the same rows meet).
     auto exchange = [&](float x) {
       const int buf = paired & 1;
@@ -539,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(bar(kQFull));
       }
       // the values' power of two that the output is in: the least of the tiles' so far
-      float unit = __int_as_float(254 << 23);
+      float unit = __int_as_float(253 << 23);
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < nb && live; ++j, ++blk) {
         live = wait_copies(bar(kSFull + (blk & 1)), (blk >> 1) & 1);
@@ -649,6 +679,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       l += exchange(l);
       if (!live) break;
       const float off_unit = std::is_same<T, __half>::value ? 1.f : __fdividef(1.0f, unit);
+      // whether the row attends a value of NaN in the channels of group c
+      const int* const nans = reinterpret_cast<const int*>(mem + L::nans) + (parts & 3) * 16;
+      auto nan_in = [&](int c) {
+        return nb > 0 && min(min(nans[c], nans[4 + c]), min(nans[8 + c], nans[12 + c])) < row_keys;
+      };
+      if (nb > 0) ++parts;
       T* const op = static_cast<T*>(a.out) + (((long long)part.b * a.tq + tok) * a.QH + qh) * D;
       // a row's 32 columns, in the operands' order, as the output's channels
       auto store = [&](int c, const float (&v)[32], float f) {
@@ -672,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int c = hx * (D / 64); c < (hx + 1) * (D / 64); ++c) {
             float v[32];
             tmem_ld32(trow + kTmemO + c * 32, v);
-            if (mine) store(c, v, inv);
+            if (mine) store(c, v, nan_in(c) ? NAN : inv);
           }
         }
         continue;
@@ -685,12 +721,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = hx * (D / 64); c < (hx + 1) * (D / 64); ++c) {
           float v[32];
           if (nb > 0) tmem_ld32(trow + kTmemO + c * 32, v);
+          const float f = nan_in(c) ? NAN : off_unit;
           if (mine && nb > 0)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
               __stcg(reinterpret_cast<float4*>(own + 4 + c * 32) + i,
-                     make_float4(v[4 * i] * off_unit, v[4 * i + 1] * off_unit, v[4 * i + 2] * off_unit,
-                                 v[4 * i + 3] * off_unit));
+                     make_float4(v[4 * i] * f, v[4 * i + 1] * f, v[4 * i + 2] * f, v[4 * i + 3] * f));
         }
       }
       if (!together()) break;

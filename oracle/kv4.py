@@ -34,9 +34,12 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts) -> torc
     group = qh // k.shape[2]
     out = torch.empty(b, t, qh, d, dtype=torch.float64)
     for i in range(b):
-        for j in range(t):
-            n = int(starts[i]) + j + 1
-            for h in range(qh):
-                s = k[i, :n, h // group] @ q[i, j, h] / math.sqrt(d)
-                out[i, j, h] = torch.softmax(s, 0) @ v[i, :n, h // group]
+        n = int(starts[i]) + t
+        late = torch.arange(n)[None, :] > int(starts[i]) + torch.arange(t)[:, None]
+        for h in range(qh):
+            kh, vh = k[i, :n, h // group], v[i, :n, h // group]
+            w = torch.softmax((q[i, :, h] @ kh.T / math.sqrt(d)).masked_fill(late, -math.inf), 1)
+            # a row that is not attended does not count, whatever it holds
+            nan = (~late).double() @ vh.isnan().double() > 0
+            out[i, :, h] = (w @ vh.nan_to_num(0.0)).masked_fill(nan, math.nan)
     return out.reshape(b, t, qh * d)

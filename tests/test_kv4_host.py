@@ -180,6 +180,9 @@ def test_c_entries_check_their_arguments():
     _rejects("neb_kv4_attention", EINVAL, "positive", FAKE, s4, p, FAKE, FAKE, FAKE, 1, 1, 0, 0.1, FAKE, 1 << 40, None)
     _rejects("neb_kv4_attention", EINVAL, "multiple of the pool's heads", FAKE, s4, p, FAKE, FAKE, FAKE, 1, 1, 3, 0.1, FAKE, 1 << 40, None)
     _rejects("neb_kv4_attention", EUNSUPPORTED, "innermost stride", FAKE, s5, p, FAKE, FAKE, FAKE, 1, 1, 2, 0.1, FAKE, 1 << 40, None)
+    for scale in (0.0, -1.0, float("inf"), float("nan")):
+        _rejects("neb_kv4_attention", EINVAL, "positive and finite", FAKE, s4, p, FAKE, FAKE, FAKE, 1, 1, 2, scale, FAKE,
+                 1 << 40, None)
     _rejects("neb_kv4_attention", EINVAL, "exceeds max_seq", FAKE, s4, p, FAKE, FAKE, FAKE, 1, 65, 2, 0.1, FAKE, 1 << 40, None)
     _rejects("neb_kv4_attention", EUNSUPPORTED, "too many queries", FAKE, s4, p, FAKE, FAKE, FAKE, 1 << 24, 64, 1 << 20,
              0.1, FAKE, 1 << 40, None)
