@@ -16,9 +16,9 @@
 //   keys' codes [32][16 G bytes], keys' parameters [32][G][2] (s, z) in T,
 //   values' codes, values' parameters.
 //
-// Order of the codes within a row.  The attention kernel feeds codes straight
-// to mma.sync.m16n8k16 fragments; the order makes a thread's codes of all
-// groups one contiguous chunk, for keys and for values.
+// Order of the codes within a row.  The row kernel feeds bytes of codes to
+// mma.sync m16n8k32 operands as they lie; the order makes a thread's codes of
+// all groups one contiguous chunk, for keys and for values.
 //   keys:   chunk t (of 4, 4 G bytes) holds for each group one 32-bit word,
 //           its channels 8 t .. 8 t + 7;
 //   values: chunk l (of 8, 2 G bytes) holds for each group one 16-bit word,

@@ -11,9 +11,17 @@
 // lo + 16 hi.  It is used twice: as it lies, and with its upper half masked off:
 //   16 (q0 lo + q1 hi) = q1 (lo + 16 hi) + (16 q0 - q1) lo
 //   sum P hi = (sum P (lo + 16 hi) - sum P lo) / 16
-// so eight codes cost one logic instruction for the keys.  (Spreading them into
-// bfloat16 operands costs seven, and the integer ALU was what bounded that
-// form: 44 us against 15 us for 64 requests of 128 .. 2303 positions.)
+// so eight codes cost one logic instruction for the keys.  Spreading them into
+// bfloat16 operands costs seven, and the integer ALU was what bounded that form:
+// 44 us for 64 requests of 128 .. 2303 positions (8 heads of 128, bf16), 30 us now.
+//
+// Measured (bf16, heads of 128, device time):
+//   32 requests x 16 heads x 512 .. 639    17.4 us   2.7 TB/s of cache
+//   64 requests x  8 heads x 128 .. 2303   29.6 us   3.4
+//    1 request  x 16 heads x 100001        49.9 us   5.1
+// Long streams come near the memory's rate; what is left of the shorter ones is
+// latency: about 2 us until the first copies are issued, 1 to 2 us for a segment's
+// query, flush and output, and the join where segments are split.
 //
 // What is rounded: q to 27 bits below its largest channel (four 8-bit digits;
 // the 16-bit types and all but the smallest channels of fp32 are exact), the

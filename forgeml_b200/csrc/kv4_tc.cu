@@ -19,7 +19,14 @@
 //               positions (and of the output's channels) each, the scores read from
 //               TMEM once.
 //
-// Rounded below fp32: the operands (keys, values) and P, to fp16.
+// Rounded below fp32: the operands (keys, values) and P, to fp16, whose 11 bits cost
+// the output no more than its own rounding to the cache's type.
+//
+// Measured: 8 x 1000 tokens after 0 .. 1048 others, 16 heads of 128, bf16: 217 us,
+// 308 TFLOP/s; 16 requests of 4000 .. 8190 positions, 8 heads of 128 with 4 query
+// heads each, go through the row kernel (tc_covers).  A block of 128 positions takes
+// about 4400 cycles, bound by the softmax warps' chain (scores from TMEM, maximum,
+// exponentials, P to TMEM), with the dequantisation hidden behind it.
 //
 // Work: either one segment per CTA (prompts: enough segments), or, for few
 // segments, equal shares of all blocks per CTA with the split segments joined by

@@ -86,9 +86,10 @@ class KV4Pool:
     numbers (at most 256) of ``dtype``.
 
     Per group of 32 channels a row keeps the minimum and a step in ``dtype``
-    and a 4-bit code per channel: 4.5 to 5 bits a number for 16-bit types at
-    the usual head sizes (2 bytes of codes and 4 bytes of parameters per 4 and
-    32 channels), against 16.  The format is stated in
+    and a 4-bit code per channel: 5 bits a number for 16-bit types against 16,
+    and 6 for fp32 against 32, where head_dim is a multiple of 32 (a shorter
+    last group takes a whole group's room, and positions go by 32).  The
+    format is stated in
     include/forgeml_b200.h; ``ops.kv4_append`` writes rows, ``ops.kv4_read``
     gives them back as numbers and ``ops.kv4_attention`` attends over them in
     place.  Rows never written hold whatever the memory held."""
@@ -111,8 +112,12 @@ class KV4Pool:
         self.slots, self.heads, self.max_seq_len, self.head_dim = slots, heads, max_seq_len, head_dim
         self.device, self.dtype = device, dtype
         code = _native.dtype_code(dtype)
-        self.data = torch.empty(_native.load().neb_kv4_pool_bytes(slots, heads, max_seq_len, head_dim, code),
-                                device=device, dtype=torch.uint8)
+        need = 0
+        if max(sizes.values()) <= 1 << 30:
+            need = int(_native.load().neb_kv4_pool_bytes(slots, heads, max_seq_len, head_dim, code))
+        if need == 0:
+            raise CacheError("the 4-bit cache's pool is too large")
+        self.data = torch.empty(need, device=device, dtype=torch.uint8)
         self._struct = _native.neb_kv4_pool(self.data.data_ptr(), slots, heads, max_seq_len, head_dim, code)
         self.handle = ctypes.byref(self._struct)
         self.scale = 1.0 / math.sqrt(head_dim)

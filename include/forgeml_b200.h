@@ -254,6 +254,8 @@ typedef struct neb_kv4_pool {
   int32_t dtype;
 } neb_kv4_pool;
 
+/* 0 for sizes or a dtype that are not covered (slots and max_seq up to 2^30,
+ * heads up to 2^18, head_dim up to 256). */
 FML_API size_t neb_kv4_pool_bytes(int64_t slots, int64_t heads, int64_t max_seq, int64_t head_dim, int dtype);
 /* Quantise k and v [B,T,H,D] (dtype of the pool, element strides, innermost 1)
  * into rows start_pos[b] .. start_pos[b]+T-1.  The requests of a batch hold
@@ -272,7 +274,11 @@ FML_API int neb_kv4_read(const neb_kv4_pool* pool, const int32_t* slot_of, const
  * attends rows 0 .. start_pos[b]+t.  q is [B,T,q_heads,D] (dtype of the pool,
  * element strides, innermost 1), q_heads a multiple of the pool's heads: query
  * head h reads head h / (q_heads / heads).  out is [B,T,q_heads*D] contiguous.
- * Scores, softmax and the sums over the rows in fp32. */
+ * scale is positive and finite.  Scores, softmax and the sums over the rows in
+ * fp32; more than 8 query rows of a head (16-bit types, D 64 or 128) run on the
+ * tensor cores with keys, values and weights rounded to fp16.  Queries without
+ * a place in the pool give zeros and raise bit 4.  Rows past a query's position
+ * count nothing, whatever they hold. */
 FML_API int neb_kv4_attention(const void* q, const int64_t q_strides[4], const neb_kv4_pool* pool,
                       const int32_t* slot_of, const int32_t* start_pos, void* out,
                       int64_t batch, int64_t t, int64_t q_heads, float scale,

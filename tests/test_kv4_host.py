@@ -26,6 +26,9 @@ CPU = torch.device("cpu")
     (dict(head_dim=257), "head_dim <= 256"),
     (dict(dtype=torch.float64), "not supported"),
     (dict(device=CPU), "needs a CUDA device"),
+    (dict(slots=1 << 64), "too large"),
+    (dict(heads=1 << 19), "too large"),
+    (dict(slots=1 << 30, heads=1 << 18, max_seq_len=1 << 30), "too large"),  # would wrap round 64 bits
 ])
 def test_pool_refusals(bad, match):
     kw = dict(slots=1, heads=1, max_seq_len=8, head_dim=64, device=torch.device("cuda", 0), dtype=torch.bfloat16)
@@ -134,6 +137,8 @@ def test_pool_sizes():
     for bad in ((0, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), (1, 1, 1, 0), (1, 1, 1, 257)):
         assert lib.neb_kv4_pool_bytes(*bad, BF16) == 0
     assert lib.neb_kv4_pool_bytes(1, 1, 1, 1, 9) == 0
+    for big in ((1 << 31, 1, 1, 1), (1, 1 << 19, 1, 1), (1, 1, 1 << 31, 1), (1 << 30, 1 << 18, 1 << 30, 256)):
+        assert lib.neb_kv4_pool_bytes(*big, BF16) == 0
 
 
 def c_pool(**kw):
