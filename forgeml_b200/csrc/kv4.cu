@@ -99,12 +99,42 @@ template <> __device__ __forceinline__ float smallest_normal<float>() { return 1
 template <> __device__ __forceinline__ float smallest_normal<__half>() { return 6.103515625e-05f; }
 template <> __device__ __forceinline__ float smallest_normal<__nv_bfloat16>() { return 1.17549435e-38f; }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ uint32_t quantise8(const Row8<T, VEC>& row, float& s, float& z) {
-  float x[8], hi;
-  row.floats(x);
-  range(row, x, z, hi);
-  const float half_range = fmaf(0.5f, hi, -0.5f * z);
+// bits of kRound + code are those of kRound plus the code: 16^i of each, summed
+__device__ __forceinline__ uint32_t pack8(const float (&q)[8]) {
+  uint32_t w = 0u - 0x4b400000u * 0x11111111u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w += __float_as_uint(q[i] + kRound) << (4 * i);
+  return w;
+}
+__device__ __forceinline__ float near_reciprocal(float u) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(u));
+  return y;
+}
+constexpr float kPerStep = 1.0f / 7.5f;  // s / half_range
+// A 16-bit step that needs none of the checks below: whether half_range is large
+// enough for a normal step and no underflow, and finite.
+template <typename T>
+__device__ __forceinline__ bool plain(float half_range) {
+  return sizeof(T) == 2 && half_range >= (std::is_same<T, __half>::value ? 5e-4f : 1e-15f) &&
+         half_range <= 3.402823466e38f;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t quantise8_plain(const float (&x)[8], float half_range, float z, float& s) {
+  const float s0 = half_range * kPerStep;
+  s = to_f32<T>(from_f32<T>(fmaf(fmaf(-s0, 7.5f, half_range), kPerStep, s0)));
+  const float u = 0.5f * s, zs = -0.5f * z, y = near_reciprocal(u);
+  float q[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float d = fmaf(x[i], 0.5f, zs), q0 = d * y;
+    q[i] = fmaf(fmaf(-q0, u, d), y, q0);
+  }
+  return pack8(q);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float half_range, float hi, float& s, float& z) {
   if (!(half_range <= 3.402823466e38f)) {  // an infinity or a NaN in the group
     s = z = NAN;
     return 0u;
@@ -115,18 +145,15 @@ __device__ __forceinline__ uint32_t quantise8(const Row8<T, VEC>& row, float& s,
   if constexpr (sizeof(T) == 4) {
     s = (float)(((double)hi - (double)z) / 15.0);
   } else {
-    constexpr float y = 1.0f / 7.5f;
-    const float q0 = half_range * y;
-    s = fmaf(fmaf(-q0, 7.5f, half_range), y, q0);
+    const float s0 = half_range * kPerStep;
+    s = fmaf(fmaf(-s0, 7.5f, half_range), kPerStep, s0);
     if (half_range < 1e-30f) s = __fdiv_rn(half_range, 7.5f);  // the remainder would underflow
     s = to_f32<T>(from_f32<T>(s));
   }
   if (s == 0.f) return 0u;
   float scale = 0.5f;
   if (s < 8.6736174e-19f) scale = 0.5f * 1.1529215e18f;  // 2^-60, 2^60
-  const float u = s * scale, zs = -z * scale;
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(u));
+  const float u = s * scale, zs = -z * scale, y = near_reciprocal(u);
   float q[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -147,11 +174,7 @@ __device__ __forceinline__ uint32_t quantise8(const Row8<T, VEC>& row, float& s,
 #pragma unroll
     for (int i = 0; i < 8; ++i) q[i] = fminf(q[i], 15.f);
   }
-  // bits of kRound + code are those of kRound plus the code: 16^i of each, summed
-  uint32_t w = 0u - 0x4b400000u * 0x11111111u;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w += __float_as_uint(q[i] + kRound) << (4 * i);
-  return w;
+  return pack8(q);
 }
 
 // Duplicate requests: true when an earlier request of the batch holds the same
@@ -209,22 +232,41 @@ __global__ void __launch_bounds__(256)
   uint8_t* const tiles = head_tiles(p, max(slot, 0), h);
   const bool pairs = (p.G & 1) == 0, odd = (g & 1) != 0;
   const int k_at = k_byte(p.G, c0), v_at = v_byte(p.G, pairs ? (g & ~1) * kGroup + quarter * 8 + (odd ? 4 : 0) : c0, 0);
-#pragma unroll 2
+  int r = (start + t0) % kTile;
+  uint8_t* tile = tiles + (long long)((start + t0) / kTile) * (2 * p.half);
+  // the next token's rows are on their way while this one's are quantised
+  Row8<T, VEC> kn, vn;
+  if (t0 < t1) {
+    kn.load(kr, src_c, p.D);
+    vn.load(vr, src_c, p.D);
+  }
+#pragma unroll 1
   for (int t = t0; t < t1; ++t, kr += ks1, vr += vs1) {
-    Row8<T, VEC> kx, vx;
-    kx.load(kr, src_c, p.D);
-    vx.load(vr, src_c, p.D);
-    const int pos = start + t, r = pos % kTile;
-    uint8_t* const tile = tiles + (long long)(pos / kTile) * (2 * p.half);
-    float ks, kz, vs, vz;
-    const uint32_t kw = quantise8(kx, ks, kz) & real;
-    const uint32_t vw = quantise8(vx, vs, vz) & real;
+    const Row8<T, VEC> kx = kn, vx = vn;
+    if (t + 1 < t1) {
+      kn.load(kr + ks1, src_c, p.D);
+      vn.load(vr + vs1, src_c, p.D);
+    }
+    float kf[8], vf[8], ks, kz, k_hi, vs, vz, v_hi;
+    kx.floats(kf);
+    vx.floats(vf);
+    range(kx, kf, kz, k_hi);
+    range(vx, vf, vz, v_hi);
+    const float k_half = fmaf(0.5f, k_hi, -0.5f * kz), v_half = fmaf(0.5f, v_hi, -0.5f * vz);
+    uint32_t kw, vw;
+    if (plain<T>(k_half) && plain<T>(v_half)) {
+      kw = quantise8_plain<T>(kf, k_half, kz, ks) & real;
+      vw = quantise8_plain<T>(vf, v_half, vz, vs) & real;
+    } else {
+      kw = quantise8<T>(kf, k_half, k_hi, ks, kz) & real;
+      vw = quantise8<T>(vf, v_half, v_hi, vs, vz) & real;
+    }
     uint8_t* const vrow = tile + p.half + r * 16 * p.G;
     const uint32_t vx2 = pairs ? swap_halves(vw, odd) : 0u;
     if (live) {
       *reinterpret_cast<uint32_t*>(tile + r * 16 * p.G + k_at) = kw;
       if (pairs) {
-        *reinterpret_cast<uint32_t*>(vrow + (v_at ^ v_swizzle(p.G, pos))) = vx2;
+        *reinterpret_cast<uint32_t*>(vrow + (v_at ^ v_swizzle(p.G, r))) = vx2;
       } else {
         *reinterpret_cast<uint16_t*>(vrow + v_at) = (uint16_t)vw;
         *reinterpret_cast<uint16_t*>(vrow + v_at + 2 * p.G) = (uint16_t)(vw >> 16);
@@ -235,6 +277,10 @@ __global__ void __launch_bounds__(256)
         if (sizeof(T) == 4) *reinterpret_cast<uint2*>(at) = *reinterpret_cast<uint2*>(sz);
         else *reinterpret_cast<uint32_t*>(at) = *reinterpret_cast<uint32_t*>(sz);
       }
+    }
+    if (++r == kTile) {
+      r = 0;
+      tile += 2 * p.half;
     }
   }
 }
