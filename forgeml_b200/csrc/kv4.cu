@@ -99,13 +99,19 @@ template <> __device__ __forceinline__ float smallest_normal<float>() { return 1
 template <> __device__ __forceinline__ float smallest_normal<__half>() { return 6.103515625e-05f; }
 template <> __device__ __forceinline__ float smallest_normal<__nv_bfloat16>() { return 1.17549435e-38f; }
 
-// bits of kRound + code are those of kRound plus the code: 16^i of each, summed
-__device__ __forceinline__ uint32_t pack8(const float (&q)[8]) {
-  uint32_t w = 0u - 0x4b400000u * 0x11111111u;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w += __float_as_uint(q[i] + kRound) << (4 * i);
-  return w;
+// Rounds eight quotients and lays the codes side by side, on the fp32 pipe (the
+// integer one is what bounds the kernel).  Adding 16^i q to 1.5 * 2^(23 + 4 i), whose
+// last place is 16^i, rounds q to an integer (ties to even: what lies above is a
+// multiple of 2 * 16^i) above the codes still to come; taking it down to 1.5 *
+// 2^(19 + 4 i) is exact.  Four codes a sum.
+__device__ __forceinline__ uint32_t pack4(const float* q) {
+  constexpr float k3 = kRound * 4096.f, k2 = kRound * 256.f, k1 = kRound * 16.f;
+  float x = __fadd_rn(fmaf(q[3], 4096.f, k3), -(k3 - k2));
+  x = __fadd_rn(fmaf(q[2], 256.f, x), -(k2 - k1));
+  x = __fadd_rn(fmaf(q[1], 16.f, x), -(k1 - kRound));
+  return __float_as_uint(__fadd_rn(x, q[0]));
 }
+__device__ __forceinline__ uint32_t pack8(const float (&q)[8]) { return __byte_perm(pack4(q), pack4(q + 4), 0x5410); }
 __device__ __forceinline__ float near_reciprocal(float u) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(u));
