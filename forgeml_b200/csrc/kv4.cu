@@ -205,9 +205,10 @@ __device__ __forceinline__ uint32_t swap_halves(uint32_t w, bool odd) {
   return odd ? __byte_perm(other, w, 0x7610) : __byte_perm(w, other, 0x5410);
 }
 
-// Work per number: 2 bytes read, 0.6 written, some 14 instructions (minimum and
-// maximum, quotient with its correction, packing), which bound it: 32 x 512 tokens x
-// 16 heads of 128 in bf16 take 62 us, 2.8 TB/s, where the bytes alone take 27.
+// Work: 2 bytes read and 0.6 written a number, and some 20 instructions (minimum
+// and maximum, the quotient with its correction, rounding, packing), whose issue
+// bounds it (0.8 of the slots): 32 x 512 tokens x 16 heads of 128 in bf16 take about
+// 45 us, 3.9 TB/s, where the bytes alone take 27.
 //
 // One thread: eight channels of one head, keys and values, of a run of a
 // request's tokens.  threadIdx.x (and blockIdx.y) = (head, group, quarter);
@@ -428,8 +429,9 @@ static int append(const void* k, const int64_t* ks, const void* v, const int64_t
   const int block = lanes >= 256 ? 256 : (lanes + 31) / 32 * 32;
   const long long gy = (lanes + block - 1) / block;
   // Tokens per block: one while blocks are few, up to 16 where they are many
-  // (the request's look-ups and addresses are made once a block).
-  const long long spread = 148LL * 16;
+  // (the request's look-ups and addresses are made once a block: about two waves of
+  // blocks, 81 us, against six, 82.4, for 32 x 512 tokens and their reading back).
+  const long long spread = 148LL * 6;
   const int run = (int)std::min<long long>(16, std::max<long long>(1, batch * t * gy / spread));
   const long long runs = (t + run - 1) / run;
   auto addressable = [&](const void* x, const int64_t* s) {
