@@ -916,7 +916,7 @@ extern "C" int neb_kv4_attention(const void* q, const int64_t q_strides[4], cons
     a.start_pos = start_pos;
     a.q = q;
     a.out = out;
-    a.out_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0;
+    a.out_vec = p.D % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
     return kv4::tc_attention(p, a, pool->dtype, st);
   }
   // Units are counted in 31 bits: a larger batch goes in slices of requests.

@@ -1,6 +1,6 @@
 // Attention of several query rows over the 4-bit key/value cache on the tcgen05
 // tensor cores: a prompt's tokens, a few drafted ones, query heads that share a
-// key/value head (16-bit types, head dim 64 or 128).
+// key/value head (16-bit types, head dim up to 128).
 //
 // A segment is a request's key/value head with up to 128 of its query rows (row =
 // token * group + query head within the group: UMMA M, the TMEM lanes).  Its
@@ -52,11 +52,11 @@ constexpr int kDequant = 8, kMma = 12;  // first warps of the roles
 // whose bandwidth the operands' writes and reads are bound by.
 constexpr uint32_t kTmemCols = 512, kTmemO = 2 * kBlock, kTmemP = 384, kTmemQ = 448;
 
-template <int D>
+template <int G>
 struct Smem {
-  static constexpr int G = D / 32, kSlabs = D / 64;  // 128-byte slabs along the head dim
+  static constexpr int D = 32 * G, kSlabs = (G + 1) / 2;  // 128-byte slabs along the head dim
   static constexpr uint32_t kTileBytes = 2 * kTile * G * (16 + 4);
-  static constexpr uint32_t kOperand = kRows * D * 2;
+  static constexpr uint32_t kOperand = kRows * 128 * kSlabs;
   static constexpr uint32_t k = 0, v = 2 * kOperand;
   static constexpr uint32_t bars = 4 * kOperand;
   static constexpr uint32_t rows = bars + 512;  // what a row's two threads tell each other: [2][2][128] fp32
@@ -229,13 +229,13 @@ struct Walk {
   }
 };
 
-template <typename T, int D>
+template <typename T, int G>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_tc_kernel(const Pool p, const Problem a, const int row_tiles, const int shared_blocks) {
-  using L = Smem<D>;
-  constexpr int G = L::G;
+  using L = Smem<G>;
+  constexpr int D = L::D;  // channels of whole groups; the row has p.D of them
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  static_assert(G == 2 || G == 4, "head dim 64 or 128");
+  static_assert(G >= 1 && G <= 4, "TMEM columns of O and Q");
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const mem = smem_raw + (base - smem_u32(smem_raw));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -293,8 +293,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int keys = keys_of(p, a, b), good = keys == 0 ? 0 : min(a.tq, keys - a.start_pos[b]);
     if (good == a.tq) continue;
     if (threadIdx.x == 0) raise_device_error(DEV_ERR_ATTN_RANGE);
-    const long long n = (long long)(a.tq - good) * a.QH * D;
-    T* bad = static_cast<T*>(a.out) + ((long long)b * a.tq + good) * a.QH * D;
+    const long long n = (long long)(a.tq - good) * a.QH * p.D;
+    T* bad = static_cast<T*>(a.out) + ((long long)b * a.tq + good) * a.QH * p.D;
     for (long long i = threadIdx.x; i < n; i += kThreads) bad[i] = from_f32<T>(0.f);
   }
   tc_fence_before();
@@ -380,11 +380,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint8_t* const half = rows + (long long)j * (kBlock / kTile) * L::kTileBytes + kv * (L::kTileBytes / 2);
 #pragma unroll
         for (int i = 0; i < G; ++i) codes[kv][i] = __ldcg(reinterpret_cast<const uint4*>(half + lane * 16 * G) + i);
+        if constexpr (G % 2 != 0) {
 #pragma unroll
-        for (int i = 0; i < G; i += 2) {
-          const uint2 x = __ldcg(reinterpret_cast<const uint2*>(half + kTile * 16 * G + lane * G * 4) + i / 2);
-          sz[kv][i] = x.x;
-          sz[kv][i + 1] = x.y;
+          for (int i = 0; i < G; ++i)
+            sz[kv][i] = __ldcg(reinterpret_cast<const uint32_t*>(half + kTile * 16 * G + lane * G * 4) + i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < G; i += 2) {
+            const uint2 x = __ldcg(reinterpret_cast<const uint2*>(half + kTile * 16 * G + lane * G * 4) + i / 2);
+            sz[kv][i] = x.x;
+            sz[kv][i + 1] = x.y;
+          }
         }
       };
       load(0, part.lo);
@@ -443,10 +449,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int c = 0; c < D / 8; ++c)
                 sts4(dst + (c / 8) * (kBlock * 128) + (((c % 8) ^ (row & 7)) * 16), make_uint4(0u, 0u, 0u, 0u));
           } else {
+            if constexpr (G == 4) {
 #pragma unroll
-            for (int c = 0; c < G; ++c) {  // 16-byte chunks of the row
-              uint4 x = codes[kv][c];
-              if (G == 4) {
+              for (int c = 0; c < G; ++c) {  // 16-byte chunks of the row
+                uint4 x = codes[kv][c];
                 int quarter = c;
                 if (kv) {  // the values' order is turned by position; half words of channels 8 q .. and 8 q + 4 ..
                   quarter = c ^ (((lane >> 1) & 1) * 2);
@@ -457,14 +463,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 put(4 + quarter, x.y, sz[kv][1]);
                 put(8 + quarter, x.z, sz[kv][G - 2]);
                 put(12 + quarter, x.w, sz[kv][G - 1]);
-              } else {
-                if (kv)
-                  x = make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632),
-                                 __byte_perm(x.z, x.w, 0x5410), __byte_perm(x.z, x.w, 0x7632));
-                put(2 * c, x.x, sz[kv][0]);
-                put(4 + 2 * c, x.y, sz[kv][1]);
-                put(2 * c + 1, x.z, sz[kv][0]);
-                put(4 + 2 * c + 1, x.w, sz[kv][1]);
+              }
+            } else {
+              const uint32_t* const w = reinterpret_cast<const uint32_t*>(codes[kv]);
+#pragma unroll
+              for (int i = 0; i < 4 * G; ++i) {
+                const int quarter = i / G, group = i % G;
+                uint32_t x = w[i];
+                if (kv) {  // half words of channels 8 q .. and 8 q + 4 ..
+                  const int h0 = 2 * quarter * G + group, h1 = h0 + G;
+                  x = __byte_perm(w[h0 / 2], w[h1 / 2], (h0 % 2 ? 0x32 : 0x10) | (h1 % 2 ? 0x7600 : 0x5400));
+                }
+                put(4 * group + quarter, x, sz[kv][group]);
               }
             }
           }
@@ -481,6 +491,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quad = warp & 3, hx = warp >> 2, r = quad * 32 + lane;  // row of the segment = TMEM lane; half
     const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16);
     float* const told = reinterpret_cast<float*>(mem + L::rows);
+    // the thread's share of the channels, in groups
+    constexpr int kHalf = (G + 1) / 2;
+    const int group0 = hx ? kHalf : 0, group1 = hx ? G : kHalf;
     constexpr int kShare = kRows * (4 + D);  // floats of a part in the workspace
     bool live = true;
     unsigned blk = 0, parts = 0, met = 0, paired = 0;
@@ -516,20 +529,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       float q_scale = a.scale_log2;  // of the scores, the row's power of two taken off
       if (nb > 0) {
-        uint4 w[D / 16];  // half of the row's channels; zeros where there is no row
+        uint4 w[4 * kHalf];  // the thread's groups' channels; zeros where there is no row or channel
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) w[c] = make_uint4(0u, 0u, 0u, 0u);
+        for (int c = 0; c < 4 * kHalf; ++c) w[c] = make_uint4(0u, 0u, 0u, 0u);
         float big = 0.f;
         if (mine) {
-          const T* qp = static_cast<const T*>(a.q) + part.b * a.qs0 + tok * a.qs1 + qh * a.qs2 + hx * (D / 2);
+          const T* qp = static_cast<const T*>(a.q) + part.b * a.qs0 + tok * a.qs1 + qh * a.qs2;
 #pragma unroll
-          for (int c = 0; c < D / 16; ++c) {
+          for (int c = 0; c < 4 * kHalf; ++c) {
+            const int c0 = 32 * group0 + 8 * c;
+            if (c0 >= p.D) continue;
             if (a.q_vec) {
-              w[c] = reinterpret_cast<const uint4*>(qp)[c];
+              w[c] = *reinterpret_cast<const uint4*>(qp + c0);
             } else {
               T e[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) e[i] = qp[c * 8 + i];
+              for (int i = 0; i < 8; ++i) e[i] = c0 + i < p.D ? qp[c0 + i] : from_f32<T>(0.f);
               w[c] = *reinterpret_cast<const uint4*>(e);
             }
           }
@@ -537,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
           if (mine) {
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
+            for (int c = 0; c < 4 * kHalf; ++c) {
               const uint32_t x[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
 #pragma unroll
               for (int i = 0; i < 4; ++i)
@@ -549,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float f = power_to_12(big);
           q_scale = __fdividef(a.scale_log2, f);
 #pragma unroll
-          for (int c = 0; c < D / 16; ++c) {
+          for (int c = 0; c < 4 * kHalf; ++c) {
             uint32_t x[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -559,7 +574,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // the operands' order: 0 4 1 5 2 6 3 7
 #pragma unroll
-        for (int c = 0; c < D / 16; c += 4) {
+        for (int c = 0; c < 4 * kHalf; c += 4) {
+          if (group0 + c / 4 >= G) break;
           uint32_t x[16];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -568,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             x[4 * i + 2] = __byte_perm(w[c + i].y, w[c + i].w, 0x5410);
             x[4 * i + 3] = __byte_perm(w[c + i].y, w[c + i].w, 0x7632);
           }
-          tmem_st16(trow + kTmemQ + hx * (D / 4) + 4 * c, x);
+          tmem_st16(trow + kTmemQ + 16 * group0 + 4 * c, x);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -635,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
           if (used && !__all_sync(0xffffffffu, alpha == 1.f || !mine)) {
 #pragma unroll 1
-            for (int c = hx * (D / 64); c < (hx + 1) * (D / 64); ++c) {
+            for (int c = group0; c < group1; ++c) {
               float o[32];
               tmem_ld32(to + c * 32, o);
 #pragma unroll
@@ -692,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return nb > 0 && min(min(nans[c], nans[4 + c]), min(nans[8 + c], nans[12 + c])) < row_keys;
       };
       if (nb > 0) ++parts;
-      T* const op = static_cast<T*>(a.out) + (((long long)part.b * a.tq + tok) * a.QH + qh) * D;
+      T* const op = static_cast<T*>(a.out) + (((long long)part.b * a.tq + tok) * a.QH + qh) * p.D;
       // a row's 32 columns, in the operands' order, as the output's channels
       auto store = [&](int c, const float (&v)[32], float f) {
 #pragma unroll
@@ -700,11 +716,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float* x = v + 8 * i;
           const uint4 w = make_uint4(pack2<T>(x[0] * f, x[2] * f), pack2<T>(x[4] * f, x[6] * f),
                                      pack2<T>(x[1] * f, x[3] * f), pack2<T>(x[5] * f, x[7] * f));
+          const int c0 = c * 32 + 8 * i;
           if (a.out_vec) {
-            reinterpret_cast<uint4*>(op + c * 32)[i] = w;
+            if (c0 < p.D) *reinterpret_cast<uint4*>(op + c0) = w;
           } else {
             const T* e = reinterpret_cast<const T*>(&w);
-            for (int k = 0; k < 8; ++k) op[c * 32 + 8 * i + k] = e[k];
+            for (int k = 0; k < 8; ++k)
+              if (c0 + k < p.D) op[c0 + k] = e[k];
           }
         }
       };
@@ -712,7 +730,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (used) {
           const float inv = __fdividef(1.0f, l) * off_unit;
 #pragma unroll 1
-          for (int c = hx * (D / 64); c < (hx + 1) * (D / 64); ++c) {
+          for (int c = group0; c < group1; ++c) {
             float v[32];
             tmem_ld32(trow + kTmemO + c * 32, v);
             if (mine) store(c, v, nan_in(c) ? NAN : inv);
@@ -725,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (used) {
         if (mine && hx == 0) __stcg(reinterpret_cast<float4*>(own), make_float4(m, l, 0.f, 0.f));
 #pragma unroll 1
-        for (int c = hx * (D / 64); c < (hx + 1) * (D / 64); ++c) {
+        for (int c = group0; c < group1; ++c) {
           float v[32];
           if (nb > 0) tmem_ld32(trow + kTmemO + c * 32, v);
           const float f = nan_in(c) ? NAN : off_unit;
@@ -756,7 +774,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!(ml.x == -INFINITY && ml.y == 0.f)) ls = fmaf(ex2(ml.x - mx), ml.y, ls);
         }
 #pragma unroll 1
-        for (int c = hx * (D / 64); c < (hx + 1) * (D / 64); ++c) {
+        for (int c = group0; c < group1; ++c) {
           float x[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[e] = 0.f;
@@ -788,22 +806,32 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <typename T, int D>
+template <typename T, int G>
 static int launch(const Pool& p, const Problem& a, int row_tiles, bool shared, cudaStream_t st) {
   static std::atomic<bool> ready[64] = {};
   const int dev = current_device();
   if (dev < 0 || dev >= 64) return fail(FML_EUNSUPPORTED, "neb_kv4_attention: device index out of range");
   if (!ready[dev].load()) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)Smem<D>::total);
+    const cudaError_t e = cudaFuncSetAttribute(attn_tc_kernel<T, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)Smem<G>::total);
     if (e != cudaSuccess) return check_cuda(e, "neb_kv4_attention smem attribute");
     ready[dev].store(true);
   }
   const long long grid = shared ? num_sms(dev) : (long long)a.B * p.H * row_tiles;
-  const cudaError_t e = launch_pdl(attn_tc_kernel<T, D>, dim3((unsigned)grid), dim3(kThreads), Smem<D>::total, st, 1, p, a,
+  const cudaError_t e = launch_pdl(attn_tc_kernel<T, G>, dim3((unsigned)grid), dim3(kThreads), Smem<G>::total, st, 1, p, a,
                                    row_tiles, shared ? 1 : 0);
   count_launch();
   return check_cuda(e, "neb_kv4_attention launch");
+}
+
+template <typename T>
+static int launch_groups(const Pool& p, const Problem& a, int row_tiles, bool shared, cudaStream_t st) {
+  switch (p.G) {
+    case 1: return launch<T, 1>(p, a, row_tiles, shared, st);
+    case 2: return launch<T, 2>(p, a, row_tiles, shared, st);
+    case 3: return launch<T, 3>(p, a, row_tiles, shared, st);
+    default: return launch<T, 4>(p, a, row_tiles, shared, st);
+  }
 }
 
 }  // namespace tc
@@ -816,7 +844,7 @@ static int launch(const Pool& p, const Problem& a, int row_tiles, bool shared, c
 //    2 requests x 8 heads x 6000             16 / 20 /  31 /  44 against  47 ..  51 us
 //    4 requests x 8 heads x 300               8 /  8 /  10 /  12 against  23 ..  24 us
 bool tc_covers(const Pool& p, int dtype, int64_t t, int64_t group) {
-  return (dtype == FML_BF16 || dtype == FML_F16) && (p.D == 64 || p.D == 128) && t * group > 8;
+  return (dtype == FML_BF16 || dtype == FML_F16) && p.G <= 4 && t * group > 8;
 }
 static bool tc_shared(const Pool& p, int64_t segments, int64_t requests_units) {
   return segments < 2 * num_sms(current_device()) && requests_units < (1ll << 31);
@@ -825,7 +853,7 @@ size_t tc_workspace_bytes(const Pool& p, int64_t batch, int64_t t, int64_t group
   const int64_t tiles = (t * group + tc::kRows - 1) / tc::kRows, segs = batch * p.H * tiles;
   if (!tc_shared(p, segs, segs * ((p.max_seq + tc::kBlock - 1) / tc::kBlock))) return 0;
   const size_t sms = (size_t)num_sms(current_device());
-  return sms * 2 * tc::kRows * (4 + p.D) * sizeof(float) + sms * sizeof(unsigned long long);
+  return sms * 2 * tc::kRows * (4 + 32 * p.G) * sizeof(float) + sms * sizeof(unsigned long long);
 }
 int tc_attention(const Pool& p, Problem a, int dtype, cudaStream_t st) {
   const int tiles = (int)(((int64_t)a.tq * a.group + tc::kRows - 1) / tc::kRows);
@@ -835,12 +863,10 @@ int tc_attention(const Pool& p, Problem a, int dtype, cudaStream_t st) {
   a.segs = p.H * tiles;
   const size_t sms = (size_t)num_sms(current_device());
   a.tickets = reinterpret_cast<unsigned long long*>(reinterpret_cast<uint8_t*>(a.ws) +
-                                                    sms * 2 * tc::kRows * (4 + p.D) * sizeof(float));
+                                                    sms * 2 * tc::kRows * (4 + 32 * p.G) * sizeof(float));
   a.launch = launch_number();
-  if (dtype == FML_BF16)
-    return p.D == 64 ? tc::launch<__nv_bfloat16, 64>(p, a, tiles, shared, st)
-                     : tc::launch<__nv_bfloat16, 128>(p, a, tiles, shared, st);
-  return p.D == 64 ? tc::launch<__half, 64>(p, a, tiles, shared, st) : tc::launch<__half, 128>(p, a, tiles, shared, st);
+  return dtype == FML_BF16 ? tc::launch_groups<__nv_bfloat16>(p, a, tiles, shared, st)
+                           : tc::launch_groups<__half>(p, a, tiles, shared, st);
 }
 
 }  // namespace kv4

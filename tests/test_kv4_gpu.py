@@ -67,7 +67,7 @@ def check_values(got, want64, dtype):
 
 
 def on_tensor_cores(dtype, t, group, d):
-    return dtype != torch.float32 and d in (64, 128) and t * group > 8
+    return dtype != torch.float32 and d <= 128 and t * group > 8
 
 
 def attention_bound(q, kx, vx, starts, dtype, tc):
@@ -348,6 +348,13 @@ def test_attention_of_long_and_many_requests(cuda, dtype, starts, t, h, group, d
     ([900, 0, 2500, 31], 20, 8, 1, 64),  # CTAs that end one segment and begin the next
     ([60 * i for i in range(10)], 130, 8, 4, 64),  # enough segments for one a CTA
     ([128], 257, 1, 1, 64),
+    ([40, 333], 70, 2, 1, 32),  # one group of channels, three, and short ones
+    ([1000], 3, 2, 5, 96),
+    ([100, 0, 511], 50, 3, 2, 80),
+    ([77], 140, 2, 1, 100),
+    ([12, 260], 33, 1, 3, 7),
+    ([5], 21, 2, 1, 33),
+    ([0], 10, 1, 1, 1),
 ])
 def test_attention_on_the_tensor_cores(cuda, dtype, starts, t, h, group, d):
     assert on_tensor_cores(dtype, t, group, d)
@@ -442,15 +449,17 @@ def test_calls_at_once_on_two_streams_and_graphs(cuda):
 
 def test_attention_of_strided_queries_into_out(cuda):
     """q as column views of a projection's output, aligned and not; out given."""
-    dtype, starts, h, d = torch.bfloat16, [90, 20], 3, 64
-    pool, slots, st, kx, vx = fill(cuda, dtype, starts, 1, h, d, seed=1)
-    for off in (0, 8, 3):
-        wide = torch.randn(2, 3 * h * d + off, generator=torch.Generator().manual_seed(off)).to(dtype)
-        q = wide[:, off:off + h * d].unflatten(1, (h, d)).unsqueeze(1)
-        qd = wide.to(cuda)[:, off:off + h * d].unflatten(1, (h, d)).unsqueeze(1)
-        out = torch.full((2, 1, h * d), math.nan, dtype=dtype, device=cuda)
+    dtype, starts, h = torch.bfloat16, [90, 20], 3
+    for off, t, d in ((0, 1, 64), (8, 1, 64), (3, 1, 64), (0, 12, 64), (8, 12, 80), (3, 12, 128), (0, 9, 36)):
+        pool, slots, st, kx, vx = fill(cuda, dtype, starts, t, h, d, seed=1)
+        wide = torch.randn(2 * t, 3 * h * d + off, generator=torch.Generator().manual_seed(off)).to(dtype)
+        q = wide[:, off:off + h * d].unflatten(1, (h, d)).unflatten(0, (2, t))
+        qd = wide.to(cuda)[:, off:off + h * d].unflatten(1, (h, d)).unflatten(0, (2, t))
+        memory = torch.full((2 * t * h * d + off,), math.nan, dtype=dtype, device=cuda)
+        out = memory[off:].view(2, t, h * d)
         assert ops.kv4_attention(qd, pool, slots, st, out=out) is out
         check_attention(out, q, kx, vx, starts, dtype)
+        assert memory[:off].isnan().all()
 
 
 def test_a_row_that_reads_nan_reaches_only_those_who_attend_it(cuda):
