@@ -1,6 +1,6 @@
 // Attention of several query rows over the 4-bit key/value cache on the tcgen05
 // tensor cores: a prompt's tokens, a few drafted ones, query heads that share a
-// key/value head (16-bit types, head dim up to 128).
+// key/value head (16-bit types).
 //
 // A segment is a request's key/value head with up to 128 of its query rows (row =
 // token * group + query head within the group: UMMA M, the TMEM lanes).  Its
@@ -49,20 +49,25 @@ constexpr int kThreads = 416;
 constexpr int kDequant = 8, kMma = 12;  // first warps of the roles
 // TMEM columns: two score blocks, the output, P and the queries (fp16 pairs).  P and
 // the queries as operands from TMEM halve what the products read of shared memory,
-// whose bandwidth the operands' writes and reads are bound by.
-constexpr uint32_t kTmemCols = 512, kTmemO = 2 * kBlock, kTmemP = 384, kTmemQ = 448;
+// whose bandwidth the operands' writes and reads are bound by.  Above 128 channels
+// there is room for one block of operands and of scores, and P takes the place of
+// the scores that it is made of: a block's softmax then waits for the block before.
+constexpr uint32_t kTmemCols = 512;
 
 template <int G>
 struct Smem {
   static constexpr int D = 32 * G, kSlabs = (G + 1) / 2;  // 128-byte slabs along the head dim
   static constexpr uint32_t kTileBytes = 2 * kTile * G * (16 + 4);
   static constexpr uint32_t kOperand = kRows * 128 * kSlabs;
-  static constexpr uint32_t k = 0, v = 2 * kOperand;
-  static constexpr uint32_t bars = 4 * kOperand;
+  static constexpr uint32_t stages = G > 4 ? 1 : 2;
+  static constexpr uint32_t tm_o = stages * kBlock, tm_p = G > 4 ? 0 : 384, tm_q = G > 4 ? 384 : 448;
+  static_assert(tm_o + D <= (G > 4 ? tm_q : tm_p) && tm_q + D / 2 <= kTmemCols, "TMEM");
+  static constexpr uint32_t k = 0, v = stages * kOperand;
+  static constexpr uint32_t bars = 2 * stages * kOperand;
   static constexpr uint32_t rows = bars + 512;  // what a row's two threads tell each other: [2][2][128] fp32
   static constexpr uint32_t factors = rows + 2048;  // powers of two of the tiles' keys and values: [4 blocks][2][4]
-  static constexpr uint32_t nans = factors + 128;   // first position whose value is NaN: [4 parts][4 tiles][4 groups]
-  static constexpr uint32_t total = nans + 256 + 1024;  // 1024: alignment of the base
+  static constexpr uint32_t nans = factors + 128;   // first position whose value is NaN: [4 parts][4 tiles][8 groups]
+  static constexpr uint32_t total = nans + 512 + 1024;  // 1024: alignment of the base
   static_assert(total <= 227 * 1024, "shared memory");
 };
 enum Bar : int {
@@ -235,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using L = Smem<G>;
   constexpr int D = L::D;  // channels of whole groups; the row has p.D of them
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  static_assert(G >= 1 && G <= 4, "TMEM columns of O and Q");
+  constexpr unsigned NS = L::stages;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const mem = smem_raw + (base - smem_u32(smem_raw));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -322,16 +327,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       return live;
     };
     auto scores = [&](unsigned n) {
-      if (!await(kKFull + (n & 1), (n >> 1) & 1)) return;
+      if (!await(kKFull + n % NS, (n / NS) & 1)) return;
       tc_fence_after();
       if (leader) {
-        const uint64_t dk = dk0 + (n & 1) * (L::kOperand >> 4);
-        const uint32_t to = tmem + (n & 1) * kBlock;
+        const uint64_t dk = dk0 + (n % NS) * (L::kOperand >> 4);
+        const uint32_t to = tmem + (n % NS) * kBlock;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          umma_f16_ts(to, tmem + kTmemQ + k * 8, dk + (uint32_t)(((k / 4) * kBlock * 128 + (k % 4) * 32) >> 4), id_s, k != 0);
-        umma_commit(bar(kSFull + (n & 1)));
-        umma_commit(bar(kKEmpty + (n & 1)));
+          umma_f16_ts(to, tmem + L::tm_q + k * 8, dk + (uint32_t)(((k / 4) * kBlock * 128 + (k % 4) * 32) >> 4), id_s, k != 0);
+        umma_commit(bar(kSFull + n % NS));
+        umma_commit(bar(kKEmpty + n % NS));
       }
       __syncwarp();
       s_issued = n + 1;
@@ -343,23 +348,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++parts;
       scores(blk);
       for (int j = 0; j < nb && live; ++j, ++blk) {
-        if (j + 1 < nb) scores(blk + 1);
-        if (!await(kVFull + (blk & 1), (blk >> 1) & 1) || !await(kPFull, blk & 1)) break;
+        if (NS == 2 && j + 1 < nb) scores(blk + 1);
+        if (!await(kVFull + blk % NS, (blk / NS) & 1) || !await(kPFull, blk & 1)) break;
         tc_fence_after();
         if (leader) {
-          const uint64_t dv = dv0 + (blk & 1) * (L::kOperand >> 4);
+          const uint64_t dv = dv0 + (blk % NS) * (L::kOperand >> 4);
 #pragma unroll
           for (int k = 0; k < kBlock / 16; ++k)
-            umma_f16_ts(tmem + kTmemO, tmem + kTmemP + k * 8, dv + (uint32_t)((k * 16 * 128) >> 4), id_o, (j | k) != 0);
+            umma_f16_ts(tmem + L::tm_o, tmem + L::tm_p + k * 8, dv + (uint32_t)((k * 16 * 128) >> 4), id_o, (j | k) != 0);
           umma_commit(bar(kOFull));
-          umma_commit(bar(kVEmpty + (blk & 1)));
+          umma_commit(bar(kVEmpty + blk % NS));
         }
         __syncwarp();
         o_issued = blk + 1;
+        if (NS == 1 && j + 1 < nb) {  // the next scores go where P is
+          if (!await(kOFull, blk & 1)) break;
+          scores(blk + 1);
+        }
       }
     }
     // every UMMA issued completes before TMEM is released
-    if (s_issued > 0) mbar_wait(bar(kSFull + ((s_issued - 1) & 1)), ((s_issued - 1) >> 1) & 1, DEV_ERR_ATTN_TIMEOUT);
+    if (s_issued > 0) mbar_wait(bar(kSFull + (s_issued - 1) % NS), ((s_issued - 1) / NS) & 1, DEV_ERR_ATTN_TIMEOUT);
     if (o_issued > 0) mbar_wait(bar(kOFull), (o_issued - 1) & 1, DEV_ERR_ATTN_TIMEOUT);
     __syncwarp();
   } else if (warp >= kDequant) {
@@ -427,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
-          if (blk >= 2) live = wait_copies(bar((kv ? kVEmpty : kKEmpty) + (blk & 1)), ((blk >> 1) - 1) & 1);
+          if (blk >= NS) live = wait_copies(bar((kv ? kVEmpty : kKEmpty) + blk % NS), (blk / NS - 1) & 1);
           if (!__all_sync(0xffffffffu, live)) {
             live = false;
             break;
@@ -438,8 +447,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (kv == 0 && lane < 2) factors[(blk & 3) * 8 + 4 * lane + dw] = mine;
           // likewise four parts': S of a part's first block is issued after the softmax's
           // warps have read all of the part before
-          if (kv == 0 && lane < G) nans[(parts & 3) * 16 + 4 * dw + lane] = nan;
-          const uint32_t dst = base + (kv ? L::v : L::k) + (blk & 1) * L::kOperand + out_row;
+          if (kv == 0 && lane < G) nans[(parts & 3) * 32 + 8 * dw + lane] = nan;
+          const uint32_t dst = base + (kv ? L::v : L::k) + (blk % NS) * L::kOperand + out_row;
           // eight channels, number o8 of the row
           auto put = [&](int o8, uint32_t x, uint32_t sz8) {
             sts4(dst + (o8 / 8) * (kBlock * 128) + (((o8 & 7) ^ (row & 7)) * 16), operand8(x, sz8));
@@ -470,18 +479,23 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int i = 0; i < 4 * G; ++i) {
                 const int quarter = i / G, group = i % G;
                 uint32_t x = w[i];
-                if (kv) {  // half words of channels 8 q .. and 8 q + 4 ..
+                if (kv && G < 8) {  // half words of channels 8 q .. and 8 q + 4 ..
                   const int h0 = 2 * quarter * G + group, h1 = h0 + G;
                   x = __byte_perm(w[h0 / 2], w[h1 / 2], (h0 % 2 ? 0x32 : 0x10) | (h1 % 2 ? 0x7600 : 0x5400));
                 }
-                put(4 * group + quarter, x, sz[kv][group]);
+                int o8 = 4 * group + quarter;
+                if (kv && G == 8) {  // turned by position: a pair of 16-byte chunks is another quarter's
+                  x = __byte_perm(w[8 * quarter + group / 2], w[8 * quarter + 4 + group / 2], group % 2 ? 0x7632 : 0x5410);
+                  o8 = 4 * group + (quarter ^ (lane & 3));
+                }
+                put(o8, x, sz[kv][group]);
               }
             }
           }
           load(kv, j + 1);
           fence_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar((kv ? kVFull : kKFull) + (blk & 1)));
+          if (lane == 0) mbar_arrive(bar((kv ? kVFull : kKFull) + blk % NS));
         }
       }
       if (part.lo < part.hi) ++parts;
@@ -584,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             x[4 * i + 2] = __byte_perm(w[c + i].y, w[c + i].w, 0x5410);
             x[4 * i + 3] = __byte_perm(w[c + i].y, w[c + i].w, 0x7632);
           }
-          tmem_st16(trow + kTmemQ + 16 * group0 + 4 * c, x);
+          tmem_st16(trow + L::tm_q + 16 * group0 + 4 * c, x);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -595,13 +609,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       float unit = __int_as_float(253 << 23);
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < nb && live; ++j, ++blk) {
-        live = wait_copies(bar(kSFull + (blk & 1)), (blk >> 1) & 1);
+        live = wait_copies(bar(kSFull + blk % NS), (blk / NS) & 1);
         if (!__all_sync(0xffffffffu, live)) {
           live = false;
           break;
         }
         tc_fence_after();
-        const uint32_t ts = trow + (blk & 1) * kBlock, to = trow + kTmemO;
+        const uint32_t ts = trow + (blk % NS) * kBlock, to = trow + L::tm_o;
         const int lim = row_keys - (part.lo + j) * kBlock;  // positions of the block that the row attends
         const bool full = __all_sync(0xffffffffu, lim >= kBlock || !mine);
         const bool any = __any_sync(0xffffffffu, lim > 0);
@@ -627,8 +641,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * k_scale[c]);
           }
+          if (NS == 1) tc_fence_before();  // the other thread's P goes over these scores
           mx = fmaxf(mx, exchange(mx));
           if (!live) break;
+          if (NS == 1) tc_fence_after();
           const float mn = fmaxf(m, mx);
           alpha = m == -INFINITY ? 0.f : ex2(m - mn);
           m = mn;
@@ -679,14 +695,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 lp[e & 3] += p0 + p1;
               }
             }
-            tmem_st16(trow + kTmemP + 32 * hx + 16 * c, w);
+            tmem_st16(trow + L::tm_p + 32 * hx + 16 * c, w);
           }
           tmem_st_wait();
           l += (lp[0] + lp[1]) + (lp[2] + lp[3]);
         } else if (used) {  // all masked: weights of zero
           const uint32_t w[16] = {};
-          tmem_st16(trow + kTmemP + 32 * hx, w);
-          tmem_st16(trow + kTmemP + 32 * hx + 16, w);
+          tmem_st16(trow + L::tm_p + 32 * hx, w);
+          tmem_st16(trow + L::tm_p + 32 * hx + 16, w);
           tmem_st_wait();
         }
         tc_fence_before();
@@ -703,9 +719,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!live) break;
       const float off_unit = std::is_same<T, __half>::value ? 1.f : __fdividef(1.0f, unit);
       // whether the row attends a value of NaN in the channels of group c
-      const int* const nans = reinterpret_cast<const int*>(mem + L::nans) + (parts & 3) * 16;
+      const int* const nans = reinterpret_cast<const int*>(mem + L::nans) + (parts & 3) * 32;
       auto nan_in = [&](int c) {
-        return nb > 0 && min(min(nans[c], nans[4 + c]), min(nans[8 + c], nans[12 + c])) < row_keys;
+        return nb > 0 && min(min(nans[c], nans[8 + c]), min(nans[16 + c], nans[24 + c])) < row_keys;
       };
       if (nb > 0) ++parts;
       T* const op = static_cast<T*>(a.out) + (((long long)part.b * a.tq + tok) * a.QH + qh) * p.D;
@@ -732,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (int c = group0; c < group1; ++c) {
             float v[32];
-            tmem_ld32(trow + kTmemO + c * 32, v);
+            tmem_ld32(trow + L::tm_o + c * 32, v);
             if (mine) store(c, v, nan_in(c) ? NAN : inv);
           }
         }
@@ -745,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int c = group0; c < group1; ++c) {
           float v[32];
-          if (nb > 0) tmem_ld32(trow + kTmemO + c * 32, v);
+          if (nb > 0) tmem_ld32(trow + L::tm_o + c * 32, v);
           const float f = nan_in(c) ? NAN : off_unit;
           if (mine && nb > 0)
 #pragma unroll
@@ -830,7 +846,11 @@ static int launch_groups(const Pool& p, const Problem& a, int row_tiles, bool sh
     case 1: return launch<T, 1>(p, a, row_tiles, shared, st);
     case 2: return launch<T, 2>(p, a, row_tiles, shared, st);
     case 3: return launch<T, 3>(p, a, row_tiles, shared, st);
-    default: return launch<T, 4>(p, a, row_tiles, shared, st);
+    case 4: return launch<T, 4>(p, a, row_tiles, shared, st);
+    case 5: return launch<T, 5>(p, a, row_tiles, shared, st);
+    case 6: return launch<T, 6>(p, a, row_tiles, shared, st);
+    case 7: return launch<T, 7>(p, a, row_tiles, shared, st);
+    default: return launch<T, 8>(p, a, row_tiles, shared, st);
   }
 }
 
@@ -844,7 +864,7 @@ static int launch_groups(const Pool& p, const Problem& a, int row_tiles, bool sh
 //    2 requests x 8 heads x 6000             16 / 20 /  31 /  44 against  47 ..  51 us
 //    4 requests x 8 heads x 300               8 /  8 /  10 /  12 against  23 ..  24 us
 bool tc_covers(const Pool& p, int dtype, int64_t t, int64_t group) {
-  return (dtype == FML_BF16 || dtype == FML_F16) && p.G <= 4 && t * group > 8;
+  return (dtype == FML_BF16 || dtype == FML_F16) && t * group > 8;
 }
 static bool tc_shared(const Pool& p, int64_t segments, int64_t requests_units) {
   return segments < 2 * num_sms(current_device()) && requests_units < (1ll << 31);

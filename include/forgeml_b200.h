@@ -275,7 +275,7 @@ FML_API int neb_kv4_read(const neb_kv4_pool* pool, const int32_t* slot_of, const
  * element strides, innermost 1), q_heads a multiple of the pool's heads: query
  * head h reads head h / (q_heads / heads).  out is [B,T,q_heads*D] contiguous.
  * scale is positive and finite.  Scores, softmax and the sums over the rows in
- * fp32; more than 8 query rows of a head (16-bit types, D up to 128) run on the
+ * fp32; more than 8 query rows of a head (16-bit types) run on the
  * tensor cores with keys, values and weights rounded to fp16.  Queries without
  * a place in the pool give zeros and raise bit 4.  Rows past a query's position
  * count nothing, whatever they hold. */

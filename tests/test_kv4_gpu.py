@@ -66,8 +66,8 @@ def check_values(got, want64, dtype):
     assert not bad.any(), (got[bad][:4], want64[bad][:4])
 
 
-def on_tensor_cores(dtype, t, group, d):
-    return dtype != torch.float32 and d <= 128 and t * group > 8
+def on_tensor_cores(dtype, t, group):
+    return dtype != torch.float32 and t * group > 8
 
 
 def attention_bound(q, kx, vx, starts, dtype, tc):
@@ -154,7 +154,7 @@ def attention_bound(q, kx, vx, starts, dtype, tc):
 def check_attention(got, q, kx, vx, starts, dtype, t=None):
     """t: the call's tokens, where q holds only its first ones."""
     want = orc.attention(q, kx, vx, starts)
-    tc = on_tensor_cores(dtype, t or q.shape[1], q.shape[2] // kx.shape[2], q.shape[3])
+    tc = on_tensor_cores(dtype, t or q.shape[1], q.shape[2] // kx.shape[2])
     bound = attention_bound(q, kx, vx, starts, dtype, tc)
     f = torch.finfo(dtype)
     tol = bound * (1 + f.eps) + f.eps / 2 * want.nan_to_num(0.0).abs() + f.tiny * f.eps / 2
@@ -355,15 +355,20 @@ def test_attention_of_long_and_many_requests(cuda, dtype, starts, t, h, group, d
     ([12, 260], 33, 1, 3, 7),
     ([5], 21, 2, 1, 33),
     ([0], 10, 1, 1, 1),
+    ([300, 70], 40, 1, 1, 160),  # one block of operands and scores at a time
+    ([128, 1000], 20, 2, 2, 192),
+    ([63], 150, 1, 1, 224),
+    ([1500, 2, 640], 130, 2, 1, 256),
+    ([200], 4, 1, 3, 250),
 ])
 def test_attention_on_the_tensor_cores(cuda, dtype, starts, t, h, group, d):
-    assert on_tensor_cores(dtype, t, group, d)
+    assert on_tensor_cores(dtype, t, group)
     pool, slots, st, kx, vx = fill(cuda, dtype, starts, t, h, d, seed=d + t + 2)
     q = torch.randn(len(starts), t, h * group, d, generator=torch.Generator().manual_seed(d)).to(dtype)
     check_attention(ops.kv4_attention(q.to(cuda), pool, slots, st), q, kx, vx, starts, dtype)
 
 
-@pytest.mark.parametrize("t,d", [(1, 128), (5, 96), (40, 128), (150, 64)])
+@pytest.mark.parametrize("t,d", [(1, 128), (5, 96), (40, 128), (150, 64), (30, 256)])
 @pytest.mark.parametrize("qp,kp,vp", [(60, -60, -80), (-70, 70, 100), (0, 0, 0)])
 def test_bf16_magnitudes(cuda, t, d, qp, kp, vp):
     """bf16's range: queries, keys and values far from 1, tiles of different
@@ -386,7 +391,8 @@ def test_bf16_magnitudes(cuda, t, d, qp, kp, vp):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("t,group,d", [(1, 1, 128), (6, 1, 64), (40, 1, 128), (100, 2, 64), (3, 3, 80)])
+@pytest.mark.parametrize("t,group,d", [(1, 1, 128), (6, 1, 64), (40, 1, 128), (100, 2, 64), (3, 3, 80),
+                                       (50, 1, 192)])
 def test_nan_in_values_reaches_its_group_of_those_who_attend_it(cuda, dtype, t, group, d):
     """A value of NaN or infinity in one group's channels, a key of NaN further on:
     earlier rows' weights of zero undo both."""
