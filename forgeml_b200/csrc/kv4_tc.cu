@@ -4,7 +4,7 @@
 //
 // A segment is a request's key/value head with up to 128 of its query rows (row =
 // token * group + query head within the group: UMMA M, the TMEM lanes).  Its
-// positions go by in blocks of 128, flash-attention schedule, warp-specialised:
+// positions go by in blocks of 128, a running maximum and sum, warp-specialised:
 //
 //   warps 8-11  turn the cache's codes into fp16 operands: a lane takes a position's
 //               key and value, loaded a block ahead, and writes z + c s, rounded once,
@@ -863,6 +863,11 @@ static int launch_groups(const Pool& p, const Problem& a, int row_tiles, bool sh
 //   16 requests x 8 heads x 6000 positions   47 / 77 / 139 / 262 against 117 .. 120 us
 //    2 requests x 8 heads x 6000             16 / 20 /  31 /  44 against  47 ..  51 us
 //    4 requests x 8 heads x 300               8 /  8 /  10 /  12 against  23 ..  24 us
+// and at 4 / 8 rows against 9 .. 32 rows here, other head dims, 16 requests x 8 heads:
+//   32 x 6000 positions  44 /  74 against  90 ..  93 us
+//   96 x 6000            66 / 115 against 104 .. 110
+//   256 x 3000           81 / 145 against 178 .. 184
+// (The lengths, which decide where exactly the two meet, lie on the device.)
 bool tc_covers(const Pool& p, int dtype, int64_t t, int64_t group) {
   return (dtype == FML_BF16 || dtype == FML_F16) && t * group > 8;
 }
