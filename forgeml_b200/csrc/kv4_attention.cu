@@ -617,14 +617,14 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
           for (int gi = 0; gi < G; ++gi) zacc[gi] *= alpha;
         }
         since = 0;
-        if (over) {
 #pragma unroll
-          for (int gi = 0; gi < G; ++gi) {
-            // a quarter of headroom, so that it moves seldom
-            const float big = 1.25f * warp_max(pr * step[gi]);
-            to_int[gi] = fminf(to_int[gi], __fdividef(kPMax, fmaxf(big, 1e-32f)));
-            n[gi] = fmaf(pr * step[gi], to_int[gi], 8388608.f);
-          }
+        for (int gi = 0; gi < G; ++gi) {
+          // What went before counts alpha times as much now, for the bound too: a large
+          // step whose weight vanishes must not leave the later weights without digits.
+          // A quarter of headroom, so that it falls seldom.
+          const float big = 1.25f * warp_max(pr * step[gi]);
+          to_int[gi] = fminf(__fdividef(to_int[gi], alpha), __fdividef(kPMax, fmaxf(big, 1e-32f)));
+          n[gi] = fmaf(pr * step[gi], to_int[gi], 8388608.f);
         }
       }
       ++since;

@@ -1,0 +1,161 @@
+"""The 4-bit key/value cache where numbers of very different sizes meet: a row's
+result depends on the positions that it attends, each by its weight, and on
+nothing else.  Bounds are taken over the attended rows only (``attended_bound``);
+the definition is oracle/kv4.py in float64."""
+
+import math
+
+import pytest
+import torch
+
+from forgeml_b200 import _native
+from forgeml_b200.nebula import KV4Pool, ops
+from oracle import kv4 as orc
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+LEVELS = {torch.bfloat16: 65530, torch.float16: 8388600, torch.float32: 8388600}
+
+
+@pytest.fixture(autouse=True)
+def clean_status(cuda):
+    _native.device_status()
+    yield
+    assert _native.device_status() == 0
+
+
+def table(values, cuda):
+    return torch.tensor(values, dtype=torch.int32, device=cuda)
+
+
+def filled(cuda, k, v, slots=1):
+    """A pool whose slot 0 holds k and v [1, n, H, D], and those rows in float64."""
+    _, n, h, d = k.shape
+    pool = KV4Pool(slots=slots, heads=h, max_seq_len=n, head_dim=d, device=cuda, dtype=k.dtype)
+    pool.data.fill_(255)
+    ops.kv4_append(k.to(cuda), v.to(cuda), pool, table([0], cuda), table([0], cuda))
+    return pool, orc.stands_for(k), orc.stands_for(v)
+
+
+def attended_bound(q, kx, vx, starts, dtype, tc):
+    """float64 [B, T, QH * D]: what a kernel may be off by before the output's
+    rounding, from the rows that a query attends.  e = 2^-24, w the weights, A =
+    sum w |v| of an output, n the attended positions.  Weights whose scores are off
+    by x are off by expm1(x) of themselves against their sum.
+
+    Up to 8 rows of a head, or fp32 (a group of 32 channels is z + c s, its span
+    15 s; a = |z| + 15 s, for fp32 |z + 8 s| + 8 s):
+      scores    q as an integer q / max|q| * 1.2e8, rounded to fp32, then to the
+                integer; put together in fp32, (G + 8) e of scale * sum |q| a (in
+                float64 for fp32).  The exponent: e times the distance from the
+                maximum.
+      weights   exponential 2^-22, and once more each time that the maximum moves.
+      digits    w s goes as an integer of units of at most 1.25 max (w s) / levels, half
+                a unit off at the most: times 15 (the code) and n.
+      sums      4 (n / 32 + 40) e of sum w a.
+    On the tensor cores, u = 2^-11 the rounding to fp16.  bf16's operands are scaled
+    by powers of two to 2^12 at least for the largest number of a position or, where
+    32 neighbouring positions differ by less than 2^10, of those; the largest weight
+    times value of a row to 2^13 at least, or 2^3 where neighbours differ; M the
+    largest |number| of a position.
+      scores    u of every |q k|, the products' sums (d + 8) 2^-23, and the subnormal
+                step: 2^-25 (fp16), 2^-37 of the largest |q|, 2^-26 of M for the keys;
+                the exponent as above.
+      weights   2^-22 each and per move; weights and values rounded, 2 u A; the
+                subnormal steps: of a value 2^-25 (fp16) or 2^-26 M, of a weight 2^-26
+                of the row's largest w M; sums (n / 16 + 40) 2^-23 A."""
+    b, t, qh, d = q.shape
+    q = q.detach().cpu().double()
+    h, u, e = kx.shape[2], 2.0 ** -11, 2.0 ** -24
+    group, scale, wide = qh // h, 1 / math.sqrt(d), dtype == torch.float32
+    bound = torch.empty(b, t, qh, d, dtype=torch.float64)
+
+    def spans(x, wide):
+        a, st = torch.empty_like(x), torch.empty_like(x)
+        for c0 in range(0, d, 32):
+            g = x[..., c0:c0 + 32]
+            z, s15 = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True) - g.amin(-1, keepdim=True)
+            a[..., c0:c0 + 32] = ((z + s15 * 8 / 15).abs() + s15 * 8 / 15) if wide else z.abs() + s15
+            st[..., c0:c0 + 32] = s15 / 15
+        return a, st
+
+    ka, _ = spans(kx, False)
+    va, vs = spans(vx, wide)
+    for i in range(b):
+        for j in range(t):
+            n = int(starts[i]) + j + 1
+            moves = n / 32 + 1
+            for hq in range(qh):
+                hk = hq // group
+                kh, vh, qi = kx[i, :n, hk], vx[i, :n, hk], q[i, j, hq]
+                sc = kh @ qi * scale
+                w = torch.softmax(sc, 0)
+                A = w @ vh.abs()
+                far = sc.max() - sc
+                if tc:
+                    km, vm = kh.abs().amax(1), vh.abs().amax(1)
+                    x = (u + (d + 8) * 2 * e) * (kh.abs() @ qi.abs()) * scale + 2 * e * (far + sc.abs())
+                    if dtype == torch.float16:
+                        x = x + 2.0 ** -25 * (qi.abs().sum() + kh.abs().sum(1)) * scale
+                        step = 2.0 ** -25
+                    else:
+                        x = x + (2.0 ** -26 * qi.abs().sum() * km + 2.0 ** -37 * qi.abs().max() * kh.abs().sum(1)) * scale
+                        step = 2.0 ** -26 * (w @ vm)
+                    rel = moves / 4 * 2.0 ** -22 + 2.0 ** -22 + x
+                    other = 2 * u * A + step + n * 2.0 ** -26 * (w * vm).max() + (n / 16 + 40) * 2 * e * A
+                else:
+                    small = ka[i, :n, hk] @ qi.abs() * scale
+                    x = e * small + 0.6 / 1.2e8 * qi.abs().max() * scale * ka[i, :n, hk].sum(1) + e * far
+                    x = x + (0 if wide else (-(-d // 32) + 8) * e * small)
+                    rel = x + moves * 2.0 ** -22
+                    unit = 1.25 * (w[:, None] * vs[i, :n, hk]).amax(0) / LEVELS[dtype]
+                    other = 15 * unit * n + 4 * (n / 32 + 40) * e * (w @ va[i, :n, hk])
+                off = w * torch.expm1(rel)
+                bound[i, j, hq] = off @ vh.abs() + off.sum() * A + other
+    return bound.reshape(b, t, qh * d)
+
+
+def check(got, q, kx, vx, starts, dtype, tc, rows=None):
+    """rows: how many of the call's query rows are looked at (all)."""
+    b = q.shape[0]
+    kx, vx = (x.expand(b, -1, -1, -1) for x in (kx, vx))
+    rows = q.shape[1] if rows is None else rows
+    q, got = q[:, :rows], got[:, :rows].cpu().double()
+    n = max(starts) + rows
+    want = orc.attention(q, kx[:, :n], vx[:, :n], starts)
+    f = torch.finfo(dtype)
+    tol = attended_bound(q, kx[:, :n], vx[:, :n], starts, dtype, tc) * (1 + f.eps)
+    tol = tol + f.eps / 2 * want.abs() + f.tiny * f.eps / 2
+    assert want.isfinite().all() and tol.isfinite().all()
+    err = (got - want).abs()
+    assert (err <= tol).all(), (float(err.max()), float((err / tol).max()), float(want.abs().max()))
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+MANY = 128  # requests of 16 heads, all reading the same slot: more segments than the chip has warps
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("power", [7, 10, 14, 26])
+def test_a_large_value_of_vanishing_weight_among_later_rows(cuda, dtype, power):
+    """Position 5's value is 2^power times the others', the first 32 positions score
+    far below the later ones.  One warp holds whole segments of 1024 positions."""
+    n, h, d = 1024, 16, 32
+    if dtype == torch.float16:
+        power = min(power, 12)
+    dirn = torch.where(torch.rand(h, d, generator=gen(1)) < 0.5, -1.0, 1.0)
+    k = 0.3 * torch.randn(1, n, h, d, generator=gen(2))
+    gap = 10 + power  # nats
+    k[:, :32] -= gap / math.sqrt(d) * dirn
+    v = torch.randn(1, n, h, d, generator=gen(3))
+    v[:, 5] *= 2.0 ** power
+    k, v = k.to(dtype), v.to(dtype)
+    q = (dirn + 0.1 * torch.randn(MANY, 1, h, d, generator=gen(4))).to(dtype)
+    pool, kx, vx = filled(cuda, k, v)
+    got = ops.kv4_attention(q.to(cuda), pool, table([0] * MANY, cuda), table([n - 1] * MANY, cuda))
+    check(got[:2], q[:2], kx, vx, [n - 1] * 2, dtype, False)
+    check(got[-2:], q[-2:], kx, vx, [n - 1] * 2, dtype, False)
