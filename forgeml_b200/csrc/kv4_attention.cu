@@ -26,8 +26,11 @@
 // What is rounded: q to 27 bits below its largest channel (four 8-bit digits;
 // the 16-bit types and all but the smallest channels of fp32 are exact), the
 // weights p s to 16 bits below their running bound (two digits; three, 23
-// bits, for fp16 and fp32, whose outputs keep more bits than bf16's).  Scores,
-// maxima, sums and outputs are fp32.  An fp32 cache's scores, whose errors the
+// bits, for fp16 and fp32, whose outputs keep more bits than bf16's).  What a lane
+// rounds off it adds to the weight of its next position: of many weights below a
+// whole step none would count otherwise, beside a large one, while the sum of
+// weights and the minima's share count them all.  Scores, maxima, sums and outputs
+// are fp32.  An fp32 cache's scores, whose errors the
 // exponentials pass on whole, are put together from the integers in 64 bits, and
 // its values' codes count from 8: p (z + 8 s) + p s (c - 8) keeps the bits that
 // p z + p s c, two sums of a group's whole range that all but cancel, loses.
@@ -396,7 +399,7 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
   int accm[G][4], accr[G][4];                                // sums of P lo and of P (lo + 16 hi)
   int accm3[PP == 3 ? G : 1][4], accr3[PP == 3 ? G : 1][4];  // third digits
   int ones[kWide ? SETS : 1][4], ones3[kWide ? SETS : 1][4];  // sums of P: the codes count from 8 then
-  float zacc[G], to_int[G], m = -INFINITY, l = 0.f;
+  float zacc[G], to_int[G], carry[G], m = -INFINITY, l = 0.f;
   float* const o = reinterpret_cast<float*>(mem + U::out) + lane;  // channel 32 gi + 4 g + i: o[(4 gi + i) * 32]
   int stage = 0, since = 0;
   uint32_t parity = 0;
@@ -531,6 +534,7 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
       }
       zacc[gi] = 0.f;
       to_int[gi] = kToInt0;
+      carry[gi] = 0.5f;
     }
     if constexpr (kWide) {
 #pragma unroll
@@ -580,30 +584,31 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
       const bool part = nk < kUnit, valid = my_pos < nk;
       float step[G], low[G];
       lds_params<T, G>(st + U::kp + my_pos * U::PR, part, valid, step, low);
-      Score x = 0, y = 0;
+      Score codes = 0, lows = 0;
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) {
         const float* d = dots + (gi / 4) * 8 * 36 + (gi & 3) * 36 + lane;
         if constexpr (kWide) {
           const int* e = reinterpret_cast<const int*>(d);
-          x = fma((double)step[gi], fma((double)e[0], 65536.0, (double)e[4 * 36]), x);
-          y = fma((double)low[gi], qsum[gi], y);
+          codes = fma((double)step[gi], fma((double)e[0], 65536.0, (double)e[4 * 36]), codes);
+          lows = fma((double)low[gi], qsum[gi], lows);
         } else {
-          x = fmaf(step[gi], fmaf(d[0], 65536.f, d[4 * 36]), x);
-          y = fmaf(low[gi], qsum[gi], y);
+          codes = fmaf(step[gi], fmaf(d[0], 65536.f, d[4 * 36]), codes);
+          lows = fmaf(low[gi], qsum[gi], lows);
         }
       }
-      const Score sc = valid ? x * unit_q + y : (Score)-INFINITY;
+      const Score sc = valid ? codes * unit_q + lows : (Score)-INFINITY;
       const float mx = warp_max((float)sc);
       lds_params<T, G>(st + U::vp + my_pos * U::PR, part, valid, step, low);
       // ---- weights, as integers up to kPMax
       const float mn = fmaxf(m, mx);
       const float pr = valid ? ex2((float)(sc - mn)) : 0.f;
-      float n[G];
+      float x[G], n[G];
       bool over = false;
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) {
-        n[gi] = fmaf(pr * step[gi], to_int[gi], 8388608.f);
+        x[gi] = fmaf(pr * step[gi], to_int[gi], carry[gi]);
+        n[gi] = __fadd_rz(x[gi], 8388608.f);
         over |= n[gi] > 8388608.f + kPMax;
       }
       over = __any_sync(0xffffffffu, over);
@@ -624,11 +629,14 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
           // A quarter of headroom, so that it falls seldom.
           const float big = 1.25f * warp_max(pr * step[gi]);
           to_int[gi] = fminf(__fdividef(to_int[gi], alpha), __fdividef(kPMax, fmaxf(big, 1e-32f)));
-          n[gi] = fmaf(pr * step[gi], to_int[gi], 8388608.f);
+          x[gi] = fmaf(pr * step[gi], to_int[gi], 0.5f);
+          n[gi] = __fadd_rz(x[gi], 8388608.f);
         }
       }
       ++since;
       l += pr;
+#pragma unroll  // (cut off, from half a step on: 0 <= carry < 1)
+      for (int gi = 0; gi < G; ++gi) carry[gi] = x[gi] - (n[gi] - 8388608.f);
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) zacc[gi] = fmaf(pr, kWide ? fmaf(8.f, step[gi], low[gi]) : low[gi], zacc[gi]);
 #pragma unroll

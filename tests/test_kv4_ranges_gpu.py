@@ -38,7 +38,7 @@ def filled(cuda, k, v, slots=1):
     return pool, orc.stands_for(k), orc.stands_for(v)
 
 
-def attended_bound(q, kx, vx, starts, dtype, tc):
+def attended_bound(q, kx, vx, starts, dtype, tc, terms=None):
     """float64 [B, T, QH * D]: what a kernel may be off by before the output's
     rounding, from the rows that a query attends.  e = 2^-24, w the weights, A =
     sum w |v| of an output, n the attended positions.  Weights whose scores are off
@@ -51,8 +51,12 @@ def attended_bound(q, kx, vx, starts, dtype, tc):
                 float64 for fp32).  The exponent: e times the distance from the
                 maximum.
       weights   exponential 2^-22, and once more each time that the maximum moves.
-      digits    w s goes as an integer of units of at most 1.25 max (w s) / levels, half
-                a unit off at the most: times 15 (the code) and n.
+      digits    w s goes as an integer of units of at most 1.25 max (w s) / levels,
+                and what a lane rounds off is carried to its next position: the
+                rounding of a position is off by r_j = e_(j-1) - e_j, |e| at most one
+                unit, and sum r_j c_j = sum e_j (c_(j+1) - c_j) is at most a unit times
+                15 for each of the ``terms`` positions where the lane's next code is
+                another (n of them unless the caller knows better).
       sums      4 (n / 32 + 40) e of sum w a.
     On the tensor cores, u = 2^-11 the rounding to fp16.  bf16's operands are scaled
     by powers of two to 2^12 at least for the largest number of a position or, where
@@ -110,13 +114,13 @@ def attended_bound(q, kx, vx, starts, dtype, tc):
                     x = x + (0 if wide else (-(-d // 32) + 8) * e * small)
                     rel = x + moves * 2.0 ** -22
                     unit = 1.25 * (w[:, None] * vs[i, :n, hk]).amax(0) / LEVELS[dtype]
-                    other = 15 * unit * n + 4 * (n / 32 + 40) * e * (w @ va[i, :n, hk])
+                    other = 15 * unit * (n if terms is None else min(n, terms)) + 4 * (n / 32 + 40) * e * (w @ va[i, :n, hk])
                 off = w * torch.expm1(rel)
                 bound[i, j, hq] = off @ vh.abs() + off.sum() * A + other
     return bound.reshape(b, t, qh * d)
 
 
-def check(got, q, kx, vx, starts, dtype, tc, rows=None):
+def check(got, q, kx, vx, starts, dtype, tc, terms=None, rows=None):
     """rows: how many of the call's query rows are looked at (all)."""
     b = q.shape[0]
     kx, vx = (x.expand(b, -1, -1, -1) for x in (kx, vx))
@@ -125,7 +129,7 @@ def check(got, q, kx, vx, starts, dtype, tc, rows=None):
     n = max(starts) + rows
     want = orc.attention(q, kx[:, :n], vx[:, :n], starts)
     f = torch.finfo(dtype)
-    tol = attended_bound(q, kx[:, :n], vx[:, :n], starts, dtype, tc) * (1 + f.eps)
+    tol = attended_bound(q, kx[:, :n], vx[:, :n], starts, dtype, tc, terms) * (1 + f.eps)
     tol = tol + f.eps / 2 * want.abs() + f.tiny * f.eps / 2
     assert want.isfinite().all() and tol.isfinite().all()
     err = (got - want).abs()
@@ -159,3 +163,25 @@ def test_a_large_value_of_vanishing_weight_among_later_rows(cuda, dtype, power):
     got = ops.kv4_attention(q.to(cuda), pool, table([0] * MANY, cuda), table([n - 1] * MANY, cuda))
     check(got[:2], q[:2], kx, vx, [n - 1] * 2, dtype, False)
     check(got[-2:], q[-2:], kx, vx, [n - 1] * 2, dtype, False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_small_weights_beside_a_large_one(cuda, dtype):
+    """One position takes nearly all the weight, with channels of zero; each of the
+    8191 others has a weight of a fraction of the integers' unit.  Together they are
+    what those channels hold."""
+    n, h, d = 8192, 16, 32
+    dirn = torch.where(torch.rand(h, d, generator=gen(1)) < 0.5, -1.0, 1.0)
+    small = 0.3 * 1.25 / LEVELS[dtype]
+    half = -math.log(small) / 2 / math.sqrt(d)
+    k = (-half * dirn).expand(1, n, h, d).clone()
+    k[:, 0] = half * dirn
+    v = torch.randn(h, d, generator=gen(3)).abs().expand(1, n, h, d).clone()
+    v[:, 0] = torch.arange(d) % 2 * v[:, 1].amax(-1, keepdim=True)
+    k, v = k.to(dtype), v.to(dtype)
+    q = dirn.expand(MANY, 1, h, d).to(dtype)
+    pool, kx, vx = filled(cuda, k, v)
+    got = ops.kv4_attention(q.to(cuda), pool, table([0] * MANY, cuda), table([n - 1] * MANY, cuda))
+    # the codes differ behind the first position and at the ends of 32 lanes in at most 4 shares
+    for i in (0, 77, MANY - 1):
+        check(got[i:i + 1], q[i:i + 1], kx, vx, [n - 1], dtype, False, terms=2 + 4 * 32)
