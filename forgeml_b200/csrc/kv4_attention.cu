@@ -274,7 +274,12 @@ __device__ __forceinline__ void store4(T* op, int c, int D, bool vec, float4 f) 
 }
 
 constexpr int kFlush = 1000;
-constexpr float kToInt0 = 1e37f;  // before any weight was seen: the first one of any size is over the bound
+// The integers' scale to_int stays finite: with kToIntMax the weights p s have all
+// their digits down to 2^-110 (two digits) or 2^-103 (three).  Where those of every
+// group are below kTiny, weights and sums are taken kLift times larger, which keeps the
+// digits of the smallest steps.
+constexpr float kToIntMax = 8.507059e37f;  // 2^126; a fast division by more gives 0
+constexpr float kTiny = 5.42101086e-20f, kLift = 1.1529215e18f;  // 2^-64, 2^60
 constexpr float kQMax = 1.2e8f;  // |16 q0 - q1| stays within four digits
 
 template <typename T, int G>
@@ -283,6 +288,7 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
   constexpr int PP = Parts<T>::p, SETS = U::SETS, kWarps = U::warps, kStages = U::stages;
   constexpr float kPMax = PP == 3 ? 8388600.f : 65530.f;
   constexpr bool kWide = std::is_same<T, float>::value;
+  constexpr bool kLifts = !std::is_same<T, __half>::value;  // fp16's smallest step is 2^-24
   using Score = typename std::conditional<kWide, double, float>::type;
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -399,7 +405,7 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
   int accm[G][4], accr[G][4];                                // sums of P lo and of P (lo + 16 hi)
   int accm3[PP == 3 ? G : 1][4], accr3[PP == 3 ? G : 1][4];  // third digits
   int ones[kWide ? SETS : 1][4], ones3[kWide ? SETS : 1][4];  // sums of P: the codes count from 8 then
-  float zacc[G], to_int[G], carry[G], m = -INFINITY, l = 0.f;
+  float zacc[G], to_int[G], carry[G], lift = 1.f, m = -INFINITY, l = 0.f;
   float* const o = reinterpret_cast<float*>(mem + U::out) + lane;  // channel 32 gi + 4 g + i: o[(4 gi + i) * 32]
   int stage = 0, since = 0;
   uint32_t parity = 0;
@@ -533,7 +539,7 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
         o[(4 * gi + i) * 32] = 0.f;
       }
       zacc[gi] = 0.f;
-      to_int[gi] = kToInt0;
+      to_int[gi] = kToIntMax;
       carry[gi] = 0.5f;
     }
     if constexpr (kWide) {
@@ -544,6 +550,7 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
     }
     m = -INFINITY;
     l = 0.f;
+    lift = 1.f;
     since = -1;
     for (int i = 0; i < n_units && live; ++i) {
     live = __all_sync(0xffffffffu, wait_copies(bars + 8 * stage, parity >> stage & 1));
@@ -607,7 +614,7 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
       bool over = false;
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) {
-        x[gi] = fmaf(pr * step[gi], to_int[gi], carry[gi]);
+        x[gi] = fmaf(pr * lift * step[gi], to_int[gi], carry[gi]);
         n[gi] = __fadd_rz(x[gi], 8388608.f);
         over |= n[gi] > 8388608.f + kPMax;
       }
@@ -615,8 +622,20 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
       if (mx > m || over || since == kFlush) {  // the same in every lane
         const float alpha = ex2(m - mn);
         m = mn;
+        // The bounds of p s.  What went before counts alpha times as much now, for its
+        // bound too: a large step whose weight vanishes must not leave the later weights
+        // without digits.  A quarter of headroom, so that they rise seldom.
+        float bound[G], most = 0.f;
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi) {
+          const float past = __fdividef(kPMax * alpha, to_int[gi]) * (lift == 1.f ? 1.f : 1.f / kLift);
+          bound[gi] = fmaxf(1.25f * warp_max(pr * step[gi]), since < 0 ? 0.f : past);
+          most = fmaxf(most, bound[gi]);
+        }
+        const float was = lift;
+        lift = kLifts && most < kTiny ? kLift : 1.f;
         if (since >= 0) {  // not the segment's first unit
-          flush(alpha);
+          flush(lift == was ? alpha : lift == 1.f ? alpha * (1.f / kLift) : alpha * kLift);
           l *= alpha;
 #pragma unroll
           for (int gi = 0; gi < G; ++gi) zacc[gi] *= alpha;
@@ -624,12 +643,8 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
         since = 0;
 #pragma unroll
         for (int gi = 0; gi < G; ++gi) {
-          // What went before counts alpha times as much now, for the bound too: a large
-          // step whose weight vanishes must not leave the later weights without digits.
-          // A quarter of headroom, so that it falls seldom.
-          const float big = 1.25f * warp_max(pr * step[gi]);
-          to_int[gi] = fminf(__fdividef(to_int[gi], alpha), __fdividef(kPMax, fmaxf(big, 1e-32f)));
-          x[gi] = fmaf(pr * step[gi], to_int[gi], 0.5f);
+          to_int[gi] = __fdividef(kPMax, fmaxf(bound[gi] * lift, kPMax / kToIntMax));
+          x[gi] = fmaf(pr * lift * step[gi], to_int[gi], 0.5f);
           n[gi] = __fadd_rz(x[gi], 8388608.f);
         }
       }
@@ -718,19 +733,19 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
       part_units[warp][which] = cur.units;
       part_op[warp][which] = seg_keys <= cur.keys ? seg_op : nullptr;  // null: a token outside the pool, zeros already
     }
-    const float inv = __frcp_rn(l);
+    const float inv = __frcp_rn(l), drop = lift == 1.f ? 1.f : 1.f / kLift;
 #pragma unroll
     for (int gi = 0; gi < G; ++gi) {
       const float z = warp_sum(zacc[gi]);
       float4 f;
       f.x = o[(4 * gi + 0) * 32];
-      f.x += __shfl_xor_sync(0xffffffffu, f.x, 2) + z;
+      f.x = fmaf(f.x + __shfl_xor_sync(0xffffffffu, f.x, 2), drop, z);
       f.y = o[(4 * gi + 1) * 32];
-      f.y += __shfl_xor_sync(0xffffffffu, f.y, 2) + z;
+      f.y = fmaf(f.y + __shfl_xor_sync(0xffffffffu, f.y, 2), drop, z);
       f.z = o[(4 * gi + 2) * 32];
-      f.z += __shfl_xor_sync(0xffffffffu, f.z, 2) + z;
+      f.z = fmaf(f.z + __shfl_xor_sync(0xffffffffu, f.z, 2), drop, z);
       f.w = o[(4 * gi + 3) * 32];
-      f.w += __shfl_xor_sync(0xffffffffu, f.w, 2) + z;
+      f.w = fmaf(f.w + __shfl_xor_sync(0xffffffffu, f.w, 2), drop, z);
       if (t == (gi & 3) >> 1) {
         const int c = 32 * gi + 4 * g;
         if (!whole) {

@@ -185,3 +185,34 @@ def test_many_small_weights_beside_a_large_one(cuda, dtype):
     # the codes differ behind the first position and at the ends of 32 lanes in at most 4 shares
     for i in (0, 77, MANY - 1):
         check(got[i:i + 1], q[i:i + 1], kx, vx, [n - 1], dtype, False, terms=2 + 4 * 32)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("exponent", [-80, -100, -110, -118])
+def test_values_near_the_smallest_numbers(cuda, dtype, exponent):
+    n, h, d = 1024, 16, 32
+    k = torch.randn(1, n, h, d, generator=gen(2)).to(dtype)
+    v = (torch.randn(1, n, h, d, generator=gen(3)) * 2.0 ** exponent).to(dtype)
+    q = torch.randn(MANY, 1, h, d, generator=gen(4)).to(dtype)
+    pool, kx, vx = filled(cuda, k, v)
+    got = ops.kv4_attention(q.to(cuda), pool, table([0] * MANY, cuda), table([n - 1] * MANY, cuda))
+    check(got[:2], q[:2], kx, vx, [n - 1] * 2, dtype, False)
+
+
+@pytest.mark.parametrize("lead", [0.0, 2.0 ** -30])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_steps_that_grow_by_many_powers_of_two(cuda, dtype, lead):
+    """Constant or tiny values first, then larger and larger ones, then tiny again."""
+    n, h, d = 1024, 16, 32
+    k = 0.3 * torch.randn(1, n, h, d, generator=gen(2)).to(dtype)
+    v = torch.randn(1, n, h, d, generator=gen(3))
+    v[:, :100] *= lead
+    for i, x in enumerate((-118, -60, 0, 40, 100)):
+        v[:, 100 + 64 * i:164 + 64 * i] *= 2.0 ** x
+    v[:, 420:] *= 2.0 ** -100
+    v = v.to(dtype)
+    q = torch.randn(MANY, 1, h, d, generator=gen(4)).to(dtype)
+    pool, kx, vx = filled(cuda, k, v)
+    for last in (90, 150, 230, 300, n - 1):
+        got = ops.kv4_attention(q.to(cuda), pool, table([0] * MANY, cuda), table([last] * MANY, cuda))
+        check(got[:1], q[:1], kx, vx, [last], dtype, False)
