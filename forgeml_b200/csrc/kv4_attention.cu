@@ -600,11 +600,13 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
           codes = fma((double)step[gi], fma((double)e[0], 65536.0, (double)e[4 * 36]), codes);
           lows = fma((double)low[gi], qsum[gi], lows);
         } else {
-          codes = fmaf(step[gi], fmaf(d[0], 65536.f, d[4 * 36]), codes);
+          // (the steps' products with the integers may overflow: unit_q goes with the steps)
+          codes = fmaf(step[gi] * unit_q, fmaf(d[0], 65536.f, d[4 * 36]), codes);
           lows = fmaf(low[gi], qsum[gi], lows);
         }
       }
-      const Score sc = valid ? codes * unit_q + lows : (Score)-INFINITY;
+      if constexpr (kWide) codes *= unit_q;
+      const Score sc = valid ? codes + lows : (Score)-INFINITY;
       const float mx = warp_max((float)sc);
       lds_params<T, G>(st + U::vp + my_pos * U::PR, part, valid, step, low);
       // ---- weights, as integers up to kPMax

@@ -216,3 +216,27 @@ def test_steps_that_grow_by_many_powers_of_two(cuda, dtype, lead):
     for last in (90, 150, 230, 300, n - 1):
         got = ops.kv4_attention(q.to(cuda), pool, table([0] * MANY, cuda), table([last] * MANY, cuda))
         check(got[:1], q[:1], kx, vx, [last], dtype, False)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16])
+@pytest.mark.parametrize("qp,kp", [(-88, 90), (-20, 100), (60, -64)])
+def test_scores_of_large_keys_and_small_queries(cuda, dtype, qp, kp):
+    n, h, d = 200, 4, 64
+    k = (torch.randn(1, n, h, d, generator=gen(2)) * 2.0 ** kp).to(dtype)
+    if qp + kp > 8:
+        # such scores leave one position; it is apart from the others by far
+        k[0, :, :, :] = k[0, :, :, :].float().mul(2.0 ** -40).to(dtype)
+        k[0, 77] = k[0, 77].float().mul(2.0 ** 40).to(dtype)
+    v = torch.randn(1, n, h, d, generator=gen(3)).to(dtype)
+    q = (torch.randn(1, 1, h, d, generator=gen(4)) * 2.0 ** qp).to(dtype)
+    if qp + kp > 8:  # towards that position
+        q = (k[:, 77:78].float().sign() * q.float().abs()).to(dtype)
+    pool, kx, vx = filled(cuda, k, v)
+    got = ops.kv4_attention(q.to(cuda), pool, table([0], cuda), table([n - 1], cuda))
+    if qp + kp > 8:
+        want = vx[0, 77].reshape(-1)
+        f = torch.finfo(dtype)
+        err = (got[0, 0].cpu().double() - want).abs()
+        assert (err <= f.eps / 2 * want.abs() + 200 * 2.0 ** -24 * want.abs().max() + 32 * 20 / LEVELS[dtype]).all(), err.max()
+    else:
+        check(got, q, kx, vx, [n - 1], dtype, False)
