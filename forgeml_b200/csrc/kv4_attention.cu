@@ -607,11 +607,18 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
       }
       if constexpr (kWide) codes *= unit_q;
       const Score sc = valid ? codes + lows : (Score)-INFINITY;
-      const float mx = warp_max((float)sc);
+      // In 32 bits; a score that has more is rounded up, so that no weight passes 1.
+      float near;
+      if constexpr (kWide) near = __double2float_ru(sc);
+      else near = sc;
+      const float mx = warp_max(near);
       lds_params<T, G>(st + U::vp + my_pos * U::PR, part, valid, step, low);
       // ---- weights, as integers up to kPMax
       const float mn = fmaxf(m, mx);
-      const float pr = valid ? ex2((float)(sc - mn)) : 0.f;
+      float away = (float)(sc - mn);
+      // Scores that 32 bits do not keep apart from the largest one count, however large.
+      if (kWide && near == mn) away = fmaxf(away, -16.f);
+      const float pr = valid ? ex2(away) : 0.f;
       float x[G], n[G];
       bool over = false;
 #pragma unroll

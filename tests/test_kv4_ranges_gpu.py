@@ -218,7 +218,7 @@ def test_steps_that_grow_by_many_powers_of_two(cuda, dtype, lead):
         check(got[:1], q[:1], kx, vx, [last], dtype, False)
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("qp,kp", [(-88, 90), (-20, 100), (60, -64)])
 def test_scores_of_large_keys_and_small_queries(cuda, dtype, qp, kp):
     n, h, d = 200, 4, 64
