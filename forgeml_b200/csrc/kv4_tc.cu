@@ -64,8 +64,8 @@ struct Smem {
   static_assert(tm_o + D <= (G > 4 ? tm_q : tm_p) && tm_q + D / 2 <= kTmemCols, "TMEM");
   static constexpr uint32_t k = 0, v = stages * kOperand;
   static constexpr uint32_t bars = 2 * stages * kOperand;
-  static constexpr uint32_t rows = bars + 512;  // what a row's two threads tell each other: [2][2][128] fp32
-  static constexpr uint32_t factors = rows + 2048;  // powers of two of the tiles' keys and values: [4 blocks][2][4]
+  static constexpr uint32_t rows = bars + 512;  // what a row's two threads tell each other: [2][2][128] fp32 pairs
+  static constexpr uint32_t factors = rows + 4096;  // the tiles' keys' powers of two and values' exponents: [4 blocks][2][4]
   static constexpr uint32_t nans = factors + 128;   // first position whose value is NaN: [4 parts][4 tiles][8 groups]
   static constexpr uint32_t total = nans + 512 + 1024;  // 1024: alignment of the base
   static_assert(total <= 227 * 1024, "shared memory");
@@ -142,7 +142,12 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
 // rounded to 8 bits once more, would double the output's error.  bf16's range is
 // kept by powers of two: of a query row, of a tile's keys and of a tile's values,
 // each chosen so that the largest number lies near 2^12 (numbers 2^-26 of that are
-// still whole); they are taken off the scores, and put on the weights.
+// still whole).  They are taken off the scores.  On the values' side a row's weights
+// become P = p 2^(14 - e - w): e the exponent of the position's tile, w the running
+// maximum of (log2 of the tile's largest p) - e over the tiles that the row attends.
+// So P is at most 2^14, and near it where weight times value is largest, whatever a
+// value of vanishing weight, or one that the row does not attend, is; the output is
+// in units of 2^(w - 14).  w is kept against the scores' running maximum.
 //
 // 2^12 over the power of two at or below x (positive, not NaN); 2^126 at most (a
 // fast division by more gives 0).
@@ -150,6 +155,7 @@ __device__ __forceinline__ float power_to_12(float x) {
   const int e = __float_as_int(x) >> 23;
   return __int_as_float(max(1, min(253, 266 - e)) << 23);
 }
+constexpr float kTop = 14.f;  // log2 of the largest weight as the tensor cores get it
 
 // A word of eight codes as eight fp16 numbers z + c s (s, z in `sz`), in the order
 // 0 4 1 5 2 6 3 7, within the finite range that a rounded-up step could leave.
@@ -421,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (who != 0 && lane == i) nan = min(nan, j * kBlock + dw * 32 + __ffs((int)who) - 1);
           }
         }
-        float mine = 1.f;  // lane 0: the keys' power of two, lane 1: the values'
+        float mine = 1.f;  // lane 0: the keys' power of two, lane 1: the values' exponent
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
@@ -429,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < G; ++i) big = fmaxf(big, ok ? largest_of(sz[kv][i]) : 0.f);
             const float f = power_to_12(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big))));
-            if (lane == kv) mine = f;
+            if (lane == kv) mine = kv ? (float)((__float_as_int(f) >> 23) - 127) : f;
 #pragma unroll
             for (int i = 0; i < G; ++i) sz[kv][i] = scaled_params<T>(sz[kv][i], f);
           }
@@ -504,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ queries, softmax, epilogue
     const int quad = warp & 3, hx = warp >> 2, r = quad * 32 + lane;  // row of the segment = TMEM lane; half
     const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16);
-    float* const told = reinterpret_cast<float*>(mem + L::rows);
+    float2* const told = reinterpret_cast<float2*>(mem + L::rows);
     // the thread's share of the channels, in groups
     constexpr int kHalf = (G + 1) / 2;
     const int group0 = hx ? kHalf : 0, group1 = hx ? G : kHalf;
@@ -512,9 +518,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool live = true;
     unsigned blk = 0, parts = 0, met = 0, paired = 0;
     // What the row's other thread has to tell (the two warps of the same rows meet).
-    auto exchange = [&](float x) {
+    auto exchange = [&](float x, float y = 0.f) {
       const int buf = paired & 1;
-      told[(buf * 2 + hx) * kRows + r] = x;
+      told[(buf * 2 + hx) * kRows + r] = make_float2(x, y);
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(kPair + quad));
       live = __all_sync(0xffffffffu, live && wait_copies(bar(kPair + quad), buf));
@@ -573,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 big = fmaxf(big, fmaxf(fabsf(__uint_as_float(x[i] << 16)), fabsf(__uint_as_float(x[i] & 0xffff0000u))));
             }
           }
-          big = fmaxf(big, exchange(big));
+          big = fmaxf(big, exchange(big).x);
           if (!live) break;
           const float f = power_to_12(big);
           q_scale = __fdividef(a.scale_log2, f);
@@ -605,9 +611,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kQFull));
       }
-      // the values' power of two that the output is in: the least of the tiles' so far
-      float unit = __int_as_float(253 << 23);
-      float m = -INFINITY, l = 0.f;
+      // Scores' running maximum and sum of weights; w - m (bf16: see power_to_12).
+      float m = -INFINITY, l = 0.f, wm = -INFINITY;
       for (int j = 0; j < nb && live; ++j, ++blk) {
         live = wait_copies(bar(kSFull + blk % NS), (blk / NS) & 1);
         if (!__all_sync(0xffffffffu, live)) {
@@ -620,14 +625,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool full = __all_sync(0xffffffffu, lim >= kBlock || !mine);
         const bool any = __any_sync(0xffffffffu, lim > 0);
         const float* const f = reinterpret_cast<const float*>(mem + L::factors) + (blk & 3) * 8;
+        constexpr bool kScaled = std::is_same<T, __nv_bfloat16>::value;
         float alpha = 1.f, v[64], k_scale[2], v_scale[2];
         if (any) {
           tmem_ld64(ts + 64 * hx, v);
-          float mx = -INFINITY;
+          float mt[2];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             // scores in log2 units: both powers of two off
-            k_scale[c] = std::is_same<T, __half>::value ? q_scale : fmaxf(__fdividef(q_scale, f[2 * hx + c]), 1.2e-38f);
+            k_scale[c] = kScaled ? fmaxf(__fdividef(q_scale, f[2 * hx + c]), 1.2e-38f) : q_scale;
             float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             if (full) {
 #pragma unroll
@@ -639,23 +645,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                 m4[e & 3] = fmaxf(m4[e & 3], v[32 * c + e]);
               }
             }
-            mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * k_scale[c]);
+            mt[c] = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * k_scale[c];
           }
+          const float mx = fmaxf(mt[0], mt[1]);
+          // the largest weight times value of the thread's tiles, against its own maximum
+          // (NaN where it attends nothing: fmaxf passes it over)
+          const float at = kScaled ? fmaxf(mt[0] - mx - f[4 + 2 * hx], mt[1] - mx - f[5 + 2 * hx]) : 0.f;
           if (NS == 1) tc_fence_before();  // the other thread's P goes over these scores
-          mx = fmaxf(mx, exchange(mx));
+          const float2 other = exchange(mx, at);
           if (!live) break;
           if (NS == 1) tc_fence_after();
-          const float mn = fmaxf(m, mx);
+          const float mn = fmaxf(m, fmaxf(mx, other.x));
           alpha = m == -INFINITY ? 0.f : ex2(m - mn);
-          m = mn;
           l *= alpha;
-        }
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-          const float least = fminf(unit, fminf(fminf(f[4], f[5]), fminf(f[6], f[7])));
-          alpha *= __fdividef(least, unit);
-          unit = least;
+          if constexpr (kScaled) {
+            const float was = m == -INFINITY ? -INFINITY : wm + (m - mn);
+            wm = fmaxf(was, fmaxf(at + (mx - mn), other.y + (other.x - mn)));
+            alpha = was == -INFINITY ? 0.f : ex2(was - wm);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) v_scale[c] = __fdividef(unit, f[4 + 2 * hx + c]);
+            for (int c = 0; c < 2; ++c) v_scale[c] = ex2(fminf(kTop - f[4 + 2 * hx + c] - wm, 126.f));
+          }
+          m = mn;
         }
         // P and the running output are free once the block before is through
         if (j > 0) {
@@ -715,9 +725,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
       }
       if (!live) break;
-      l += exchange(l);
+      l += exchange(l).x;
       if (!live) break;
-      const float off_unit = std::is_same<T, __half>::value ? 1.f : __fdividef(1.0f, unit);
+      // the output's unit, in two factors: their product may pass the range of numbers
+      const float unit = std::is_same<T, __half>::value ? 1.f : 1.f / (float)(1 << (int)kTop);
+      const float scale = std::is_same<T, __half>::value || wm == -INFINITY ? 1.f : ex2(wm);
       // whether the row attends a value of NaN in the channels of group c
       const int* const nans = reinterpret_cast<const int*>(mem + L::nans) + (parts & 3) * 32;
       auto nan_in = [&](int c) {
@@ -726,12 +738,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (nb > 0) ++parts;
       T* const op = static_cast<T*>(a.out) + (((long long)part.b * a.tq + tok) * a.QH + qh) * p.D;
       // a row's 32 columns, in the operands' order, as the output's channels
-      auto store = [&](int c, const float (&v)[32], float f) {
+      auto store = [&](int c, const float (&v)[32], float f, float f2) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float* x = v + 8 * i;
-          const uint4 w = make_uint4(pack2<T>(x[0] * f, x[2] * f), pack2<T>(x[4] * f, x[6] * f),
-                                     pack2<T>(x[1] * f, x[3] * f), pack2<T>(x[5] * f, x[7] * f));
+          auto two = [&](int i0, int i1) { return pack2<T>(x[i0] * f * f2, x[i1] * f * f2); };
+          const uint4 w = make_uint4(two(0, 2), two(4, 6), two(1, 3), two(5, 7));
           const int c0 = c * 32 + 8 * i;
           if (a.out_vec) {
             if (c0 < p.D) *reinterpret_cast<uint4*>(op + c0) = w;
@@ -744,12 +756,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       if (part.whole) {
         if (used) {
-          const float inv = __fdividef(1.0f, l) * off_unit;
+          const float inv = __fdividef(unit, l);
 #pragma unroll 1
           for (int c = group0; c < group1; ++c) {
             float v[32];
             tmem_ld32(trow + L::tm_o + c * 32, v);
-            if (mine) store(c, v, nan_in(c) ? NAN : inv);
+            if (mine) store(c, v, nan_in(c) ? NAN : inv, scale);
           }
         }
         continue;
@@ -762,12 +774,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = group0; c < group1; ++c) {
           float v[32];
           if (nb > 0) tmem_ld32(trow + L::tm_o + c * 32, v);
-          const float f = nan_in(c) ? NAN : off_unit;
+          const float f = nan_in(c) ? NAN : unit;
           if (mine && nb > 0)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
               __stcg(reinterpret_cast<float4*>(own + 4 + c * 32) + i,
-                     make_float4(v[4 * i] * f, v[4 * i + 1] * f, v[4 * i + 2] * f, v[4 * i + 3] * f));
+                     make_float4(v[4 * i] * f * scale, v[4 * i + 1] * f * scale, v[4 * i + 2] * f * scale,
+                                 v[4 * i + 3] * f * scale));
         }
       }
       if (!together()) break;
@@ -808,7 +821,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               x[4 * i + 3] = fmaf(f, y.w, x[4 * i + 3]);
             }
           }
-          store(c, x, 1.0f / ls);
+          store(c, x, 1.0f / ls, 1.f);
         }
       }
       together();  // taken_sh is read

@@ -240,3 +240,40 @@ def test_scores_of_large_keys_and_small_queries(cuda, dtype, qp, kp):
         assert (err <= f.eps / 2 * want.abs() + 200 * 2.0 ** -24 * want.abs().max() + 32 * 20 / LEVELS[dtype]).all(), err.max()
     else:
         check(got, q, kx, vx, [n - 1], dtype, False)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("power", [7, 14, 18, 22, 26])
+@pytest.mark.parametrize("at,d", [(110, 64), (110, 128), (64, 160)])
+def test_a_prompt_row_does_not_depend_on_a_large_later_value(cuda, dtype, power, at, d):
+    """Position ``at``'s value is 2^power times the others'."""
+    t, h = 128, 2
+    if dtype == torch.float16:
+        power = min(power, 13)
+    k, v = (torch.randn(1, t, h, d, generator=gen(s)) for s in (2, 3))
+    v[:, at] *= 2.0 ** power
+    k, v = k.to(dtype), v.to(dtype)
+    q = torch.randn(1, t, h, d, generator=gen(4)).to(dtype)
+    pool, kx, vx = filled(cuda, k, v)
+    got = ops.kv4_attention(q.to(cuda), pool, table([0], cuda), table([0], cuda))
+    check(got, q, kx, vx, [0], dtype, True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("power", [7, 14, 18, 22, 26, 60])
+@pytest.mark.parametrize("at", [5, 40, 200])
+def test_a_large_value_of_vanishing_weight_in_a_prompt(cuda, dtype, power, at):
+    """Scores of the rows around ``at`` lie far below the others'."""
+    t, h, d, start = 40, 2, 64, 300
+    if dtype == torch.float16:
+        power = min(power, 13)
+    dirn = torch.where(torch.rand(h, d, generator=gen(1)) < 0.5, -1.0, 1.0)
+    k = 0.3 * torch.randn(1, start + t, h, d, generator=gen(2))
+    k[:, at // 32 * 32:at // 32 * 32 + 32] -= (10 + power) / math.sqrt(d) * dirn
+    v = torch.randn(1, start + t, h, d, generator=gen(3))
+    v[:, at] *= 2.0 ** power
+    k, v = k.to(dtype), v.to(dtype)
+    q = (dirn + 0.1 * torch.randn(1, t, h, d, generator=gen(4))).to(dtype)
+    pool, kx, vx = filled(cuda, k, v)
+    got = ops.kv4_attention(q.to(cuda), pool, table([0], cuda), table([start], cuda))
+    check(got, q, kx, vx, [start], dtype, True)
