@@ -67,7 +67,9 @@ struct Smem {
   static constexpr uint32_t rows = bars + 512;  // what a row's two threads tell each other: [2][2][128] fp32 pairs
   static constexpr uint32_t factors = rows + 4096;  // the tiles' keys' powers of two and values' exponents: [4 blocks][2][4]
   static constexpr uint32_t nans = factors + 128;   // first position whose value is NaN: [4 parts][4 tiles][8 groups]
-  static constexpr uint32_t total = nans + 512 + 1024;  // 1024: alignment of the base
+  static constexpr uint32_t own = nans + 512;  // positions' factors of their scores, values' exponents: [4 blocks][2][128] fp32
+  static constexpr uint32_t largest = own + 4096;  // rows' largest weight times value in wide blocks: [2][128] fp32
+  static constexpr uint32_t total = largest + 1024 + 1024;  // 1024: alignment of the base
   static_assert(total <= 227 * 1024, "shared memory");
 };
 enum Bar : int {
@@ -121,6 +123,25 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&w)[16
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 8 fp32 columns; complete on return.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const float (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n\ttcgen05.wait::st.sync.aligned;" ::"r"(taddr),
+               "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&w)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};\n\ttcgen05.wait::st.sync.aligned;" ::"r"(taddr),
+               "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+               : "memory");
+}
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
@@ -149,6 +170,11 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
 // value of vanishing weight, or one that the row does not attend, is; the output is
 // in units of 2^(w - 14).  w is kept against the scores' running maximum.
 //
+// A tile whose positions' largest keys, or values, differ by more than kWide is a wide
+// one: its positions have powers of their own, so that none takes the others' bits,
+// attended or not, and a block with such a tile has its weights formed position by
+// position.  (None of the usual caches has any.)
+//
 // 2^12 over the power of two at or below x (positive, not NaN); 2^126 at most (a
 // fast division by more gives 0).
 __device__ __forceinline__ float power_to_12(float x) {
@@ -156,6 +182,7 @@ __device__ __forceinline__ float power_to_12(float x) {
   return __int_as_float(max(1, min(253, 266 - e)) << 23);
 }
 constexpr float kTop = 14.f;  // log2 of the largest weight as the tensor cores get it
+constexpr float kWide = 1024.f;
 
 // A word of eight codes as eight fp16 numbers z + c s (s, z in `sz`), in the order
 // 0 4 1 5 2 6 3 7, within the finite range that a rounded-up step could leave.
@@ -427,18 +454,32 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (who != 0 && lane == i) nan = min(nan, j * kBlock + dw * 32 + __ffs((int)who) - 1);
           }
         }
-        float mine = 1.f;  // lane 0: the keys' power of two, lane 1: the values' exponent
+        // bf16: powers of two of the tile, or of the lane's position
+        bool wide = false;
+        float own[2], powers[2], exponent = 0.f;
+        float mine = 1.f;  // lane 0: the keys' power of two (-1: a wide tile), lane 1: the values' exponent
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
             float big = 0.f;
 #pragma unroll
             for (int i = 0; i < G; ++i) big = fmaxf(big, ok ? largest_of(sz[kv][i]) : 0.f);
-            const float f = power_to_12(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big))));
-            if (lane == kv) mine = kv ? (float)((__float_as_int(f) >> 23) - 127) : f;
-#pragma unroll
-            for (int i = 0; i < G; ++i) sz[kv][i] = scaled_params<T>(sz[kv][i], f);
+            const uint32_t bits = __float_as_uint(big);
+            const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, bits));
+            const float least = __uint_as_float(__reduce_min_sync(0xffffffffu, bits == 0 ? 0x7f800000u : bits));
+            wide |= most > least * kWide;
+            own[kv] = big;
+            powers[kv] = power_to_12(most);
           }
+          if (wide)  // the same in every lane
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) powers[kv] = power_to_12(own[kv]);
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+            for (int i = 0; i < G; ++i) sz[kv][i] = scaled_params<T>(sz[kv][i], powers[kv]);
+          exponent = (float)((__float_as_int(powers[1]) >> 23) - 127);
+          mine = lane == 0 ? (wide ? -1.f : powers[0]) : exponent;
         }
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
@@ -451,6 +492,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           // keys' place is free once S of the block two before is done, which was issued
           // after the softmax of the block four before.
           if (kv == 0 && lane < 2) factors[(blk & 3) * 8 + 4 * lane + dw] = mine;
+          if (std::is_same<T, __nv_bfloat16>::value && kv == 0) {
+            float* const at = reinterpret_cast<float*>(mem + L::own) + (blk & 3) * 2 * kBlock + row;
+            at[0] = wide ? __int_as_float((254 << 23) - __float_as_int(powers[0])) : 1.f;  // 1 / power
+            at[kBlock] = exponent;
+          }
           // likewise four parts': S of a part's first block is issued after the softmax's
           // warps have read all of the part before
           if (kv == 0 && lane < G) nans[(parts & 3) * 32 + 8 * dw + lane] = nan;
@@ -626,6 +672,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool any = __any_sync(0xffffffffu, lim > 0);
         const float* const f = reinterpret_cast<const float*>(mem + L::factors) + (blk & 3) * 8;
         constexpr bool kScaled = std::is_same<T, __nv_bfloat16>::value;
+        // A block with a wide tile: its scores take their positions' factors first, and the
+        // largest weight times value is looked for.  (Rolled loops around the block's usual
+        // way: these lines, though no usual block takes them, cost the prompts 9 us, and 20
+        // unrolled or within it.)
+        const float* const own = reinterpret_cast<const float*>(mem + L::own) + (blk & 3) * 2 * kBlock + 64 * hx;
+        float* const largest = reinterpret_cast<float*>(mem + L::largest) + hx * kRows + r;
+        auto wide = [&]() { return kScaled && fminf(fminf(f[0], f[1]), fminf(f[2], f[3])) < 0.f; };
+        auto scale_of = [&](int c) { return fmaxf(__fdividef(q_scale, fabsf(f[2 * hx + c])), 1.2e-38f); };
+        if (kScaled && any && wide()) {
+          float at = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            const float k = scale_of(c / 4);
+            float x[8];
+            tmem_ld8(ts + 64 * hx + 8 * c, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              x[e] *= own[8 * c + e];
+              if (64 * hx + 8 * c + e < lim) at = fmaxf(at, fmaf(x[e], k, -own[kBlock + 8 * c + e]));
+            }
+            tmem_st8(ts + 64 * hx + 8 * c, x);
+          }
+          *largest = at;
+        }
         float alpha = 1.f, v[64], k_scale[2], v_scale[2];
         if (any) {
           tmem_ld64(ts + 64 * hx, v);
@@ -633,7 +703,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             // scores in log2 units: both powers of two off
-            k_scale[c] = kScaled ? fmaxf(__fdividef(q_scale, f[2 * hx + c]), 1.2e-38f) : q_scale;
+            k_scale[c] = kScaled ? scale_of(c) : q_scale;
             float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             if (full) {
 #pragma unroll
@@ -650,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float mx = fmaxf(mt[0], mt[1]);
           // the largest weight times value of the thread's tiles, against its own maximum
           // (NaN where it attends nothing: fmaxf passes it over)
-          const float at = kScaled ? fmaxf(mt[0] - mx - f[4 + 2 * hx], mt[1] - mx - f[5 + 2 * hx]) : 0.f;
+          const float at = !kScaled ? 0.f : wide() ? *largest - mx : fmaxf(mt[0] - mx - f[4 + 2 * hx], mt[1] - mx - f[5 + 2 * hx]);
           if (NS == 1) tc_fence_before();  // the other thread's P goes over these scores
           const float2 other = exchange(mx, at);
           if (!live) break;
@@ -705,7 +775,33 @@ __global__ void __launch_bounds__(kThreads, 1)
                 lp[e & 3] += p0 + p1;
               }
             }
-            tmem_st16(trow + L::tm_p + 32 * hx + 16 * c, w);
+            if (NS == 2 || !kScaled || !wide()) tmem_st16(trow + L::tm_p + 32 * hx + 16 * c, w);
+          }
+          if (kScaled && wide()) {  // with their own exponents
+            // (With one block of scores P goes over them: a thread's own go by ahead of it,
+            // those of the row's first thread before its second one begins.)
+            if (NS == 1 && hx == 1) {
+              exchange(0.f);
+              tc_fence_after();
+            }
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              const float k = scale_of(c / 4), top = kTop - wm;
+              float x[8];
+              tmem_ld8(ts + 64 * hx + 8 * c, x);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float up = fmaf(x[e], k, -off) - own[kBlock + 8 * c + e] + top;
+                x[e] = 64 * hx + 8 * c + e < lim ? ex2(fminf(up, kTop + 1.f)) : 0.f;
+              }
+              tmem_st4(trow + L::tm_p + 32 * hx + 4 * c,
+                       {pack2<__half>(x[0], x[1]), pack2<__half>(x[2], x[3]), pack2<__half>(x[4], x[5]), pack2<__half>(x[6], x[7])});
+            }
+            if (NS == 1 && hx == 0) {
+              tc_fence_before();
+              exchange(0.f);
+            }
+            if (!live) break;
           }
           tmem_st_wait();
           l += (lp[0] + lp[1]) + (lp[2] + lp[3]);

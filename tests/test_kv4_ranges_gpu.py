@@ -243,8 +243,8 @@ def test_scores_of_large_keys_and_small_queries(cuda, dtype, qp, kp):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("power", [7, 14, 18, 22, 26])
-@pytest.mark.parametrize("at,d", [(110, 64), (110, 128), (64, 160)])
+@pytest.mark.parametrize("power", [7, 14, 18, 22, 26, 40, 100])
+@pytest.mark.parametrize("at,d", [(110, 64), (110, 128), (64, 160), (10, 64)])
 def test_a_prompt_row_does_not_depend_on_a_large_later_value(cuda, dtype, power, at, d):
     """Position ``at``'s value is 2^power times the others'."""
     t, h = 128, 2
@@ -257,6 +257,19 @@ def test_a_prompt_row_does_not_depend_on_a_large_later_value(cuda, dtype, power,
     pool, kx, vx = filled(cuda, k, v)
     got = ops.kv4_attention(q.to(cuda), pool, table([0], cuda), table([0], cuda))
     check(got, q, kx, vx, [0], dtype, True)
+
+
+@pytest.mark.parametrize("power", [14, 26, 30, 40, 100])
+@pytest.mark.parametrize("at,d", [(110, 64), (110, 192), (64, 64)])
+def test_a_prompt_row_does_not_depend_on_a_large_later_key(cuda, power, at, d):
+    dtype, t, h = torch.bfloat16, 128, 2
+    k, v = (torch.randn(1, t, h, d, generator=gen(s)) for s in (2, 3))
+    k[:, at] *= 2.0 ** power
+    k, v = k.to(dtype), v.to(dtype)
+    q = torch.randn(1, t, h, d, generator=gen(4)).to(dtype)
+    pool, kx, vx = filled(cuda, k, v)
+    got = ops.kv4_attention(q.to(cuda), pool, table([0], cuda), table([0], cuda))
+    check(got, q, kx, vx, [0], dtype, True, rows=at)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
