@@ -68,8 +68,7 @@ struct Smem {
   static constexpr uint32_t factors = rows + 4096;  // the tiles' keys' powers of two and values' exponents: [4 blocks][2][4]
   static constexpr uint32_t nans = factors + 128;   // first position whose value is NaN: [4 parts][4 tiles][8 groups]
   static constexpr uint32_t own = nans + 512;  // positions' factors of their scores, values' exponents: [4 blocks][2][128] fp32
-  static constexpr uint32_t largest = own + 4096;  // rows' largest weight times value in wide blocks: [2][128] fp32
-  static constexpr uint32_t total = largest + 1024 + 1024;  // 1024: alignment of the base
+  static constexpr uint32_t total = own + 4096 + 1024;  // 1024: alignment of the base
   static_assert(total <= 227 * 1024, "shared memory");
 };
 enum Bar : int {
@@ -183,6 +182,8 @@ __device__ __forceinline__ float power_to_12(float x) {
 }
 constexpr float kTop = 14.f;  // log2 of the largest weight as the tensor cores get it
 constexpr float kWide = 1024.f;
+// Scores from which on the rounding of their maximum shows in the weights.
+constexpr float kFar = 4194304.f;  // 2^22
 
 // A word of eight codes as eight fp16 numbers z + c s (s, z in `sz`), in the order
 // 0 4 1 5 2 6 3 7, within the finite range that a rounded-up step could leave.
@@ -594,6 +595,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (threadIdx.x == 0) open_tickets(a.tickets + w0, a.launch);
       }
       float q_scale = a.scale_log2;  // of the scores, the row's power of two taken off
+      // Where a block's least factor is below this, scores could pass kFar: the products of
+      // bf16's operands are below 2^34 (2^26 D), fp16's below the query's sum times 65504.
+      float far_below = 0.f;
       if (nb > 0) {
         uint4 w[4 * kHalf];  // the thread's groups' channels; zeros where there is no row or channel
 #pragma unroll
@@ -615,6 +619,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
+        if constexpr (std::is_same<T, __half>::value) {
+          float sum = 0.f;
+#pragma unroll
+          for (int c = 0; c < 4 * kHalf; ++c) {
+            const __half2* const x = reinterpret_cast<const __half2*>(&w[c]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum += fabsf(__low2float(x[i])) + fabsf(__high2float(x[i]));
+          }
+          sum += exchange(sum).x;
+          if (!live) break;
+          far_below = sum * 65504.f * q_scale > kFar ? 2.f : 0.f;  // the factors are 1
+        }
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
           if (mine) {
 #pragma unroll
@@ -629,6 +645,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!live) break;
           const float f = power_to_12(big);
           q_scale = __fdividef(a.scale_log2, f);
+          far_below = q_scale * (1.71798692e10f / kFar);
 #pragma unroll
           for (int c = 0; c < 4 * kHalf; ++c) {
             uint32_t x[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
@@ -672,130 +689,91 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool any = __any_sync(0xffffffffu, lim > 0);
         const float* const f = reinterpret_cast<const float*>(mem + L::factors) + (blk & 3) * 8;
         constexpr bool kScaled = std::is_same<T, __nv_bfloat16>::value;
-        // A block with a wide tile: its scores take their positions' factors first, and the
-        // largest weight times value is looked for.  (Rolled loops around the block's usual
-        // way: these lines, though no usual block takes them, cost the prompts 9 us, and 20
-        // unrolled or within it.)
-        const float* const own = reinterpret_cast<const float*>(mem + L::own) + (blk & 3) * 2 * kBlock + 64 * hx;
-        float* const largest = reinterpret_cast<float*>(mem + L::largest) + hx * kRows + r;
-        auto wide = [&]() { return kScaled && fminf(fminf(f[0], f[1]), fminf(f[2], f[3])) < 0.f; };
-        auto scale_of = [&](int c) { return fmaxf(__fdividef(q_scale, fabsf(f[2 * hx + c])), 1.2e-38f); };
-        if (kScaled && any && wide()) {
-          float at = -INFINITY;
-#pragma unroll 1
-          for (int c = 0; c < 8; ++c) {
-            const float k = scale_of(c / 4);
-            float x[8];
-            tmem_ld8(ts + 64 * hx + 8 * c, x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              x[e] *= own[8 * c + e];
-              if (64 * hx + 8 * c + e < lim) at = fmaxf(at, fmaf(x[e], k, -own[kBlock + 8 * c + e]));
+        // The maximum of the row's scores moves to mn, that of weight times value to `seen`
+        // against it at least; the running sum and output follow.  False where a wait gave up.
+        auto move = [&](float mn, float seen) {
+          float alpha = 1.f;
+          if (any) {
+            alpha = m == -INFINITY ? 0.f : ex2(m - mn);
+            l *= alpha;
+            if constexpr (kScaled) {
+              const float was = m == -INFINITY ? -INFINITY : wm + (m - mn);
+              wm = fmaxf(was, seen);
+              alpha = was == -INFINITY ? 0.f : ex2(was - wm);
             }
-            tmem_st8(ts + 64 * hx + 8 * c, x);
+            m = mn;
           }
-          *largest = at;
-        }
-        float alpha = 1.f, v[64], k_scale[2], v_scale[2];
-        if (any) {
-          tmem_ld64(ts + 64 * hx, v);
-          float mt[2];
+          // P and the running output are free once the block before is through
+          if (j > 0) {
+            live = wait_copies(bar(kOFull), (blk - 1) & 1);
+            if (!__all_sync(0xffffffffu, live)) {
+              live = false;
+              return false;
+            }
+            tc_fence_after();
+            if (used && !__all_sync(0xffffffffu, alpha == 1.f || !mine)) {
+#pragma unroll 1
+              for (int c = group0; c < group1; ++c) {
+                float o[32];
+                tmem_ld32(to + c * 32, o);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            // scores in log2 units: both powers of two off
-            k_scale[c] = kScaled ? scale_of(c) : q_scale;
-            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (full) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], v[32 * c + e]);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                if (64 * hx + 32 * c + e >= lim) v[32 * c + e] = -INFINITY;
-                m4[e & 3] = fmaxf(m4[e & 3], v[32 * c + e]);
+                for (int e = 0; e < 32; ++e) o[e] *= alpha;
+                tmem_st32(to + c * 32, o);
               }
             }
-            mt[c] = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * k_scale[c];
           }
-          const float mx = fmaxf(mt[0], mt[1]);
-          // the largest weight times value of the thread's tiles, against its own maximum
-          // (NaN where it attends nothing: fmaxf passes it over)
-          const float at = !kScaled ? 0.f : wide() ? *largest - mx : fmaxf(mt[0] - mx - f[4 + 2 * hx], mt[1] - mx - f[5 + 2 * hx]);
-          if (NS == 1) tc_fence_before();  // the other thread's P goes over these scores
-          const float2 other = exchange(mx, at);
-          if (!live) break;
-          if (NS == 1) tc_fence_after();
-          const float mn = fmaxf(m, fmaxf(mx, other.x));
-          alpha = m == -INFINITY ? 0.f : ex2(m - mn);
-          l *= alpha;
-          if constexpr (kScaled) {
-            const float was = m == -INFINITY ? -INFINITY : wm + (m - mn);
-            wm = fmaxf(was, fmaxf(at + (mx - mn), other.y + (other.x - mn)));
-            alpha = was == -INFINITY ? 0.f : ex2(was - wm);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) v_scale[c] = ex2(fminf(kTop - f[4 + 2 * hx + c] - wm, 126.f));
-          }
-          m = mn;
-        }
-        // P and the running output are free once the block before is through
-        if (j > 0) {
-          live = wait_copies(bar(kOFull), (blk - 1) & 1);
-          if (!__all_sync(0xffffffffu, live)) {
-            live = false;
-            break;
-          }
-          tc_fence_after();
-          if (used && !__all_sync(0xffffffffu, alpha == 1.f || !mine)) {
+          return true;
+        };
+        auto scale_of = [&](int c) { return kScaled ? fmaxf(__fdividef(q_scale, fabsf(f[2 * hx + c])), 1.2e-38f) : q_scale; };
+        const float4 f4 = *reinterpret_cast<const float4*>(f);
+        if (__any_sync(0xffffffffu, fminf(fminf(f4.x, f4.y), fminf(f4.z, f4.w)) < far_below)) {
+          // A block with a wide tile, or with scores that could be far: position by position,
+          // the scores rounded before their maximum is taken.
+          const float* const own = reinterpret_cast<const float*>(mem + L::own) + (blk & 3) * 2 * kBlock + 64 * hx;
+          float mx = -INFINITY, at = -INFINITY, mn = m;
+          if (any) {
 #pragma unroll 1
-            for (int c = group0; c < group1; ++c) {
-              float o[32];
-              tmem_ld32(to + c * 32, o);
+            for (int c = 0; c < 8; ++c) {
+              const float k = scale_of(c / 4);
+              float x[8];
+              tmem_ld8(ts + 64 * hx + 8 * c, x);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] *= alpha;
-              tmem_st32(to + c * 32, o);
-            }
-          }
-        }
-        if (any) {
-          const float off = m == -INFINITY ? 0.f : m;
-          float lp[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t w[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int x = 32 * c + 2 * e;
-              const float p0 = ex2(fmaf(v[x], k_scale[c], -off)), p1 = ex2(fmaf(v[x + 1], k_scale[c], -off));
-              if constexpr (std::is_same<T, __half>::value) {
-                w[e] = pack2<__half>(p0, p1);
-                const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-                lp[e & 3] += g.x + g.y;  // the sum of what the tensor core multiplies
-              } else {
-                w[e] = pack2<__half>(p0 * v_scale[c], p1 * v_scale[c]);
-                lp[e & 3] += p0 + p1;
+              for (int e = 0; e < 8; ++e) {
+                x[e] = 64 * hx + 8 * c + e < lim ? __fmul_rn(kScaled ? x[e] * own[8 * c + e] : x[e], k) : -INFINITY;
+                mx = fmaxf(mx, x[e]);
+                if (kScaled) at = fmaxf(at, x[e] - own[kBlock + 8 * c + e]);
               }
+              tmem_st8(ts + 64 * hx + 8 * c, x);
             }
-            if (NS == 2 || !kScaled || !wide()) tmem_st16(trow + L::tm_p + 32 * hx + 16 * c, w);
+            tc_fence_before();
+            const float2 other = exchange(mx, at - mx);
+            if (!live) break;
+            tc_fence_after();
+            mn = fmaxf(m, fmaxf(mx, other.x));
+            at = fmaxf(at - mx + (mx - mn), other.y + (other.x - mn));
           }
-          if (kScaled && wide()) {  // with their own exponents
-            // (With one block of scores P goes over them: a thread's own go by ahead of it,
-            // those of the row's first thread before its second one begins.)
+          if (!move(mn, at)) break;
+          if (any) {
+            const float off = m == -INFINITY ? 0.f : m;
+            // With one block of scores P goes over them: a thread's own go by ahead of it, those
+            // of the row's first thread before its second one begins.
             if (NS == 1 && hx == 1) {
               exchange(0.f);
               tc_fence_after();
             }
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {
-              const float k = scale_of(c / 4), top = kTop - wm;
-              float x[8];
+              float x[8], p[8];
               tmem_ld8(ts + 64 * hx + 8 * c, x);
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
-                const float up = fmaf(x[e], k, -off) - own[kBlock + 8 * c + e] + top;
-                x[e] = 64 * hx + 8 * c + e < lim ? ex2(fminf(up, kTop + 1.f)) : 0.f;
+                x[e] -= off;
+                p[e] = ex2(x[e]);
+                l += p[e];
+                if (kScaled) p[e] = ex2(fminf(x[e] - own[kBlock + 8 * c + e] + (kTop - wm), kTop + 1.f));
               }
               tmem_st4(trow + L::tm_p + 32 * hx + 4 * c,
-                       {pack2<__half>(x[0], x[1]), pack2<__half>(x[2], x[3]), pack2<__half>(x[4], x[5]), pack2<__half>(x[6], x[7])});
+                       {pack2<__half>(p[0], p[1]), pack2<__half>(p[2], p[3]), pack2<__half>(p[4], p[5]), pack2<__half>(p[6], p[7])});
             }
             if (NS == 1 && hx == 0) {
               tc_fence_before();
@@ -803,9 +781,67 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (!live) break;
           }
-          tmem_st_wait();
-          l += (lp[0] + lp[1]) + (lp[2] + lp[3]);
-        } else if (used) {  // all masked: weights of zero
+        } else {
+          float v[64], k_scale[2], v_scale[2], mn = m, seen = -INFINITY;
+          if (any) {
+            tmem_ld64(ts + 64 * hx, v);
+            float mt[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              // scores in log2 units: both powers of two off
+              k_scale[c] = scale_of(c);
+              float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+              if (full) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], v[32 * c + e]);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  if (64 * hx + 32 * c + e >= lim) v[32 * c + e] = -INFINITY;
+                  m4[e & 3] = fmaxf(m4[e & 3], v[32 * c + e]);
+                }
+              }
+              mt[c] = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * k_scale[c];
+            }
+            const float mx = fmaxf(mt[0], mt[1]);
+            // the largest weight times value of the thread's tiles, against its own maximum
+            // (NaN where it attends nothing: fmaxf passes it over)
+            const float at = kScaled ? fmaxf(mt[0] - mx - f[4 + 2 * hx], mt[1] - mx - f[5 + 2 * hx]) : 0.f;
+            if (NS == 1) tc_fence_before();  // the other thread's P goes over these scores
+            const float2 other = exchange(mx, at);
+            if (!live) break;
+            if (NS == 1) tc_fence_after();
+            mn = fmaxf(m, fmaxf(mx, other.x));
+            seen = fmaxf(at + (mx - mn), other.y + (other.x - mn));
+          }
+          if (!move(mn, seen)) break;
+          if (any) {
+            const float off = m == -INFINITY ? 0.f : m;
+            float lp[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              if (kScaled) v_scale[c] = ex2(fminf(kTop - f[4 + 2 * hx + c] - wm, 126.f));
+              uint32_t w[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const int x = 32 * c + 2 * e;
+                const float p0 = ex2(fmaf(v[x], k_scale[c], -off)), p1 = ex2(fmaf(v[x + 1], k_scale[c], -off));
+                if constexpr (!kScaled) {
+                  w[e] = pack2<__half>(p0, p1);
+                  const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                  lp[e & 3] += g.x + g.y;  // the sum of what the tensor core multiplies
+                } else {
+                  w[e] = pack2<__half>(p0 * v_scale[c], p1 * v_scale[c]);
+                  lp[e & 3] += p0 + p1;
+                }
+              }
+              tmem_st16(trow + L::tm_p + 32 * hx + 16 * c, w);
+            }
+            tmem_st_wait();
+            l += (lp[0] + lp[1]) + (lp[2] + lp[3]);
+          }
+        }
+        if (!any && used) {  // all masked: weights of zero
           const uint32_t w[16] = {};
           tmem_st16(trow + L::tm_p + 32 * hx, w);
           tmem_st16(trow + L::tm_p + 32 * hx + 16, w);

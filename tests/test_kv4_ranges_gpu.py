@@ -290,3 +290,23 @@ def test_a_large_value_of_vanishing_weight_in_a_prompt(cuda, dtype, power, at):
     pool, kx, vx = filled(cuda, k, v)
     got = ops.kv4_attention(q.to(cuda), pool, table([0], cuda), table([start], cuda))
     check(got, q, kx, vx, [start], dtype, True)
+
+
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 3e4), (torch.bfloat16, 3e4), (torch.bfloat16, 1e12), (torch.float32, 1e12)])
+@pytest.mark.parametrize("t,d", [(1, 64), (9, 64), (9, 192)])
+def test_scores_beyond_what_their_maximum_keeps(cuda, dtype, size, t, d):
+    """One position is ahead of the others by far; its weight is 1 whatever fp32 keeps of
+    the scores."""
+    n, h = 200, 2
+    dirn = torch.where(torch.rand(h, d, generator=gen(1)) < 0.5, -1.0, 1.0)
+    k = torch.randn(1, n, h, d, generator=gen(2))
+    k[:, 77] = size * dirn
+    k, v = k.to(dtype), torch.randn(1, n, h, d, generator=gen(3)).to(dtype)
+    q = (size * (dirn + 0.1 * torch.randn(1, t, h, d, generator=gen(4)))).to(dtype)
+    pool, kx, vx = filled(cuda, k, v)
+    got = ops.kv4_attention(q.to(cuda), pool, table([0], cuda), table([n - t], cuda)).cpu().double()
+    want = vx[0, 77].reshape(-1)
+    # the value and the output rounded; p s as an integer, 15 codes; fp32 sums of z and c s
+    u = max(torch.finfo(dtype).eps / 2, 2.0 ** -11 if t > 8 and dtype != torch.float32 else 0)
+    off = 2 * u * want.abs() + (20 / LEVELS[dtype] + 40 * 2.0 ** -24) * want.abs().max()
+    assert ((got[0] - want).abs() <= off).all()
