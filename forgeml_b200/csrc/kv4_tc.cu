@@ -184,6 +184,13 @@ constexpr float kTop = 14.f;  // log2 of the largest weight as the tensor cores 
 constexpr float kWide = 1024.f;
 // Scores from which on the rounding of their maximum shows in the weights.
 constexpr float kFar = 4194304.f;  // 2^22
+// What fp16's weights and their sum are taken against, for a maximum m: they go up to
+// 2^14 as well where m keeps its ones (up to 1 they would end at 2^-25, and of many small
+// ones beside a large one none would count).
+template <typename T>
+__device__ __forceinline__ float base_of(float m) {
+  return std::is_same<T, __half>::value && fabsf(m) < kFar ? m - kTop : m;
+}
 
 // A word of eight codes as eight fp16 numbers z + c s (s, z in `sz`), in the order
 // 0 4 1 5 2 6 3 7, within the finite range that a rounded-up step could leave.
@@ -694,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto move = [&](float mn, float seen) {
           float alpha = 1.f;
           if (any) {
-            alpha = m == -INFINITY ? 0.f : ex2(m - mn);
+            alpha = m == -INFINITY ? 0.f : ex2(base_of<T>(m) - base_of<T>(mn));
             l *= alpha;
             if constexpr (kScaled) {
               const float was = m == -INFINITY ? -INFINITY : wm + (m - mn);
@@ -754,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (!move(mn, at)) break;
           if (any) {
-            const float off = m == -INFINITY ? 0.f : m;
+            const float off = m == -INFINITY ? 0.f : base_of<T>(m);
             // With one block of scores P goes over them: a thread's own go by ahead of it, those
             // of the row's first thread before its second one begins.
             if (NS == 1 && hx == 1) {
@@ -816,7 +823,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (!move(mn, seen)) break;
           if (any) {
-            const float off = m == -INFINITY ? 0.f : m;
+            const float off = m == -INFINITY ? 0.f : base_of<T>(m);
             float lp[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -901,7 +908,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---- other CTAs hold parts of the segment
       float* own = a.ws + ((long long)blockIdx.x * 2 + part.which) * kShare + r * (4 + D);
       if (used) {
-        if (mine && hx == 0) __stcg(reinterpret_cast<float4*>(own), make_float4(m, l, 0.f, 0.f));
+        if (mine && hx == 0) __stcg(reinterpret_cast<float4*>(own), make_float4(base_of<T>(m), l, 0.f, 0.f));
 #pragma unroll 1
         for (int c = group0; c < group1; ++c) {
           float v[32];

@@ -310,3 +310,20 @@ def test_scores_beyond_what_their_maximum_keeps(cuda, dtype, size, t, d):
     u = max(torch.finfo(dtype).eps / 2, 2.0 ** -11 if t > 8 and dtype != torch.float32 else 0)
     off = 2 * u * want.abs() + (20 / LEVELS[dtype] + 40 * 2.0 ** -24) * want.abs().max()
     assert ((got[0] - want).abs() <= off).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_small_weights_beside_a_large_one_on_the_tensor_cores(cuda, dtype):
+    """As above, with weights below half of fp16's smallest step."""
+    n, h, d, t, b = 8192, 16, 32, 9, 20
+    dirn = torch.where(torch.rand(h, d, generator=gen(1)) < 0.5, -1.0, 1.0)
+    half = 25.5 * math.log(2) / 2 / math.sqrt(d)
+    k = (-half * dirn).expand(1, n, h, d).clone()
+    k[:, 0] = half * dirn
+    v = torch.randn(h, d, generator=gen(3)).abs().expand(1, n, h, d).clone()
+    v[:, 0] = torch.arange(d) % 2 * v[:, 1].amax(-1, keepdim=True)
+    k, v = k.to(dtype), v.to(dtype)
+    q = dirn.expand(b, t, h, d).to(dtype)
+    pool, kx, vx = filled(cuda, k, v)
+    got = ops.kv4_attention(q.to(cuda), pool, table([0] * b, cuda), table([n - t] * b, cuda))
+    check(got[:1], q[:1], kx, vx, [n - t], dtype, True, rows=2)
