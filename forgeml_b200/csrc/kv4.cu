@@ -89,10 +89,13 @@ __device__ __forceinline__ void range(const Row8<T, VEC>& r, const float (&x)[8]
 // stays finite; scaled by a power of two when s is tiny so that 1 / u does).
 // With y near 1 / u, q0 = d y, r = d - q0 u (exact) and q = q0 + r y rounded
 // once, q is the quotient rounded to fp32 but for 2^-44 of it (Markstein's
-// correction step).  For the 16-bit types a quotient that is not itself a border
-// k + 1/2 is at least 2^-20 of it away from one, so q falls on a border only
-// where the quotient does, and adding 1.5 * 2^23 (to nearest, ties to even) gives
-// its code.  For fp32 the exact remainder, with what x - z lost, decides.
+// correction step).  For the 16-bit types, where d is exact, a quotient that is not
+// itself a border k + 1/2 is at least 2^-20 of it away from one, so q falls on a border
+// only where the quotient does, and adding 1.5 * 2^23 (to nearest, ties to even) gives
+// its code.  d is exact where no number is below 2^-16 (bf16) or 2^-13 (fp16) of the
+// group's span (`exact`).  Elsewhere the remainder, with what d lost, decides where q is a
+// border (the borders times u are exact, so rounding d and q does not pass one); for
+// fp32, whose borders are not, it always does.
 constexpr float kRound = 12582912.f;  // 1.5 * 2^23
 template <typename T> __device__ __forceinline__ float smallest_normal();
 template <> __device__ __forceinline__ float smallest_normal<float>() { return 1.17549435e-38f; }
@@ -125,8 +128,33 @@ __device__ __forceinline__ bool plain(float half_range) {
   return sizeof(T) == 2 && half_range >= (std::is_same<T, __half>::value ? 5e-4f : 1e-15f) &&
          half_range <= 3.402823466e38f;
 }
+// Whether x - z is exact in fp32 for a thread's eight numbers and the group's minimum (a
+// sufficient condition: numbers of p bits that are at least 2^(p - 24) of the span are
+// multiples of the difference's last place).
+__device__ __forceinline__ float least2(__nv_bfloat162 a) { return __bfloat162float(__hmin(a.x, a.y)); }
+__device__ __forceinline__ float least2(__half2 a) { return __half2float(__hmin(a.x, a.y)); }
+template <typename T, bool VEC>
+__device__ __forceinline__ bool exact(const Row8<T, VEC>& r, float half_range, float z) {
+  if constexpr (sizeof(T) == 4) {
+    return true;  // not looked at
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* e = reinterpret_cast<const T2*>(r.raw);
+    const float smallest = least2(__hmin2(__hmin2(__habs2(e[0]), __habs2(e[1])), __hmin2(__habs2(e[2]), __habs2(e[3]))));
+    return fminf(smallest, fabsf(z)) >= half_range * (std::is_same<T, __half>::value ? 2.44140625e-4f : 3.0517578125e-5f);  // 2^-12, 2^-15
+  }
+}
+// Where a quotient q of d + lost = x - z by u is a border, moves it off to the side that
+// the exact remainder says.
+__device__ __forceinline__ float off_border(float q, float x, float scale, float zs, float u) {
+  if (fabsf(q - rintf(q)) != 0.5f) return q;
+  const float xs = x * scale, d = xs + zs, b = d - xs;
+  const float lost = (xs - (d - b)) + (zs - b);  // x - z = d + lost exactly
+  const float r = fmaf(-q, u, d) + lost;  // (the first is exact; it is 0 or far above what d lost)
+  return r > 0.f ? q + 0.25f : r < 0.f ? q - 0.25f : q;
+}
 template <typename T>
-__device__ __forceinline__ uint32_t quantise8_plain(const float (&x)[8], float half_range, float z, float& s) {
+__device__ __forceinline__ uint32_t quantise8_plain(const float (&x)[8], float half_range, float z, bool exact, float& s) {
   const float s0 = half_range * kPerStep;
   s = to_f32<T>(from_f32<T>(fmaf(fmaf(-s0, 7.5f, half_range), kPerStep, s0)));
   const float u = 0.5f * s, zs = -0.5f * z, y = near_reciprocal(u);
@@ -135,6 +163,10 @@ __device__ __forceinline__ uint32_t quantise8_plain(const float (&x)[8], float h
   for (int i = 0; i < 8; ++i) {
     const float d = fmaf(x[i], 0.5f, zs), q0 = d * y;
     q[i] = fmaf(fmaf(-q0, u, d), y, q0);
+  }
+  if (!exact) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = off_border(q[i], x[i], 0.5f, zs, u);
   }
   return pack8(q);
 }
@@ -165,16 +197,16 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float half_ra
   for (int i = 0; i < 8; ++i) {
     const float d = fmaf(x[i], scale, zs), q0 = d * y;
     q[i] = fmaf(fmaf(-q0, u, d), y, q0);
-    if constexpr (sizeof(T) == 4) {
-      float c = rintf(q[i]);
-      const float xs = x[i] * scale, b = d - xs;
-      const float lost = (xs - (d - b)) + (zs - b);  // x - z = d + lost exactly
-      const float r = fmaf(-c, u, d) + lost, h = 0.5f * u;
-      const bool odd = ((int)c & 1) != 0;
-      if (r > h || (r == h && odd)) c += 1.f;
-      else if (r < -h || (r == -h && odd)) c -= 1.f;
-      q[i] = c;
-    }
+    float c = rintf(q[i]);
+    const float xs = x[i] * scale, b = d - xs;
+    const float lost = (xs - (d - b)) + (zs - b);  // x - z = d + lost exactly
+    // the remainder's distance above the upper border and below the lower one; both
+    // differences are exact near 0
+    const float r = fmaf(-c, u, d), h = 0.5f * u, above = (r - h) + lost, below = (r + h) + lost;
+    const bool odd = ((int)c & 1) != 0;
+    if (above > 0.f || (above == 0.f && odd)) c += 1.f;
+    else if (below < 0.f || (below == 0.f && odd)) c -= 1.f;
+    q[i] = c;
   }
   if (s < smallest_normal<T>()) {  // a step without all its bits: quotients may pass 15.5
 #pragma unroll
@@ -207,14 +239,14 @@ __device__ __forceinline__ uint32_t swap_halves(uint32_t w, bool odd) {
 
 // Work: 2 bytes read and 0.6 written a number, and some 20 instructions (minimum
 // and maximum, the quotient with its correction, rounding, packing), whose issue
-// bounds it (0.8 of the slots): 32 x 512 tokens x 16 heads of 128 in bf16 take about
-// 45 us, 3.9 TB/s, where the bytes alone take 27.
+// bounds it (0.8 of the slots): 32 x 512 tokens x 16 heads of 128 in bf16 take 47.4
+// us, 3.7 TB/s, where the bytes alone take 27.
 //
 // One thread: eight channels of one head, keys and values, of a run of a
 // request's tokens.  threadIdx.x (and blockIdx.y) = (head, group, quarter);
 // blockIdx.x = (request, run).
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 3)  // three blocks an SM (with 87 registers two fit: 54.6 us for 47.4)
     append_kernel(const T* __restrict__ k, long long ks0, long long ks1, long long ks2, const T* __restrict__ v,
                   long long vs0, long long vs1, long long vs2, const Pool p, const int32_t* __restrict__ slot_of,
                   const int32_t* __restrict__ start_pos, int tq, int run, int runs) {
@@ -262,8 +294,8 @@ __global__ void __launch_bounds__(256)
     const float k_half = fmaf(0.5f, k_hi, -0.5f * kz), v_half = fmaf(0.5f, v_hi, -0.5f * vz);
     uint32_t kw, vw;
     if (plain<T>(k_half) && plain<T>(v_half)) {
-      kw = quantise8_plain<T>(kf, k_half, kz, ks) & real;
-      vw = quantise8_plain<T>(vf, v_half, vz, vs) & real;
+      kw = quantise8_plain<T>(kf, k_half, kz, exact(kx, k_half, kz), ks) & real;
+      vw = quantise8_plain<T>(vf, v_half, vz, exact(vx, v_half, vz), vs) & real;
     } else {
       kw = quantise8<T>(kf, k_half, k_hi, ks, kz) & real;
       vw = quantise8<T>(vf, v_half, v_hi, vs, vz) & real;

@@ -327,3 +327,42 @@ def test_many_small_weights_beside_a_large_one_on_the_tensor_cores(cuda, dtype):
     pool, kx, vx = filled(cuda, k, v)
     got = ops.kv4_attention(q.to(cuda), pool, table([0] * b, cuda), table([n - t] * b, cuda))
     check(got[:1], q[:1], kx, vx, [n - t], dtype, True, rows=2)
+
+
+def borders(dtype):
+    """Groups [n, 32] whose numbers lie beside a border k + 1/2 by less than fp32 keeps
+    of x - min."""
+    far = {torch.bfloat16: 2.0 ** -40, torch.float16: 2.0 ** -23, torch.float32: 2.0 ** -40}[dtype]
+    groups = []
+    for sign in (1, -1):
+        g = torch.zeros(32, dtype=torch.float64)
+        g[0], g[1] = -7.5, 7.5  # step 1: 0 is a border
+        g[2], g[3], g[4] = sign * far, 0.5, -1.0
+        groups.append(g)
+        g = torch.arange(32).double() % 16 + 0.5  # step 1 from a minimum beside 0
+        g[0], g[1] = sign * far, 15.0
+        g[15] = 1.0
+        g = g.clamp(max=15.0)
+        g[16] = sign * far
+        groups.append(torch.where(g < 0, sign * far, g))
+        groups.append(g * 64)
+        groups.append(g.flip(0) / 8)
+    return torch.stack(groups).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_numbers_beside_a_border_by_less_than_fp32_keeps(cuda, dtype):
+    x = borders(dtype)
+    n = x.shape[0]
+    more = torch.randn(64, 32, generator=gen(1)).to(dtype)
+    more[:, ::3] *= torch.tensor(2.0 ** -12).to(dtype)
+    x = torch.cat([x, more]).view(1, n + 64, 1, 32)
+    k = torch.cat([x, x.roll(1, 1)], -1)  # two groups a row
+    pool = KV4Pool(slots=1, heads=1, max_seq_len=n + 64, head_dim=64, device=cuda, dtype=dtype)
+    zero = table([0], cuda)
+    ops.kv4_append(k.to(cuda), k.flip(-1).to(cuda), pool, zero, zero)
+    f = torch.finfo(dtype)
+    for got, src in zip(ops.kv4_read(pool, zero, n + 64), (k, k.flip(-1))):
+        want = orc.stands_for(src).transpose(1, 2)
+        got = got.cpu().double()
+        assert ((got - want).abs() <= (f.eps / 2 + 2.0 ** -24) * want.abs() + f.tiny * f.eps / 2).all()
