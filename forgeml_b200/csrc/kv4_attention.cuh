@@ -37,7 +37,7 @@ size_t tc_workspace_bytes(const Pool& p, int64_t batch, int64_t t, int64_t group
 int tc_attention(const Pool& p, Problem a, int dtype, cudaStream_t st);
 
 // Positions that request b's last query attends; 0 for a bad slot or position.
-__device__ __forceinline__ int keys_of(const Pool& p, const Problem& a, int b) {
+__host__ __device__ __forceinline__ int keys_of(const Pool& p, const Problem& a, int b) {
   const int slot = a.slot_of[b], start = a.start_pos[b];
   if (slot < 0 || slot >= p.slots || start < 0 || start >= p.max_seq) return 0;
   return min(start + a.tq, p.max_seq);
@@ -50,7 +50,7 @@ __device__ __forceinline__ int keys_of(const Pool& p, const Problem& a, int b) {
 template <int UNIT>
 struct Cursor {
   int b, seg, unit, keys, units;
-  __device__ __forceinline__ void request(const Pool& p, const Problem& a, int nb) {
+  __host__ __device__ __forceinline__ void request(const Pool& p, const Problem& a, int nb) {
     b = nb;
     keys = units = 0;
     while (b < a.B) {
@@ -60,7 +60,7 @@ struct Cursor {
       ++b;
     }
   }
-  __device__ __forceinline__ void next_segment(const Pool& p, const Problem& a) {
+  __host__ __device__ __forceinline__ void next_segment(const Pool& p, const Problem& a) {
     unit = 0;
     if (++seg == a.segs) {
       seg = 0;
@@ -68,7 +68,7 @@ struct Cursor {
     }
   }
   // The next unit; true when it opens another segment.
-  __device__ __forceinline__ bool next(const Pool& p, const Problem& a) {
+  __host__ __device__ __forceinline__ bool next(const Pool& p, const Problem& a) {
     if (unit + 1 < units) {
       ++unit;
       return false;
@@ -77,7 +77,7 @@ struct Cursor {
     return true;
   }
   // n units on.
-  __device__ __forceinline__ void skip(const Pool& p, const Problem& a, unsigned n) {
+  __host__ __device__ __forceinline__ void skip(const Pool& p, const Problem& a, unsigned n) {
     n += unit;
     while (b < a.B) {
       const unsigned here = (unsigned)(a.segs - seg) * units;
@@ -97,14 +97,14 @@ struct Cursor {
 // Contiguous shares of `total` units: part w of W begins at unit total * w / W.
 struct Shares {
   unsigned total, each, W, extra;
-  __device__ __forceinline__ Shares(unsigned total_, unsigned parts) : total(total_), W(parts) {
+  __host__ __device__ __forceinline__ Shares(unsigned total_, unsigned parts) : total(total_), W(parts) {
     each = total / W;
     extra = total - each * W;
   }
   // extra * w stays below W * W
-  __device__ __forceinline__ unsigned begin(unsigned w) const { return each * w + extra * w / W; }
+  __host__ __device__ __forceinline__ unsigned begin(unsigned w) const { return each * w + extra * w / W; }
   // The part that holds unit u, from part w on up or down.
-  __device__ __forceinline__ unsigned holder(unsigned u, unsigned w) const {
+  __host__ __device__ __forceinline__ unsigned holder(unsigned u, unsigned w) const {
     while (begin(w) > u) --w;
     while (w + 1 < W && begin(w + 1) <= u) ++w;
     return w;

@@ -37,14 +37,12 @@
 #include <string>
 #include <type_traits>
 
-#include "kv4_attention.cuh"
+#include "kv4_tc_walk.cuh"
 
 namespace fml {
 namespace kv4 {
 namespace tc {
 
-constexpr int kRows = 128;   // query rows of a segment
-constexpr int kBlock = 128;  // positions of a block
 constexpr int kThreads = 416;
 constexpr int kDequant = 8, kMma = 12;  // first warps of the roles
 // TMEM columns: two score blocks, the output, P and the queries (fp16 pairs).  P and
@@ -232,49 +230,6 @@ __device__ __forceinline__ uint32_t reads_nan(uint32_t sz) {
   return ((sz & (half ? 0x7c007c00u : 0x7f807f80u)) + (half ? 0x04000400u : 0x00800080u)) & 0x80008000u;
 }
 
-// A part of a segment: its blocks [lo, hi) (those that its rows attend at all).
-struct Part {
-  int b, h, row0, rows;  // rows of the request's head: row0 .. row0 + rows - 1
-  int start, kend;       // request's first position; positions that some row attends
-  int lo, hi;
-  bool whole;
-  unsigned seg0, units;  // in the batch's order: the segment's first unit, its units
-  int which;             // first or last part of the CTA's share
-};
-using BlockCursor = Cursor<kBlock>;
-// The parts that this CTA works through, in order; every role walks alike.
-struct Walk {
-  bool shared;
-  int row_tiles, left;
-  unsigned at, begin;
-  BlockCursor cur;
-  __device__ __forceinline__ bool next(const Pool& p, const Problem& a, Part& o) {
-    if (left == 0) return false;
-    const int n = shared ? min(cur.units - cur.unit, left) : 1;
-    const int rows = a.group * a.tq;
-    o.b = cur.b;
-    o.h = cur.seg / row_tiles;
-    o.row0 = (cur.seg - o.h * row_tiles) * kRows;
-    o.rows = min(kRows, rows - o.row0);
-    o.start = a.start_pos[cur.b];
-    o.kend = min(cur.keys, o.start + (o.row0 + o.rows - 1) / a.group + 1);
-    const int blocks = (o.kend + kBlock - 1) / kBlock;
-    o.lo = shared ? cur.unit : 0;
-    o.hi = shared ? max(o.lo, min(cur.unit + n, blocks)) : blocks;
-    o.whole = !shared || n == cur.units;
-    o.units = cur.units;
-    o.which = at == begin ? 0 : 1;
-    o.seg0 = at - cur.unit;
-    left -= n;
-    at += n;
-    if (shared) {
-      cur.unit += n;
-      if (cur.unit == cur.units) cur.next_segment(p, a);
-    }
-    return true;
-  }
-};
-
 template <typename T, int G>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_tc_kernel(const Pool p, const Problem a, const int row_tiles, const int shared_blocks) {
@@ -309,6 +264,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   pdl_trigger();
   // ---- this CTA's work
+  __shared__ unsigned taken_sh, took_sh, total_sh;  // tickets of a word; this CTA's parts that took theirs; the batch's units
+  __shared__ bool gave_up_sh;
+  if (threadIdx.x == 0) {
+    took_sh = 0;
+    gave_up_sh = false;
+  }
   Walk walk;
   walk.shared = shared_blocks != 0;
   walk.row_tiles = row_tiles;
@@ -318,6 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Plan<kBlock> plan(p, a);
     // a share of a few blocks at least: an empty one could not be joined
     shares = Shares(plan.total, min(gridDim.x, (plan.total + 1) / 2));
+    if (threadIdx.x == 0) total_sh = plan.total;
     walk.left = 0;
     if (plan.total > 0 && blockIdx.x < shares.W) {
       walk.begin = walk.at = shares.begin(blockIdx.x);
@@ -348,7 +310,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_holder) : "memory");
-  __shared__ unsigned taken_sh;
 
   Part part;
   if (warp == kMma) {
@@ -927,6 +888,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const unsigned taken = take_ticket(a.tickets + w0);
         if (taken == w1 - w0 + 1) a.tickets[w0] = 0;  // clean for the next launch
         taken_sh = taken;
+        took_sh |= 1u << part.which;
       }
       if (!together()) break;
       if (taken_sh == w1 - w0 + 1 && mine) {
@@ -965,12 +927,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       together();  // taken_sh is read
     }
+    if (!live && threadIdx.x == 0) gave_up_sh = true;
   }
   tc_fence_before();
   __syncthreads();
   if (warp == kMma) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
+  }
+  if (shared_blocks != 0 && threadIdx.x == 0 && gave_up_sh) {
+    // NaN for the CTA that joins what is missing; the error word is set
+    give_up(p, a, Shares(total_sh, min(gridDim.x, (total_sh + 1) / 2)), row_tiles, blockIdx.x, took_sh,
+            [&](const Part& o, unsigned w0) {
+              float* const own = a.ws + ((long long)blockIdx.x * 2 + o.which) * (kRows * (4 + D));
+              for (int i = 0; i < kRows; ++i) __stcg(reinterpret_cast<float4*>(own + i * (4 + D)), make_float4(NAN, NAN, 0.f, 0.f));
+              open_tickets(a.tickets + w0, a.launch);
+              return take_ticket(a.tickets + w0);
+            },
+            [&](unsigned w0) { a.tickets[w0] = 0; });
   }
 }
 
