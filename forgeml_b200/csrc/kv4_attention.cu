@@ -729,9 +729,10 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
     stage = stage == kStages - 1 ? 0 : stage + 1;
     }
 
-    // ---- the segment, or this share of it, ends
+    // ---- the segment, or this share of it, ends.  (Where a wait gave up, with NaN, and so do
+    // the share's other ones: whoever joins a segment counts every part's ticket.)
     flush(1.f);
-    l = warp_sum(l);
+    l = live ? warp_sum(l) : NAN;
     const bool whole = n_units == cur.units;
     const int which = left == share_units ? 0 : 1;
     float* own = parts + which * U::share;
@@ -770,7 +771,6 @@ __global__ void __launch_bounds__(Unit<T, G>::warps * 32, 1) attn_row_kernel(con
     }
     left -= n_units;
     cur = nxt;
-    if (!live) break;
   }
   // a wait gave up: let the copies in flight land before the warp exits
   if (!live)
