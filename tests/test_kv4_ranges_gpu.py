@@ -366,3 +366,18 @@ def test_numbers_beside_a_border_by_less_than_fp32_keeps(cuda, dtype):
         want = orc.stands_for(src).transpose(1, 2)
         got = got.cpu().double()
         assert ((got - want).abs() <= (f.eps / 2 + 2.0 ** -24) * want.abs() + f.tiny * f.eps / 2).all()
+
+
+def test_reading_and_attending_a_slot_twice_in_a_batch(cuda):
+    """Every row written, so that the numbers are compared."""
+    dtype, h, d, n = torch.float16, 3, 64, 40
+    k, v = (torch.randn(1, n, h, d, generator=gen(s)).to(dtype) for s in (1, 2))
+    pool, kx, vx = filled(cuda, k, v, slots=2)
+    for t in (1, 12):
+        q = torch.randn(1, t, h, d, generator=gen(3)).to(dtype)
+        got = ops.kv4_attention(q.expand(2, -1, -1, -1).contiguous().to(cuda), pool, table([0, 0], cuda),
+                                table([n - t] * 2, cuda))
+        for i in range(2):
+            check(got[i:i + 1], q, kx, vx, [n - t], dtype, t > 8)
+    kr, vr = ops.kv4_read(pool, table([0, 0], cuda), n)
+    assert torch.equal(kr[0], kr[1]) and torch.equal(vr[0], vr[1])
