@@ -17,15 +17,16 @@
 //               runs, O += P V into TMEM;
 //   warps 0-7   queries, softmax and epilogue: two threads a row, half of a block's
 //               positions (and of the output's channels) each, the scores read from
-//               TMEM once.
+//               TMEM once (blocks of numbers of very different sizes: position by
+//               position, see power_to_12).
 //
 // Rounded below fp32: the operands (keys, values) and P, to fp16, whose 11 bits cost
 // the output no more than its own rounding to the cache's type.
 //
-// Measured: 8 x 1000 tokens after 0 .. 1048 others, 16 heads of 128, bf16: 217 us,
-// 308 TFLOP/s; 16 requests of 4000 .. 8190 positions, 8 heads of 128 with 4 query
+// Measured: 8 x 1000 tokens after 0 .. 1048 others, 16 heads of 128, bf16: 224.6 us,
+// 299 TFLOP/s; 16 requests of 4000 .. 8190 positions, 8 heads of 128 with 4 query
 // heads each, go through the row kernel (tc_covers).  A block of 128 positions takes
-// about 4400 cycles, bound by the softmax warps' chain (scores from TMEM, maximum,
+// about 4600 cycles, bound by the softmax warps' chain (scores from TMEM, maximum,
 // exponentials, P to TMEM), with the dequantisation hidden behind it.
 //
 // Work: either one segment per CTA (prompts: enough segments), or, for few
@@ -65,7 +66,7 @@ struct Smem {
   static constexpr uint32_t rows = bars + 512;  // what a row's two threads tell each other: [2][2][128] fp32 pairs
   static constexpr uint32_t factors = rows + 4096;  // the tiles' keys' powers of two and values' exponents: [4 blocks][2][4]
   static constexpr uint32_t nans = factors + 128;   // first position whose value is NaN: [4 parts][4 tiles][8 groups]
-  static constexpr uint32_t own = nans + 512;  // positions' factors of their scores, values' exponents: [4 blocks][2][128] fp32
+  static constexpr uint32_t own = nans + 512;  // wide tiles' positions' factors of their scores, values' exponents: [4 blocks][2][128] fp32
   static constexpr uint32_t total = own + 4096 + 1024;  // 1024: alignment of the base
   static_assert(total <= 227 * 1024, "shared memory");
 };
@@ -178,8 +179,9 @@ __device__ __forceinline__ float power_to_12(float x) {
   const int e = __float_as_int(x) >> 23;
   return __int_as_float(max(1, min(253, 266 - e)) << 23);
 }
+__device__ __forceinline__ float exponent_of(float power) { return (float)((__float_as_int(power) >> 23) - 127); }
 constexpr float kTop = 14.f;  // log2 of the largest weight as the tensor cores get it
-constexpr float kWide = 1024.f;
+constexpr float kWide = 1024.f;  // (of fp16's 27 binades that leaves every position 17)
 // Scores from which on the rounding of their maximum shows in the weights.
 constexpr float kFar = 4194304.f;  // 2^22
 // What fp16's weights and their sum are taken against, for a maximum m: they go up to
@@ -425,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // bf16: powers of two of the tile, or of the lane's position
         bool wide = false;
-        float own[2], powers[2], exponent = 0.f;
+        float own[2], powers[2];
         float mine = 1.f;  // lane 0: the keys' power of two (-1: a wide tile), lane 1: the values' exponent
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
@@ -433,22 +435,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             float big = 0.f;
 #pragma unroll
             for (int i = 0; i < G; ++i) big = fmaxf(big, ok ? largest_of(sz[kv][i]) : 0.f);
-            const uint32_t bits = __float_as_uint(big);
-            const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, bits));
-            const float least = __uint_as_float(__reduce_min_sync(0xffffffffu, bits == 0 ? 0x7f800000u : bits));
-            wide |= most > least * kWide;
+            const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
+            wide |= big > 0.f && big * kWide < most;
             own[kv] = big;
             powers[kv] = power_to_12(most);
           }
-          if (wide)  // the same in every lane
+          wide = __any_sync(0xffffffffu, wide);
+          if (wide) {
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) powers[kv] = power_to_12(own[kv]);
+          }
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv)
 #pragma unroll
             for (int i = 0; i < G; ++i) sz[kv][i] = scaled_params<T>(sz[kv][i], powers[kv]);
-          exponent = (float)((__float_as_int(powers[1]) >> 23) - 127);
-          mine = lane == 0 ? (wide ? -1.f : powers[0]) : exponent;
+          mine = lane != 0 ? exponent_of(powers[1]) : wide ? -1.f : powers[0];
         }
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
@@ -461,10 +462,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           // keys' place is free once S of the block two before is done, which was issued
           // after the softmax of the block four before.
           if (kv == 0 && lane < 2) factors[(blk & 3) * 8 + 4 * lane + dw] = mine;
-          if (std::is_same<T, __nv_bfloat16>::value && kv == 0) {
+          if (kv == 0 && wide) {
             float* const at = reinterpret_cast<float*>(mem + L::own) + (blk & 3) * 2 * kBlock + row;
-            at[0] = wide ? __int_as_float((254 << 23) - __float_as_int(powers[0])) : 1.f;  // 1 / power
-            at[kBlock] = exponent;
+            at[0] = __int_as_float((254 << 23) - __float_as_int(powers[0]));  // 1 / power
+            at[kBlock] = exponent_of(powers[1]);
           }
           // likewise four parts': S of a part's first block is issued after the softmax's
           // warps have read all of the part before
@@ -696,20 +697,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float4 f4 = *reinterpret_cast<const float4*>(f);
         if (__any_sync(0xffffffffu, fminf(fminf(f4.x, f4.y), fminf(f4.z, f4.w)) < far_below)) {
           // A block with a wide tile, or with scores that could be far: position by position,
-          // the scores rounded before their maximum is taken.
+          // the scores rounded before their maximum is taken.  (Rolled, in a branch of its own:
+          // unrolled, or within the usual way, these lines cost blocks that do not take them up
+          // to 9 % of their time.)
           const float* const own = reinterpret_cast<const float*>(mem + L::own) + (blk & 3) * 2 * kBlock + 64 * hx;
           float mx = -INFINITY, at = -INFINITY, mn = m;
           if (any) {
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {
-              const float k = scale_of(c / 4);
+              const float k = scale_of(c / 4), tile = f[4 + 2 * hx + c / 4];
+              const bool wide = f[2 * hx + c / 4] < 0.f;
               float x[8];
               tmem_ld8(ts + 64 * hx + 8 * c, x);
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
-                x[e] = 64 * hx + 8 * c + e < lim ? __fmul_rn(kScaled ? x[e] * own[8 * c + e] : x[e], k) : -INFINITY;
+                x[e] = 64 * hx + 8 * c + e < lim ? __fmul_rn(wide ? x[e] * own[8 * c + e] : x[e], k) : -INFINITY;
                 mx = fmaxf(mx, x[e]);
-                if (kScaled) at = fmaxf(at, x[e] - own[kBlock + 8 * c + e]);
+                if (kScaled) at = fmaxf(at, x[e] - (wide ? own[kBlock + 8 * c + e] : tile));
               }
               tmem_st8(ts + 64 * hx + 8 * c, x);
             }
@@ -731,6 +735,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {
+              const float tile = f[4 + 2 * hx + c / 4];
+              const bool wide = f[2 * hx + c / 4] < 0.f;
               float x[8], p[8];
               tmem_ld8(ts + 64 * hx + 8 * c, x);
 #pragma unroll
@@ -738,7 +744,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 x[e] -= off;
                 p[e] = ex2(x[e]);
                 l += p[e];
-                if (kScaled) p[e] = ex2(fminf(x[e] - own[kBlock + 8 * c + e] + (kTop - wm), kTop + 1.f));
+                if (kScaled) p[e] = ex2(fminf(x[e] - (wide ? own[kBlock + 8 * c + e] : tile) + (kTop - wm), kTop + 1.f));
               }
               tmem_st4(trow + L::tm_p + 32 * hx + 4 * c,
                        {pack2<__half>(p[0], p[1]), pack2<__half>(p[2], p[3]), pack2<__half>(p[4], p[5]), pack2<__half>(p[6], p[7])});
@@ -986,13 +992,13 @@ static int launch_groups(const Pool& p, const Problem& a, int row_tiles, bool sh
 // key/value head.  Up to there the row kernel, which goes over the cache once per
 // row (from L2 after the first), is the faster one or near it.  Measured, row kernel
 // against this one, at 2 / 4 / 8 / 16 rows, head dim 128, bf16:
-//   16 requests x 8 heads x 6000 positions   47 / 77 / 139 / 262 against 117 .. 120 us
-//    2 requests x 8 heads x 6000             16 / 20 /  31 /  44 against  47 ..  51 us
-//    4 requests x 8 heads x 300               8 /  8 /  10 /  12 against  23 ..  24 us
-// and at 4 / 8 rows against 9 .. 32 rows here, other head dims, 16 requests x 8 heads:
-//   32 x 6000 positions  44 /  74 against  90 ..  93 us
-//   96 x 6000            66 / 115 against 104 .. 110
-//   256 x 3000           81 / 145 against 178 .. 184
+//   16 requests x 8 heads x 6000 positions   47 / 78 / 141 / 267 against 127 .. 130 us
+//    2 requests x 8 heads x 6000             17 / 21 /  32 /  46 against  49 ..  53 us
+//    4 requests x 8 heads x 300               9 /  9 /  10 /  13 against  25 ..  26 us
+// and at 4 / 8 / 16 rows, other head dims, 16 requests x 8 heads:
+//   32 x 6000 positions  44 /  75 / 137 against  92 ..  93 us
+//   96 x 6000            68 / 119 / 221 against 106 .. 109
+//   256 x 3000           89 / 158 / 301 against 177 .. 183
 // (The lengths, which decide where exactly the two meet, lie on the device.)
 bool tc_covers(const Pool& p, int dtype, int64_t t, int64_t group) {
   return (dtype == FML_BF16 || dtype == FML_F16) && t * group > 8;
