@@ -16,9 +16,9 @@
 // 44 us for 64 requests of 128 .. 2303 positions (8 heads of 128, bf16), 30 us now.
 //
 // Measured (bf16, heads of 128, device time):
-//   32 requests x 16 heads x 512 .. 639    17.4 us   2.7 TB/s of cache
-//   64 requests x  8 heads x 128 .. 2303   29.6 us   3.4
-//    1 request  x 16 heads x 100001        49.9 us   5.1
+//   32 requests x 16 heads x 512 .. 639    18.3 us   2.6 TB/s of cache
+//   64 requests x  8 heads x 128 .. 2303   30.2 us   3.3
+//    1 request  x 16 heads x 100001        50.4 us   5.1
 // Long streams come near the memory's rate; what is left of the shorter ones is
 // latency: about 2 us until the first copies are issued, 1 to 2 us for a segment's
 // query, flush and output, and the join where segments are split.

@@ -156,7 +156,9 @@ def kv4_attention(q: torch.Tensor, pool, slot_of: torch.Tensor, start_pos: torch
     """Masked attention of q [B,T,QH,D] over the quantised prefix: query t of
     request b sits at position start_pos[b]+t and attends rows 0 up to its own.
     QH is a multiple of the pool's heads; query head h reads head
-    h // (QH // heads).  Returns [B,T,QH*D]; scores, softmax and sums in fp32.
+    h // (QH // heads).  Returns [B,T,QH*D].  Scores, their maximum and the sums
+    are held in fp32; weights go as 16-bit (bf16) or 23-bit integers, for more
+    than 8 query rows of a head in 16-bit types as fp16 (include/forgeml_b200.h).
     A slot or position outside the pool gives zeros and raises the device
     error word's bit 4."""
     b = _kv4_tables(pool, slot_of, start_pos)

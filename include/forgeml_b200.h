@@ -274,11 +274,17 @@ FML_API int neb_kv4_read(const neb_kv4_pool* pool, const int32_t* slot_of, const
  * attends rows 0 .. start_pos[b]+t.  q is [B,T,q_heads,D] (dtype of the pool,
  * element strides, innermost 1), q_heads a multiple of the pool's heads: query
  * head h reads head h / (q_heads / heads).  out is [B,T,q_heads*D] contiguous.
- * scale is positive and finite.  Scores, softmax and the sums over the rows in
- * fp32; more than 8 query rows of a head (16-bit types) run on the
- * tensor cores with keys, values and weights rounded to fp16.  Queries without
- * a place in the pool give zeros and raise bit 4.  Rows past a query's position
- * count nothing, whatever they hold. */
+ * scale is positive and finite.  Scores, their maximum and the sums of weights
+ * and of the output are held in fp32 (fp32 pools: scores in 64 bits).  Rounded
+ * to fewer bits:
+ *   up to 8 query rows of a head, and fp32: the query to 27 bits below its
+ *     largest number; a weight times its group's step to 16 bits (bf16) or 23
+ *     below the largest such product so far, what is cut off going to a later
+ *     position;
+ *   more rows, 16-bit types (tensor cores): queries, keys, values and weights to
+ *     fp16's 11 bits, bf16's scaled by powers of two so that its range is kept.
+ * Queries without a place in the pool give zeros and raise bit 4.  Rows past a
+ * query's position count nothing, whatever they hold. */
 FML_API int neb_kv4_attention(const void* q, const int64_t q_strides[4], const neb_kv4_pool* pool,
                       const int32_t* slot_of, const int32_t* start_pos, void* out,
                       int64_t batch, int64_t t, int64_t q_heads, float scale,
