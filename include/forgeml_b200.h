@@ -278,9 +278,9 @@ FML_API int neb_kv4_read(const neb_kv4_pool* pool, const int32_t* slot_of, const
  * and of the output are held in fp32 (fp32 pools: scores in 64 bits).  Rounded
  * to fewer bits:
  *   up to 8 query rows of a head, and fp32: the query to 27 bits below its
- *     largest number; a weight times its group's step to 16 bits (bf16) or 23
- *     below the largest such product so far, what is cut off going to a later
- *     position;
+ *     largest number (or 2^-96, the larger); a weight times its group's step to
+ *     16 bits (bf16) or 23 below the largest such product so far, what is cut off
+ *     going to a later position;
  *   more rows, 16-bit types (tensor cores): queries, keys, values and weights to
  *     fp16's 11 bits, bf16's scaled by powers of two so that its range is kept.
  * Queries without a place in the pool give zeros and raise bit 4.  Rows past a
